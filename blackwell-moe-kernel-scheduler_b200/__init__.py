@@ -6,6 +6,8 @@ Sub-modules:
   planner   host planning interface (spec, worklist plan, claims, dispatch)
   engine    grouped-GEMM plan, device worklist builder, scheduler probe
   runner    correctness + CUDA-event benchmark harness (reference CSV schema), cli
+  layer     operators either side of the GEMM: router choice, row quantiser, and the
+            whole expert layer for a few tokens
   ep        expert-parallel layer (torch.distributed all-to-all)
   ep_peer   expert-parallel layer over peer memory (two routing kernels)
   ep_fused  expert-parallel layer whose exchange overlaps the grouped GEMM
@@ -45,6 +47,13 @@ from .engine import (  # noqa: F401
     read_worklist_arrays,
     tiles_to_numpy,
     worklist_layout,
+)
+
+from .layer import (  # noqa: F401
+    moe_decode,
+    moe_decode_workspace,
+    quantize_rows,
+    route_topk,
 )
 
 __all__ = [name for name in dir() if not name.startswith("_")]

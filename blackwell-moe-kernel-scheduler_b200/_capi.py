@@ -54,6 +54,20 @@ ORDER_SORTED_BY_WORK = 1
 RASTER_N_FASTEST = 0
 RASTER_M_FASTEST = 1
 
+# Operand element types (bmoe_data_type; 2 is unused).
+TYPE_BF16 = 0
+TYPE_FP8_E4M3 = 1
+TYPE_INT8 = 3
+TYPE_FP32 = 4
+INT8_MAX_K = 131071
+
+SCORINGS = {"softmax": 0, "sigmoid": 1}
+ROUTE_MAX_EXPERTS = 1024
+ROUTE_MAX_TOP_K = 32
+MOE_DECODE_MAX_TOKENS = 64
+MOE_DECODE_MAX_TOP_K = 32
+MOE_DECODE_MAX_EXPERTS = 1024
+
 DISTRIBUTIONS = {"uniform": 0, "heavy_hitter": 1, "heavy": 1, "sparse": 2, "zipf": 3,
                  "heavy_sparse": 4}
 
@@ -281,6 +295,40 @@ class GemmArgs(C.Structure):
         ("results_pushed", C.c_uint32),
         ("reserved0", C.c_uint32),
         ("tokens_per_expert_dev", C.c_void_p),
+        ("row_scale", C.POINTER(C.c_void_p)),
+        ("col_scale", C.POINTER(C.c_void_p)),
+        ("packed_row_scale", C.c_void_p),
+    ]
+
+
+class RouteTopkArgs(C.Structure):
+    _fields_ = [
+        ("logits_dev", C.c_void_p), ("bias_dev", C.c_void_p), ("expert_ids_dev", C.c_void_p),
+        ("weights_dev", C.c_void_p), ("tokens", C.c_uint64), ("row_stride", C.c_uint64),
+        ("experts", C.c_uint32), ("top_k", C.c_uint32), ("logits_type", C.c_uint32),
+        ("scoring", C.c_uint32), ("renormalize", C.c_uint32), ("scale", C.c_float),
+        ("stream", C.c_void_p),
+    ]
+
+
+class QuantizeRowsArgs(C.Structure):
+    _fields_ = [
+        ("src_dev", C.c_void_p), ("index_dev", C.c_void_p), ("dst_dev", C.c_void_p),
+        ("scale_dev", C.c_void_p), ("rows", C.c_uint64), ("src_rows", C.c_uint64),
+        ("src_stride", C.c_uint64), ("cols", C.c_uint32), ("src_type", C.c_uint32),
+        ("stream", C.c_void_p),
+    ]
+
+
+class MoeDecodeArgs(C.Structure):
+    _fields_ = [
+        ("x_dev", C.c_void_p), ("w_gate_up_dev", C.c_void_p), ("w_down_dev", C.c_void_p),
+        ("gate_up_scale_dev", C.c_void_p), ("down_scale_dev", C.c_void_p),
+        ("expert_ids_dev", C.c_void_p), ("weights_dev", C.c_void_p), ("out_dev", C.c_void_p),
+        ("workspace_dev", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("tokens", C.c_uint32), ("top_k", C.c_uint32), ("experts", C.c_uint32),
+        ("hidden", C.c_uint32), ("inter", C.c_uint32), ("data_type", C.c_uint32),
+        ("stream", C.c_void_p),
     ]
 
 
@@ -405,6 +453,10 @@ SIGNATURES = {
         [C.c_void_p, C.c_uint32, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64,
          C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32, C.c_void_p],
     ),
+    "bmoe_route_topk": (C.c_int, [_P(RouteTopkArgs)]),
+    "bmoe_quantize_rows": (C.c_int, [_P(QuantizeRowsArgs)]),
+    "bmoe_moe_decode_workspace": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint32]),
+    "bmoe_moe_decode": (C.c_int, [_P(MoeDecodeArgs)]),
     "bmoe_ep_count": (
         C.c_int,
         [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p,

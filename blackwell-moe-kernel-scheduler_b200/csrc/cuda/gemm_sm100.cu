@@ -1,4 +1,4 @@
-// Persistent, warp-specialised BF16 (and FP8 E4M3) grouped GEMM for sm_100a.
+// Persistent, warp-specialised BF16 (and FP8 E4M3, INT8) grouped GEMM for sm_100a.
 //
 // One CTA (256 threads) per SM walks a device worklist of 20-byte tile records
 // and computes, per record, a 128 x TILE_N block (one CTA) or a 256 x TILE_N
@@ -112,9 +112,27 @@ __device__ __forceinline__ void report(const GemmParams& p, uint32_t site,
   }
 }
 
+// Four integer sums of one row -> FP32 bit patterns, scaled by row and channel; columns
+// beyond the tile's valid ones have no scale and are never stored.
+__device__ __forceinline__ void scale_int32x4(uint32_t (&v)[32], uint32_t j, float row_scale,
+                                              const float* col_scale, uint32_t col,
+                                              uint32_t valid_n) {
+  if (col >= valid_n) return;
+  const float4 s = __ldg(reinterpret_cast<const float4*>(col_scale + col));
+  v[j + 0] = __float_as_uint(__int2float_rn(static_cast<int>(v[j + 0])) * (row_scale * s.x));
+  v[j + 1] = __float_as_uint(__int2float_rn(static_cast<int>(v[j + 1])) * (row_scale * s.y));
+  v[j + 2] = __float_as_uint(__int2float_rn(static_cast<int>(v[j + 2])) * (row_scale * s.z));
+  v[j + 3] = __float_as_uint(__int2float_rn(static_cast<int>(v[j + 3])) * (row_scale * s.w));
+}
+
 // OUT_F32 = true writes the FP32 accumulators unrounded (row-major FP32 D) instead
-// of BF16; everything up to the epilogue is identical.
-template <uint32_t TILE_N, bool PAIR, bool OUT_F32>
+// of BF16; everything up to the epilogue is identical. INT8 = true multiplies signed bytes
+// (kind::i8: exact 32-bit sums) and scales them by row and output channel in the epilogue:
+//     D[m, n] = float(sum_k A[m, k] B[n, k]) * (row_scale[m] * col_scale[n])
+// A lane of the epilogue holds one row, so the row scale is one register; the channel scales
+// of a chunk are read as broadcast 16-byte loads (16 per 64 columns, in L1 after the first
+// tile of a column block).
+template <uint32_t TILE_N, bool PAIR, bool OUT_F32, bool INT8>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_gemm_kernel(const __grid_constant__ GemmParams p) {
   using Cfg = Config<TILE_N, PAIR>;
@@ -483,7 +501,7 @@ grouped_gemm_kernel(const __grid_constant__ GemmParams p) {
     uint64_t t_info = 0, t_stage = 0;
     // bytes that land per stage: the A box (possibly fewer than 128 rows) and the B box
     const uint32_t tx_bytes = (p.a_box_bytes + Cfg::kBBytes) * Cfg::kGroup;
-    const uint32_t k_block_elems = p.fp8 != 0 ? 2 * kBlockK : kBlockK;   // 128 bytes of a row
+    const uint32_t k_block_elems = p.byte_operands != 0 ? 2 * kBlockK : kBlockK;   // 128 bytes of a row
     while (true) {
       const uint32_t slot = reads % kSchedSlots;
       const uint32_t round = (reads / kSchedSlots) & 1u;
@@ -561,7 +579,8 @@ grouped_gemm_kernel(const __grid_constant__ GemmParams p) {
     if (leader) {
       constexpr uint32_t idesc = ptx::make_bf16_idesc(kCtaRows * Cfg::kGroup, TILE_N);
       constexpr uint32_t idesc_fp8 = ptx::make_e4m3_idesc(kCtaRows * Cfg::kGroup, TILE_N);
-      const bool fp8 = p.fp8 != 0;
+      constexpr uint32_t idesc_s8 = ptx::make_s8_idesc(kCtaRows * Cfg::kGroup, TILE_N);
+      const bool fp8 = !INT8 && p.byte_operands != 0;
       uint32_t reads = 0;
       uint32_t stage = 0, stage_round = 0;
       uint32_t buf = 0, buf_round = 0;
@@ -606,7 +625,18 @@ grouped_gemm_kernel(const __grid_constant__ GemmParams p) {
               ptx::make_kmajor_sw128_desc(base + Cfg::kOffB + stage * Cfg::kBBytes);
           const long long issue_t0 = tracing ? clock64() : 0;
           if (ptx::elect_one()) {
-            if (!fp8) {
+            if constexpr (INT8) {
+#pragma unroll
+              for (uint32_t ks = 0; ks < kBlockK / 16; ++ks) {
+                // 32 bytes of a row, as for FP8.
+                const uint32_t acc = (kb | ks) != 0 ? 1u : 0u;
+                if constexpr (PAIR) {
+                  ptx::umma_s8_ss_pair(d_tmem, a_desc + 2 * ks, b_desc + 2 * ks, idesc_s8, acc);
+                } else {
+                  ptx::umma_s8_ss(d_tmem, a_desc + 2 * ks, b_desc + 2 * ks, idesc_s8, acc);
+                }
+              }
+            } else if (!fp8) {
 #pragma unroll
               for (uint32_t ks = 0; ks < kBlockK / 16; ++ks) {
                 // 16 BF16 = 32 bytes along k inside the 128-byte swizzle row.
@@ -791,6 +821,19 @@ grouped_gemm_kernel(const __grid_constant__ GemmParams p) {
         }
       }
 
+      // INT8: the scale of this lane's row and the tile's channel scales.
+      float row_scale = 0.0f;
+      const float* col_scale = nullptr;
+      if constexpr (INT8) {
+        if (row_in_tile + lane < valid_m) {
+          const uint32_t row = row0 + row_in_tile + lane;
+          row_scale = p.a_row_offsets != nullptr
+                          ? p.packed_row_scale[p.a_row_offsets[expert] + row]
+                          : p.row_scale[expert][row];
+        }
+        col_scale = p.col_scale[expert] + col0;
+      }
+
       if (!timed_wait(bar_tmem_full(buf), buf_round, t_accum)) {
         if (lane == 0 && quad == 0) {
           report(p, kSiteEpiAccum, 3, static_cast<uint32_t>(tile), buf, 0);
@@ -821,6 +864,19 @@ grouped_gemm_kernel(const __grid_constant__ GemmParams p) {
           ptx::tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) arrive_at_leader(bar_tmem_empty(buf));
+        }
+        if constexpr (INT8) {
+          // n is a multiple of 8: four columns are all inside or all outside
+#pragma unroll
+          for (uint32_t j = 0; j < 32; j += 4) {
+            scale_int32x4(lo, j, row_scale, col_scale, c * kChunkCols + j, valid_n);
+          }
+          if constexpr (!OUT_F32) {
+#pragma unroll
+            for (uint32_t j = 0; j < 32; j += 4) {
+              scale_int32x4(hi, j, row_scale, col_scale, c * kChunkCols + 32 + j, valid_n);
+            }
+          }
         }
         // The store issued two chunks ago read from this staging buffer.
         if (lane == 0) ptx::tma_store_wait_read<1>();
@@ -956,7 +1012,7 @@ grouped_gemm_kernel(const __grid_constant__ GemmParams p) {
   }
 }
 
-template <uint32_t TILE_N, bool PAIR, bool OUT_F32>
+template <uint32_t TILE_N, bool PAIR, bool OUT_F32, bool INT8>
 cudaError_t launch_impl(const GemmParams& params, uint32_t units, cudaStream_t stream) {
   using Cfg = Config<TILE_N, PAIR>;
   // The opt-in shared-memory size is a per-device function attribute.
@@ -965,7 +1021,7 @@ cudaError_t launch_impl(const GemmParams& params, uint32_t units, cudaStream_t s
   cudaError_t err = cudaGetDevice(&device);
   if (err != cudaSuccess) return err;
   if (device < 0 || device >= 64 || !configured[device]) {
-    err = cudaFuncSetAttribute(grouped_gemm_kernel<TILE_N, PAIR, OUT_F32>,
+    err = cudaFuncSetAttribute(grouped_gemm_kernel<TILE_N, PAIR, OUT_F32, INT8>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(Cfg::kDynamicSmem));
     if (err != cudaSuccess) return err;
@@ -983,7 +1039,7 @@ cudaError_t launch_impl(const GemmParams& params, uint32_t units, cudaStream_t s
   attribute[0].val.clusterDim.z = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
-  err = cudaLaunchKernelEx(&config, grouped_gemm_kernel<TILE_N, PAIR, OUT_F32>, params);
+  err = cudaLaunchKernelEx(&config, grouped_gemm_kernel<TILE_N, PAIR, OUT_F32, INT8>, params);
   return err != cudaSuccess ? err : cudaPeekAtLastError();
 }
 
@@ -1001,30 +1057,59 @@ uint32_t gemm_stage_count(uint32_t tile_n, uint32_t cta_group) {
   return tile_n == 256 ? Config<256, false>::kStages : Config<128, false>::kStages;
 }
 
-cudaError_t preload_gemm_kernels() {
-  cudaError_t rc = preload_one(grouped_gemm_kernel<256, true, false>);
-  if (rc == cudaSuccess) rc = preload_one(grouped_gemm_kernel<256, false, false>);
-  if (rc == cudaSuccess) rc = preload_one(grouped_gemm_kernel<128, false, false>);
-  if (rc == cudaSuccess) rc = preload_one(grouped_gemm_kernel<64, false, false>);
-  if (rc == cudaSuccess) rc = preload_one(grouped_gemm_kernel<256, true, true>);
-  if (rc == cudaSuccess) rc = preload_one(grouped_gemm_kernel<256, false, true>);
+namespace {
+
+template <bool INT8>
+cudaError_t preload_gemm_type() {
+  cudaError_t rc = preload_one(grouped_gemm_kernel<256, true, false, INT8>);
+  if (rc == cudaSuccess) rc = preload_one(grouped_gemm_kernel<256, false, false, INT8>);
+  if (rc == cudaSuccess) rc = preload_one(grouped_gemm_kernel<128, false, false, INT8>);
+  if (rc == cudaSuccess) rc = preload_one(grouped_gemm_kernel<64, false, false, INT8>);
+  if (rc == cudaSuccess) rc = preload_one(grouped_gemm_kernel<256, true, true, INT8>);
+  if (rc == cudaSuccess) rc = preload_one(grouped_gemm_kernel<256, false, true, INT8>);
   return rc;
 }
 
-cudaError_t launch_grouped_gemm(const GemmParams& params, uint32_t tile_n,
-                                uint32_t cta_group, bool out_f32, uint32_t units,
-                                cudaStream_t stream) {
-  if (units == 0) return cudaSuccess;
+template <bool INT8>
+cudaError_t launch_typed(const GemmParams& params, uint32_t tile_n, uint32_t cta_group,
+                         bool out_f32, uint32_t units, cudaStream_t stream) {
   if (out_f32) {
-    if (cta_group == 2 && tile_n == 256) return launch_impl<256, true, true>(params, units, stream);
-    if (cta_group == 1 && tile_n == 256) return launch_impl<256, false, true>(params, units, stream);
+    if (cta_group == 2 && tile_n == 256) {
+      return launch_impl<256, true, true, INT8>(params, units, stream);
+    }
+    if (cta_group == 1 && tile_n == 256) {
+      return launch_impl<256, false, true, INT8>(params, units, stream);
+    }
     return cudaErrorInvalidValue;
   }
-  if (cta_group == 2 && tile_n == 256) return launch_impl<256, true, false>(params, units, stream);
-  if (cta_group == 1 && tile_n == 256) return launch_impl<256, false, false>(params, units, stream);
-  if (cta_group == 1 && tile_n == 128) return launch_impl<128, false, false>(params, units, stream);
-  if (cta_group == 1 && tile_n == 64) return launch_impl<64, false, false>(params, units, stream);
+  if (cta_group == 2 && tile_n == 256) {
+    return launch_impl<256, true, false, INT8>(params, units, stream);
+  }
+  if (cta_group == 1 && tile_n == 256) {
+    return launch_impl<256, false, false, INT8>(params, units, stream);
+  }
+  if (cta_group == 1 && tile_n == 128) {
+    return launch_impl<128, false, false, INT8>(params, units, stream);
+  }
+  if (cta_group == 1 && tile_n == 64) {
+    return launch_impl<64, false, false, INT8>(params, units, stream);
+  }
   return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t preload_gemm_kernels() {
+  const cudaError_t rc = preload_gemm_type<false>();
+  return rc == cudaSuccess ? preload_gemm_type<true>() : rc;
+}
+
+cudaError_t launch_grouped_gemm(const GemmParams& params, uint32_t tile_n,
+                                uint32_t cta_group, bool out_f32, bool int8, uint32_t units,
+                                cudaStream_t stream) {
+  if (units == 0) return cudaSuccess;
+  return int8 ? launch_typed<true>(params, tile_n, cta_group, out_f32, units, stream)
+              : launch_typed<false>(params, tile_n, cta_group, out_f32, units, stream);
 }
 
 }  // namespace bmoe

@@ -132,11 +132,18 @@ struct GemmParams {
   // about 64 bytes per cycle, zero-filled rows included, and that - not HBM or the tensor
   // pipe - bounds a one-wave launch over a small-M problem.
   uint32_t a_box_bytes;
-  // Operand type: 0 = BF16 (k-block = 64 elements, kind::f16), 1 = FP8 E4M3 (k-block =
-  // 128 elements, kind::f8f6f4). A k-block is 128 bytes of a row either way and one MMA
-  // instruction covers 32 of them, so the shared-memory layout, the descriptors and the
-  // pipeline are the same; only the tensor maps, k_blocks and the instruction differ.
-  uint32_t fp8;
+  // Operand width: 0 = BF16 (k-block = 64 elements, kind::f16), 1 = one byte per element
+  // (k-block = 128 elements): FP8 E4M3 (kind::f8f6f4), or signed integers in the INT8
+  // instantiation of the kernel (kind::i8). A k-block is 128 bytes of a row either way and
+  // one MMA instruction covers 32 of them, so the shared-memory layout, the descriptors and
+  // the pipeline are the same; only the tensor maps, k_blocks and the instruction differ.
+  uint32_t byte_operands;
+  // INT8 only: scale of every row of A and of every output channel. row_scale[e] holds
+  // the expert's rows; with a packed A it is nullptr and packed_row_scale is indexed by the
+  // packed row. col_scale[e] holds n floats, 16-byte aligned.
+  const float* const* row_scale;
+  const float* const* col_scale;
+  const float* packed_row_scale;
   // Extents for the -DBMOE_CHECKS build (always filled in by the plan, read by that build only).
   uint32_t check_experts;
   uint32_t check_n;
@@ -164,9 +171,9 @@ uint32_t gemm_stage_count(uint32_t tile_n, uint32_t cta_group);
 
 // Enqueues the kernel on `units` scheduling units: persistent CTAs (or CTA
 // pairs), or the tile count for CLC. The grid is units * cta_group CTAs.
-// out_f32 selects the FP32-output epilogue (tile_n 256 only).
+// out_f32 selects the FP32-output epilogue (tile_n 256 only), int8 the integer product.
 cudaError_t launch_grouped_gemm(const GemmParams& params, uint32_t tile_n,
-                                uint32_t cta_group, bool out_f32, uint32_t units,
+                                uint32_t cta_group, bool out_f32, bool int8, uint32_t units,
                                 cudaStream_t stream);
 
 }  // namespace bmoe

@@ -147,6 +147,7 @@ struct bmoe_plan {
   uint32_t stats_n = 0;    // output columns of the current problem
   uint32_t cta_group = 1;
   bool out_f32 = false;
+  bool int8 = false;
 
   void release_all() {
     meta.release();
@@ -270,11 +271,20 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
   }
   if (packed && (misaligned16(a.packed_a) || a.packed_rows == 0)) return BMOE_INVALID_ARGUMENT;
   if (pushed && a.output_f32 != 0) return BMOE_INVALID_ARGUMENT;
-  if (a.data_type > 1) return BMOE_UNSUPPORTED_DATA_TYPE;
-  // FP8 E4M3 operands: a row is k bytes, and a tensor map wants row strides of 16 bytes
-  const bool fp8 = a.data_type == 1;
-  if (fp8 && a.k % 16 != 0) return BMOE_INVALID_ARGUMENT;
-  const Elem operand = fp8 ? Elem::kByte : Elem::kBf16;
+  if (a.data_type != BMOE_TYPE_BF16 && a.data_type != BMOE_TYPE_FP8_E4M3 &&
+      a.data_type != BMOE_TYPE_INT8) {
+    return BMOE_UNSUPPORTED_DATA_TYPE;
+  }
+  // One byte per element: a row is k bytes, and a tensor map wants row strides of 16 bytes
+  const bool int8 = a.data_type == BMOE_TYPE_INT8;
+  const bool bytes = int8 || a.data_type == BMOE_TYPE_FP8_E4M3;
+  if (bytes && a.k % 16 != 0) return BMOE_INVALID_ARGUMENT;
+  // INT8: a scale per row and per channel, sums that cannot pass 2^31
+  if (int8 && (a.k > BMOE_INT8_MAX_K || a.col_scale == nullptr ||
+               (packed ? a.packed_row_scale == nullptr : a.row_scale == nullptr))) {
+    return BMOE_INVALID_ARGUMENT;
+  }
+  const Elem operand = bytes ? Elem::kByte : Elem::kBf16;
   if (a.scheduler > BMOE_SCHED_CLC) return BMOE_UNSUPPORTED_SCHEDULER;
   if (a.experts > BMOE_WORKLIST_MAX_EXPERTS) return BMOE_INVALID_ARGUMENT;
   if (a.tile_n != 0 && a.tile_n != 64 && a.tile_n != 128 && a.tile_n != 256) {
@@ -308,6 +318,10 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
     if (host_counts[e] == 0) continue;
     if ((!packed && (a.a[e] == nullptr || misaligned16(a.a[e]))) || a.b[e] == nullptr ||
         misaligned16(a.b[e]) || (!pushed && (a.d[e] == nullptr || misaligned16(a.d[e])))) {
+      return BMOE_INVALID_ARGUMENT;
+    }
+    if (int8 && (a.col_scale[e] == nullptr || misaligned16(a.col_scale[e]) ||
+                 (!packed && a.row_scale[e] == nullptr))) {
       return BMOE_INVALID_ARGUMENT;
     }
     routed_rows += host_counts[e];
@@ -389,7 +403,10 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
   const size_t map_bytes = sizeof(CUtensorMap) * 3 * static_cast<size_t>(a.experts);
   const size_t off_counts = 512;
   const size_t off_maps = (off_counts + sizeof(uint32_t) * a.experts + 127) / 128 * 128;
-  const size_t meta_bytes = off_maps + map_bytes;
+  // INT8: row and channel scale pointers [2][experts] behind the maps
+  const size_t off_scales = off_maps + map_bytes;
+  const size_t meta_bytes =
+      off_scales + (int8 ? 2 * sizeof(float*) * static_cast<size_t>(a.experts) : 0);
   const void* const staging_before = plan->staging.ptr;
   if (!plan->meta.reserve(meta_bytes) || !plan->staging.reserve(meta_bytes) ||
       !plan->worklist.reserve(sizeof(bmoe_tile) * static_cast<size_t>(tiles)) ||
@@ -468,6 +485,14 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
       return BMOE_CUDA_ERROR;
     }
   }
+  if (int8) {
+    const float** const scales = reinterpret_cast<const float**>(stage + off_scales);
+    for (uint32_t e = 0; e < a.experts; ++e) {
+      const bool live = host_counts[e] != 0;
+      scales[e] = live && !packed ? a.row_scale[e] : nullptr;
+      scales[a.experts + e] = live ? a.col_scale[e] : nullptr;
+    }
+  }
   if (cudaMemcpyAsync(meta, stage, meta_bytes, cudaMemcpyHostToDevice, stream) != cudaSuccess) {
     return BMOE_CUDA_ERROR;
   }
@@ -497,11 +522,16 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
   p.tmap_d = dev_maps + 2 * static_cast<size_t>(a.experts);
   p.tiles = static_cast<const bmoe_tile*>(plan->worklist.ptr);
   p.tile_count = tiles;
-  p.k_blocks = fp8 ? (a.k + 127) / 128 : (a.k + 63) / 64;   // 128 bytes of a row each
-  p.fp8 = fp8 ? 1u : 0u;
+  p.k_blocks = bytes ? (a.k + 127) / 128 : (a.k + 63) / 64;   // 128 bytes of a row each
+  p.byte_operands = bytes ? 1u : 0u;
+  if (int8) {
+    p.row_scale = reinterpret_cast<const float* const*>(meta + off_scales);
+    p.col_scale = p.row_scale + a.experts;
+    p.packed_row_scale = packed ? a.packed_row_scale : nullptr;
+  }
   p.check_experts = a.experts;
   p.check_n = a.n;
-  p.check_k_bytes = fp8 ? a.k : 2u * a.k;
+  p.check_k_bytes = bytes ? a.k : 2u * a.k;
   p.check_a_rows = packed ? a.packed_rows : 0;
   p.sched_mode = policy.sched_mode;
   p.claim_size = policy.claim_size;
@@ -530,6 +560,7 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
   plan->stats_n = a.n;
   plan->cta_group = cta_group;
   plan->out_f32 = out_f32;
+  plan->int8 = int8;
   plan->units = policy.one_cta_per_tile ? tiles : (tiles < unit_budget ? tiles : unit_budget);
   if (dev_counts) plan->units = unit_budget;   // the tile total is not known here
 
@@ -557,6 +588,9 @@ int bmoe_preload_kernels(void) {
   if (rc == cudaSuccess) rc = bmoe::preload_permute_kernels();
   if (rc == cudaSuccess) rc = bmoe::preload_exchange_kernels();
   if (rc == cudaSuccess) rc = bmoe::preload_probe_kernels();
+  if (rc == cudaSuccess) rc = bmoe::preload_router_kernels();
+  if (rc == cudaSuccess) rc = bmoe::preload_quantize_kernels();
+  if (rc == cudaSuccess) rc = bmoe::preload_decode_kernels();
   return rc == cudaSuccess ? BMOE_OK : BMOE_CUDA_ERROR;
 }
 
@@ -652,7 +686,7 @@ int bmoe_plan_run(bmoe_plan* plan, void* stream) {
   }
   const cudaError_t err =
       bmoe::launch_grouped_gemm(plan->params, plan->tile_n, plan->cta_group, plan->out_f32,
-                                plan->units, s);
+                                plan->int8, plan->units, s);
   plan->last_stream = s;
   if (err != cudaSuccess) return BMOE_CUDA_ERROR;
   plan->stats.launches += 1;

@@ -14,6 +14,9 @@ cudaError_t preload_worklist_kernels();
 cudaError_t preload_permute_kernels();
 cudaError_t preload_exchange_kernels();
 cudaError_t preload_probe_kernels();
+cudaError_t preload_router_kernels();
+cudaError_t preload_quantize_kernels();
+cudaError_t preload_decode_kernels();
 
 // SM count of the current device (148 on B200; partitions and other parts differ).
 inline uint32_t device_sm_count() {

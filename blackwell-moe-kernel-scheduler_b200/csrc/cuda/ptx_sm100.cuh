@@ -313,6 +313,26 @@ __device__ __forceinline__ void umma_e4m3_ss(uint32_t d_tmem, uint64_t a_desc,
       : "memory");
 }
 
+// Instruction descriptor for kind::i8 with both operands signed 8-bit integers (format
+// code 1), 32-bit integer accumulation (D format 2), no saturation; the other fields as for
+// kind::f16. One instruction covers K = 32 elements.
+__host__ __device__ constexpr uint32_t make_s8_idesc(uint32_t m, uint32_t n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// D[tmem] (+)= A[smem] * B[smem]^T for one K=32 slice of signed 8-bit operands.
+__device__ __forceinline__ void umma_s8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrives on `bar` once all tcgen05.mma issued so far by this thread finished.
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile(
@@ -475,6 +495,20 @@ __device__ __forceinline__ void umma_e4m3_ss_pair(uint32_t d_tmem, uint64_t a_de
       ".reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The same for signed 8-bit operands (K = 32 per instruction).
+__device__ __forceinline__ void umma_s8_ss_pair(uint32_t d_tmem, uint64_t a_desc,
+                                                uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
       "}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");

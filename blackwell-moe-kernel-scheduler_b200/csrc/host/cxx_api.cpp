@@ -34,6 +34,8 @@ bmoe_gemm_args to_c_args(const GroupedGemmArguments& args) {
   c.raster_along_m = args.raster_along_m;
   c.output_f32 = 0;
   c.stream = args.stream;
+  c.row_scale = args.row_scale;
+  c.col_scale = args.col_scale;
   return c;
 }
 
@@ -73,6 +75,15 @@ KernelStatus Bf16GroupedGemmPlan::initialize(const GroupedGemmArguments& args) {
 
 KernelStatus Fp8E4m3GroupedGemmPlan::initialize(const GroupedGemmArguments& args) {
   if (args.data_type != DataType::kFp8E4M3) {
+    GroupedGemmArguments probe = args;
+    probe.data_type = static_cast<DataType>(0x7fffffff);
+    return plan_.initialize_typed(probe);
+  }
+  return plan_.initialize_typed(args);
+}
+
+KernelStatus Int8GroupedGemmPlan::initialize(const GroupedGemmArguments& args) {
+  if (args.data_type != DataType::kInt8) {
     GroupedGemmArguments probe = args;
     probe.data_type = static_cast<DataType>(0x7fffffff);
     return plan_.initialize_typed(probe);

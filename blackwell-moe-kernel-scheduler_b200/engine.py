@@ -44,6 +44,39 @@ def tiles_to_numpy(tiles, count: int) -> np.ndarray:
     return raw.copy()
 
 
+def _byte_type(a, w) -> int:
+    """Operand type of one-byte tensors: INT8 when both are ``torch.int8``, FP8 E4M3 bytes
+    (``torch.float8_e4m3fn`` or ``uint8``) when neither is; -1 for a mixture."""
+    import torch
+
+    signed = (a.dtype is torch.int8, w.dtype is torch.int8)
+    if signed == (True, True):
+        return _capi.TYPE_INT8
+    return _capi.TYPE_FP8_E4M3 if signed == (False, False) else -1
+
+
+def _scales_fit(data_type, a, w, row_scale, col_scale) -> bool:
+    """Scales are there exactly for INT8 operands: FP32, one per row of ``a`` and one per
+    (expert, output channel)."""
+    import torch
+
+    if data_type != _capi.TYPE_INT8:
+        return data_type != -1 and row_scale is None and col_scale is None
+    return (row_scale is not None and col_scale is not None
+            and row_scale.dtype is torch.float32 and col_scale.dtype is torch.float32
+            and row_scale.device == a.device and col_scale.device == a.device
+            and row_scale.is_contiguous() and col_scale.is_contiguous()
+            and row_scale.numel() >= int(a.shape[0])
+            and tuple(col_scale.shape) == tuple(w.shape[:2]))
+
+
+def _expert_pointers(per_expert) -> np.ndarray:
+    """Address of every expert's slice of a contiguous FP32 tensor [experts, n]."""
+    experts, n = int(per_expert.shape[0]), int(per_expert.shape[1])
+    return (np.uint64(per_expert.data_ptr()) +
+            np.arange(experts, dtype=np.uint64) * np.uint64(n * 4))
+
+
 class GroupedGemmPlan:
     """Reusable launch plan for ``D_e = A_e @ B_e^T`` over routed experts."""
 
@@ -89,12 +122,16 @@ class GroupedGemmPlan:
         packed_rows: int = 0,
         results_pushed: bool = False,
         tokens_per_expert_dev: int = 0,
+        row_scale_ptrs: Sequence[int] | None = None,
+        col_scale_ptrs: Sequence[int] | None = None,
+        packed_row_scale: int = 0,
     ) -> int:
         """Pointer-array form of the reference arguments. Returns a status.
         ``packed_a`` / ``packed_rows``: base and row capacity of ONE buffer holding all
         experts' rows back to back (one tensor map instead of one per expert; ``a_ptrs``
         is then ignored). ``results_pushed``: no D descriptors, results leave through
-        ``set_push``."""
+        ``set_push``. ``row_scale_ptrs`` / ``col_scale_ptrs`` / ``packed_row_scale``: scales
+        of INT8 operands (``data_type`` 3)."""
         experts = len(tokens_per_expert)
 
         def pointers(values):
@@ -104,7 +141,15 @@ class GroupedGemmPlan:
                 arr = np.array([int(p or 0) for p in values], dtype=np.uint64)
             return arr if arr.size else np.zeros(1, dtype=np.uint64)
 
+        def pointer_table(values):
+            if values is None:
+                return None, None
+            arr = pointers(values)
+            return arr, arr.ctypes.data_as(C.POINTER(C.c_void_p))
+
         arr_a, arr_b, arr_d = pointers(a_ptrs), pointers(b_ptrs), pointers(d_ptrs)
+        keep_row, row_scale = pointer_table(row_scale_ptrs)
+        keep_col, col_scale = pointer_table(col_scale_ptrs)
         counts = np.ascontiguousarray(tokens_per_expert, dtype=np.uint32)
         if counts.size == 0:
             counts = np.zeros(1, dtype=np.uint32)
@@ -131,14 +176,19 @@ class GroupedGemmPlan:
             results_pushed=1 if results_pushed else 0,
             reserved0=0,
             tokens_per_expert_dev=int(tokens_per_expert_dev) or None,
+            row_scale=row_scale,
+            col_scale=col_scale,
+            packed_row_scale=int(packed_row_scale) or None,
         )
         return int(self._lib.bmoe_plan_initialize(self._handle, C.byref(args)))
 
     def initialize_packed(self, a, w, d, tokens_per_expert: Sequence[int], *,
-                          single_a_map: bool = False, **options) -> int:
+                          single_a_map: bool = False, row_scale=None, col_scale=None,
+                          **options) -> int:
         """Packed form: ``a`` [sum M, k], ``w`` [E, n, k], ``d`` [sum M, n] CUDA
         tensors, rows of expert 0 first; ``a`` and ``w`` BF16, or both one byte per element
-        (FP8 E4M3 bit patterns; k then a multiple of 16), ``d`` BF16 (FP32 with
+        (FP8 E4M3 bit patterns, or ``torch.int8`` with FP32 ``row_scale`` [rows of a] and
+        ``col_scale`` [E, n]; k then a multiple of 16), ``d`` BF16 (FP32 with
         ``output_f32``). Row offsets are the exclusive prefix sum
         of the counts; every expert's slice starts on a 16-byte boundary because
         k and n are multiples of 8. ``single_a_map``: one tensor map over the whole of
@@ -163,30 +213,50 @@ class GroupedGemmPlan:
         if elem != int(w.element_size()) or elem not in (1, 2):
             return _capi.INVALID_ARGUMENT
         if elem == 1:
-            options["data_type"] = 1          # FP8 E4M3 bytes (torch.float8_e4m3fn or uint8)
+            options["data_type"] = _byte_type(a, w)
+        if not _scales_fit(options.get("data_type"), a, w, row_scale, col_scale):
+            return _capi.INVALID_ARGUMENT
+        if row_scale is not None:
+            options["row_scale_ptrs"] = np.uint64(row_scale.data_ptr()) + first_row * np.uint64(4)
+            options["col_scale_ptrs"] = _expert_pointers(col_scale)
+            if single_a_map:
+                options["packed_row_scale"] = row_scale.data_ptr()
         a_ptrs = np.uint64(a.data_ptr()) + first_row * np.uint64(k * elem)
         b_ptrs = (np.uint64(w.data_ptr()) +
                   np.arange(experts, dtype=np.uint64) * np.uint64(n * k * elem))
         d_ptrs = np.uint64(d.data_ptr()) + first_row * np.uint64(n * d_elem)
-        self._keep = (a, w, d)
+        self._keep = (a, w, d, row_scale, col_scale)
         if single_a_map:
             options.update(packed_a=a.data_ptr(), packed_rows=int(a.shape[0]))
         return self.initialize(a_ptrs, b_ptrs, d_ptrs, counts, n, k, **options)
 
-    def initialize_packed_device_counts(self, a, w, counts_dev_ptr: int, **options) -> int:
+    def initialize_packed_device_counts(self, a, w, counts_dev_ptr: int, *, row_scale=None,
+                                        col_scale=None, **options) -> int:
         """Packed form whose counts exist only on the device: ``counts_dev_ptr`` points at
         uint32 [E] rows per expert, written by work that precedes this call in the stream
         (for example ``bmoe_ep_plan``). Nothing is read back: the worklist is built from
         the device counts, the kernel takes the tile total from device memory, the grid is
         the full persistent grid, and the results leave through ``set_push``. ``a`` is
-        the packed row buffer (its row count is the capacity)."""
+        the packed row buffer (its row count is the capacity). INT8 operands take
+        ``row_scale`` and ``col_scale`` as ``initialize_packed`` does."""
         experts = int(w.shape[0])
         n, k = int(w.shape[1]), int(w.shape[2])
         if experts == 0 or int(a.shape[1]) != k or not (a.is_contiguous() and w.is_contiguous()):
             return _capi.INVALID_ARGUMENT
-        b_ptrs = np.uint64(w.data_ptr()) + np.arange(experts, dtype=np.uint64) * np.uint64(n * k * 2)
+        elem = int(a.element_size())
+        if elem != int(w.element_size()) or elem not in (1, 2):
+            return _capi.INVALID_ARGUMENT
+        if elem == 1:
+            options["data_type"] = _byte_type(a, w)
+        if not _scales_fit(options.get("data_type"), a, w, row_scale, col_scale):
+            return _capi.INVALID_ARGUMENT
+        if row_scale is not None:
+            options["col_scale_ptrs"] = _expert_pointers(col_scale)
+            options["packed_row_scale"] = row_scale.data_ptr()
+        b_ptrs = (np.uint64(w.data_ptr()) +
+                  np.arange(experts, dtype=np.uint64) * np.uint64(n * k * elem))
         zeros = np.zeros(experts, dtype=np.uint64)
-        self._keep = (a, w)
+        self._keep = (a, w, row_scale, col_scale)
         return self.initialize(zeros, b_ptrs, zeros, np.zeros(experts, dtype=np.uint32), n, k,
                                packed_a=a.data_ptr(), packed_rows=int(a.shape[0]),
                                results_pushed=True, tokens_per_expert_dev=counts_dev_ptr,

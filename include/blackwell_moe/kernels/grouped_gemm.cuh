@@ -15,7 +15,7 @@
 
 namespace blackwell_moe {
 
-enum class DataType { kBf16, kFp8E4M3 };
+enum class DataType { kBf16, kFp8E4M3, kInt8 = 3 };  // kInt8: engine extension
 
 struct GroupedGemmArguments {
   // a, b, d: HOST arrays with `experts` entries, each a DEVICE pointer.
@@ -53,6 +53,10 @@ struct GroupedGemmArguments {
   // inside each expert, which keeps the expert's rows in L2 while its weights
   // stream once (default 1).
   std::int32_t raster_along_m = -1;
+  // kInt8 only, required then: host arrays [experts] of device pointers to the scale of
+  // every row of A_e (M_e floats) and of every output channel (n floats, 16-byte aligned).
+  const float* const* row_scale = nullptr;
+  const float* const* col_scale = nullptr;
 };
 
 enum class KernelStatus {
@@ -121,6 +125,7 @@ class Bf16GroupedGemmPlan {
 
  private:
   friend class Fp8E4m3GroupedGemmPlan;
+  friend class Int8GroupedGemmPlan;
   KernelStatus initialize_typed(const GroupedGemmArguments& args);
   struct Impl;
   Impl* impl_ = nullptr;
@@ -133,6 +138,24 @@ class Bf16GroupedGemmPlan {
 // that behaviour, this class is where the type is accepted. args.data_type must be
 // kFp8E4M3 (anything else: kUnsupportedDataType) and k a multiple of 16.
 class Fp8E4m3GroupedGemmPlan {
+ public:
+  KernelStatus initialize(const GroupedGemmArguments& args);
+  KernelStatus run(void* stream = nullptr) { return plan_.run(stream); }
+  GroupedGemmPlanStats stats() const { return plan_.stats(); }
+  KernelStatus poll() { return plan_.poll(); }
+  void* native_handle() const { return plan_.native_handle(); }
+
+ private:
+  Bf16GroupedGemmPlan plan_;
+};
+
+// Extension: the same plan over signed 8-bit operands with a scale per row of A and per
+// output channel, the product of quantised activations and weights:
+//   D_e[m, n] = float(sum_k A_e[m, k] * B_e[n, k]) * (row_scale[m] * col_scale[n])
+// (exact 32-bit sums, BF16 out). args.data_type must be kInt8 (anything else:
+// kUnsupportedDataType), k a multiple of 16 and at most 131071, both scale arrays set. The
+// reference has no integer type.
+class Int8GroupedGemmPlan {
  public:
   KernelStatus initialize(const GroupedGemmArguments& args);
   KernelStatus run(void* stream = nullptr) { return plan_.run(stream); }

@@ -322,8 +322,11 @@ typedef struct bmoe_gemm_args {
                          (no scales), FP32 accumulation, D as for BF16; k must then be a
                          multiple of 16. The reference declares the type and rejects it
                          (grouped_gemm.cuh:10, cutlass_baseline.cu:211-213); so do the
-                         C++ Bf16GroupedGemmPlan and the one-shot launcher. Other values:
-                         BMOE_UNSUPPORTED_DATA_TYPE. */
+                         C++ Bf16GroupedGemmPlan and the one-shot launcher. 3 = INT8: a[]
+                         and b[] hold signed bytes, sums are exact in 32-bit integers and
+                         leave as float(sum) * (row_scale * col_scale) (row_scale and
+                         col_scale below; k a multiple of 16, at most
+                         BMOE_INT8_MAX_K). Other values: BMOE_UNSUPPORTED_DATA_TYPE. */
   uint32_t scheduler; /* bmoe_scheduler */
   uint32_t claim_size;
   uint32_t hybrid_tail_tiles;
@@ -360,7 +363,27 @@ typedef struct bmoe_gemm_args {
    * (expert_order, static_persistent, compacted, dynamic_queue; no hybrid tail).
    * tokens_per_expert is then ignored; stats report capacities. */
   const uint32_t* tokens_per_expert_dev;
+  /* Scales of INT8 operands (appended; read for data_type 3 only, required then).
+   * row_scale: host array [experts] of device pointers to float [M_e], one scale per row
+   * of A_e; col_scale: host array [experts] of device pointers to float [n], one per
+   * row of B_e (output channel), 16-byte aligned. With packed_a set, row_scale is ignored
+   * and packed_row_scale points at float [packed_rows], in the order of packed_a's rows.
+   * Entries of experts without tokens may be NULL. */
+  const float* const* row_scale;
+  const float* const* col_scale;
+  const float* packed_row_scale;
 } bmoe_gemm_args;
+
+/* Operand element types of bmoe_gemm_args::data_type and of section 6 (2 is unused). */
+enum bmoe_data_type {
+  BMOE_TYPE_BF16 = 0,
+  BMOE_TYPE_FP8_E4M3 = 1,
+  BMOE_TYPE_INT8 = 3,
+  BMOE_TYPE_FP32 = 4 /* section 6 inputs only */
+};
+
+/* Largest k of an INT8 product: 131071 products of at most 128 * 128 stay below 2^31. */
+#define BMOE_INT8_MAX_K 131071u
 
 /* blackwell_moe::GroupedGemmPlanStats (grouped_gemm.cuh:42-46) + extensions. */
 typedef struct bmoe_plan_stats {
@@ -812,6 +835,111 @@ int bmoe_peer_free(void* ptr);
  * Call it before latency-critical work and before the first multi-GPU step, whose
  * bounded waits assume that all ranks launch within the wait budget. */
 int bmoe_preload_kernels(void);
+
+/* ======================================================================== */
+/* 6. Layer operators either side of the grouped GEMM (no counterpart in the */
+/*    reference, which takes routed token counts as its input:               */
+/*    agent/search_space.yaml:10-13)                                         */
+/* ======================================================================== */
+
+/* How bmoe_route_topk turns a logit into a score. */
+enum bmoe_scoring {
+  BMOE_SCORE_SOFTMAX = 0, /* softmax over the experts that can be chosen */
+  BMOE_SCORE_SIGMOID = 1
+};
+
+#define BMOE_ROUTE_MAX_EXPERTS 1024u
+#define BMOE_ROUTE_MAX_TOP_K 32u
+
+typedef struct bmoe_route_topk_args {
+  const void* logits_dev;    /* [tokens, experts] router outputs, rows row_stride apart */
+  const float* bias_dev;     /* [experts] or NULL: added to the score for the choice only
+                                (BMOE_SCORE_SIGMOID) */
+  int64_t* expert_ids_dev;   /* out [tokens, top_k] */
+  float* weights_dev;        /* out [tokens, top_k] */
+  uint64_t tokens;
+  uint64_t row_stride;       /* elements between rows; 0 = experts */
+  uint32_t experts;          /* <= BMOE_ROUTE_MAX_EXPERTS */
+  uint32_t top_k;            /* <= experts, <= BMOE_ROUTE_MAX_TOP_K */
+  uint32_t logits_type;      /* BMOE_TYPE_BF16 or BMOE_TYPE_FP32 */
+  uint32_t scoring;          /* bmoe_scoring */
+  uint32_t renormalize;      /* 1: weights are divided by the sum over the chosen experts */
+  float scale;               /* factor on every weight (1 = none) */
+  void* stream;
+} bmoe_route_topk_args;
+
+/* The router's choice: for every token the top_k experts with the largest scores, largest
+ * first, the lower id first among equals, and their weights in FP32; the inputs of
+ * bmoe_ep_count, bmoe_combine_topk and bmoe_moe_decode. The order is exact: without bias
+ * it is the order of the logits, with bias that of sigmoid(logit) + bias evaluated in 64
+ * bits. A NaN or -inf logit (an expert that is switched off) is never chosen, nor is a NaN
+ * or -inf sum; a token left with fewer than top_k experts gets id -1 (a dropped assignment)
+ * and weight 0 in the remaining places. Equal +inf logits share the softmax. */
+int bmoe_route_topk(const bmoe_route_topk_args* args);
+
+typedef struct bmoe_quantize_rows_args {
+  const void* src_dev;      /* [src_rows, cols], rows src_stride apart, 16-byte aligned */
+  const int64_t* index_dev; /* [rows] source row of each output row, or NULL (row i) */
+  int8_t* dst_dev;          /* out [rows, cols], 16-byte aligned */
+  float* scale_dev;         /* out [rows] */
+  uint64_t rows;
+  uint64_t src_rows;        /* rows of src */
+  uint64_t src_stride;      /* elements between source rows, a multiple of 8 (BF16) or 4
+                               (FP32); 0 = cols */
+  uint32_t cols;            /* multiple of 16 */
+  uint32_t src_type;        /* BMOE_TYPE_BF16 or BMOE_TYPE_FP32 */
+  void* stream;
+} bmoe_quantize_rows_args;
+
+/* Rows to 8-bit integers with one scale per row, the A operand and row scales of an INT8
+ * product (data_type 3); with index_dev it is also the gather of bmoe_gather_rows (token
+ * rows into expert order). Per row, in FP32 with one rounding per operation:
+ *   largest = max(max |x|, 2^-100)     scale = largest / 127
+ *   q = rint(x * (127 * (1 / largest)))      (ties to even; |q| <= 127)
+ * Indices outside [0, src_rows) leave the output row and its scale untouched. A row that
+ * holds a NaN gets scale NaN, one that holds an infinity scale inf; their q are finite, so
+ * the product's row becomes NaN or infinite rather than plausible. */
+int bmoe_quantize_rows(const bmoe_quantize_rows_args* args);
+
+#define BMOE_MOE_DECODE_MAX_TOKENS 64u
+#define BMOE_MOE_DECODE_MAX_TOP_K 32u
+#define BMOE_MOE_DECODE_MAX_EXPERTS 1024u
+
+typedef struct bmoe_moe_decode_args {
+  const void* x_dev;              /* BF16 [tokens, hidden] */
+  const void* w_gate_up_dev;      /* [experts, 2 * inter, hidden]: gate rows, then up rows */
+  const void* w_down_dev;         /* [experts, hidden, inter] */
+  const float* gate_up_scale_dev; /* INT8 weights: [experts, 2 * inter] per output channel */
+  const float* down_scale_dev;    /* INT8 weights: [experts, hidden] */
+  const int64_t* expert_ids_dev;  /* [tokens, top_k]; ids outside [0, experts) are dropped */
+  const float* weights_dev;       /* [tokens, top_k] */
+  void* out_dev;                  /* BF16 [tokens, hidden], every row written */
+  void* workspace_dev;            /* bmoe_moe_decode_workspace bytes, 256-byte aligned */
+  uint64_t workspace_bytes;
+  uint32_t tokens;                /* <= BMOE_MOE_DECODE_MAX_TOKENS */
+  uint32_t top_k;                 /* <= BMOE_MOE_DECODE_MAX_TOP_K */
+  uint32_t experts;               /* <= BMOE_MOE_DECODE_MAX_EXPERTS */
+  uint32_t hidden;                /* multiple of 8 (BF16 weights) or 16 (INT8) */
+  uint32_t inter;                 /* multiple of 8 (BF16 weights) or 16 (INT8) */
+  uint32_t data_type;             /* of the weights: BMOE_TYPE_BF16 or BMOE_TYPE_INT8 */
+  void* stream;
+} bmoe_moe_decode_args;
+
+/* Workspace of a bmoe_moe_decode call in bytes. Calls that may overlap (two streams, two
+ * captured graphs replayed at once) need a workspace each. */
+uint64_t bmoe_moe_decode_workspace(uint32_t tokens, uint32_t top_k, uint32_t inter);
+
+/* A whole expert layer for a few tokens (a decode step), in two launches:
+ *   h[t, j] = silu(x[t] Wgate_e^T) * (x[t] Wup_e^T),  e = expert_ids[t, j]
+ *   out[t]  = bf16( sum_j weights[t, j] * (h[t, j] Wdown_e^T) )
+ * with silu(v) = v / (1 + exp(-v)). Every weight of an expert that some token chose is
+ * read once, the others not at all. Products of BF16 operands are summed in FP32, h keeps
+ * 16 significant bits or more, one BF16 rounding at the end; INT8 weights are multiplied
+ * as the integers they are and scaled per output channel in FP32. An expert that a token
+ * names twice counts with the sum of both weights. Dropped assignments contribute nothing;
+ * a token with nothing else gets a row of zeros. Results do not depend on the run: no
+ * atomics. All pointers 16-byte aligned. For more tokens there is the grouped GEMM plan. */
+int bmoe_moe_decode(const bmoe_moe_decode_args* args);
 
 /* Library build information ("sm_100a", CUDA runtime version, ...). */
 const char* bmoe_build_info(void);
