@@ -67,6 +67,7 @@ ROUTE_MAX_TOP_K = 32
 MOE_DECODE_MAX_TOKENS = 64
 MOE_DECODE_MAX_TOP_K = 32
 MOE_DECODE_MAX_EXPERTS = 1024
+MOE_DECODE_MAX_WIDTH = 65536
 
 DISTRIBUTIONS = {"uniform": 0, "heavy_hitter": 1, "heavy": 1, "sparse": 2, "zipf": 3,
                  "heavy_sparse": 4}

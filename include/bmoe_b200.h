@@ -904,6 +904,7 @@ int bmoe_quantize_rows(const bmoe_quantize_rows_args* args);
 #define BMOE_MOE_DECODE_MAX_TOKENS 64u
 #define BMOE_MOE_DECODE_MAX_TOP_K 32u
 #define BMOE_MOE_DECODE_MAX_EXPERTS 1024u
+#define BMOE_MOE_DECODE_MAX_WIDTH 65536u /* hidden and inter */
 
 typedef struct bmoe_moe_decode_args {
   const void* x_dev;              /* BF16 [tokens, hidden] */

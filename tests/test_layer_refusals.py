@@ -87,7 +87,9 @@ def decode_args(cap, **change):
     (dict(experts=1025), "INVALID_ARGUMENT"),
     (dict(hidden=0), "INVALID_ARGUMENT"),
     (dict(hidden=60), "INVALID_ARGUMENT"),
+    (dict(hidden=65544), "INVALID_ARGUMENT"),
     (dict(inter=0), "INVALID_ARGUMENT"),
+    (dict(inter=65544), "INVALID_ARGUMENT"),
     (dict(inter=12), "INVALID_ARGUMENT"),
     (dict(x_dev=None), "INVALID_ARGUMENT"),
     (dict(x_dev=P + 8), "INVALID_ARGUMENT"),
