@@ -329,7 +329,7 @@ class MoeDecodeArgs(C.Structure):
         ("workspace_dev", C.c_void_p), ("workspace_bytes", C.c_uint64),
         ("tokens", C.c_uint32), ("top_k", C.c_uint32), ("experts", C.c_uint32),
         ("hidden", C.c_uint32), ("inter", C.c_uint32), ("data_type", C.c_uint32),
-        ("stream", C.c_void_p),
+        ("stream", C.c_void_p), ("status_dev", C.c_void_p),
     ]
 
 

@@ -2,66 +2,108 @@
 //   h[t, j] = silu(x[t] Wgate_e^T) * (x[t] Wup_e^T)      e = expert_ids[t, j]
 //   out[t]  = bf16( sum_j weights[t, j] * (h[t, j] Wdown_e^T) )
 //
-// What bounds it is the stream of the chosen experts' weights from HBM: an expert has one
-// to a few rows, so a weight is used a few times at most. Both kernels therefore read every
-// weight once, straight into registers in the operand layout of mma.sync m16n8k16 with the
-// WEIGHTS as the 16-row operand and up to 8 tokens as the columns: no shared-memory round
-// trip and no 128-row tile that a handful of rows would leave empty (the tile of
-// tcgen05.mma), and the tensor work stays far below the pipe's rate at these row counts.
-//
-// Operand layout. A lane (g = lane / 4, t = lane % 4) reads 16 bytes of rows g and g + 8 at
-// byte 16 t of a 64-byte step, i.e. 8 BF16 or 16 INT8 values of k, and the 8 or 16 values of
-// x (or h) at the same k for column g. The k order inside a step is permuted the same way on
-// both sides, which a sum over k does not see.
+// What bounds it is the stream of the chosen experts' weights from HBM: an expert has one to a
+// few tokens, so a weight is used a few times at most. Both kernels read every weight once,
+// 128 rows at a time through a ring of TMA boxes, with the WEIGHTS as the 128-row operand of
+// tcgen05.mma and the expert's tokens as its 16 to 64 columns: the rows are full however
+// few tokens there are, and the ring (about 100 KB per CTA, two CTAs per SM where they fit)
+// keeps enough bytes in flight to hold HBM busy while CTAs come and go.
+//   warp 0     TMA producer
+//   warp 1     MMA issuer (one elected lane), Tensor Memory
+//   warps 4-7  BF16 weights: epilogue
+//              INT8 weights: shared memory -> BF16 -> Tensor Memory, the A operand of the
+//              MMA (a signed byte is a BF16 value, so the conversion is exact); the first
+//              kernel's epilogue; the second kernel has warps 8-11 for it
+// Few tiles are split along k over the CTAs of a cluster, joined in a fixed order through
+// distributed shared memory: no atomics, the same bits on every run.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
 
 #include "bmoe_b200.h"
 #include "preload.cuh"
+#include "ptx_sm100.cuh"
+#include "tensor_map.cuh"
 
 namespace bmoe {
 namespace {
 
 constexpr uint32_t kFullWarp = 0xffffffffu;
 constexpr uint32_t kMaxTokens = BMOE_MOE_DECODE_MAX_TOKENS;
-constexpr uint32_t kStepBytes = 64;   // bytes of a weight row per step
-constexpr uint32_t kUnroll = 4;       // steps whose weights are in flight together ("block")
+constexpr uint32_t kRows = 128;                  // weight rows of a tile
+constexpr uint32_t kABytes = kRows * 128;        // one k-block of weights: 128 bytes of a row
+constexpr uint32_t kGroup = 8;                   // tokens of one activation box
+constexpr uint32_t kTwoPerSm = 108u * 1024u;     // shared memory of a CTA that shares its SM
+constexpr uint32_t kOnePerSm = 208u * 1024u;
+constexpr uint32_t kTmemA = 128;                 // first column of the INT8 A operand
+constexpr uint64_t kWaitBudgetNs = 1000000000ull;
 
 struct DecodeArgs {
-  const uint16_t* x;        // [tokens, hidden]
-  const uint8_t* w1;        // [experts, 2 * inter, hidden]
-  const uint8_t* w2;        // [experts, hidden, inter]
   const float* s1;          // INT8: [experts, 2 * inter]
   const float* s2;          // INT8: [experts, hidden]
   const int64_t* ids;       // [tokens, top_k]
   const float* coef;        // [tokens, top_k]
   uint16_t* out;            // [tokens, hidden]
-  uint16_t* h_hi;           // [tokens * top_k, inter], upper and
-  uint16_t* h_lo;           // lower half of weights * h
+  uint16_t* h;              // [2][tokens * top_k, inter]: upper and lower half of weights * h
+  uint32_t* status;         // optional: where a bounded wait gave up
   uint32_t tokens, top_k, experts, hidden, inter;
   uint32_t by_expert;       // grid.y of the first kernel: expert ids, or assignments
 };
 
-// ------------------------------------------------------------- fragments --
+struct DecodeParams {
+  CUtensorMap weights;      // w_gate_up as {hidden, experts * 2 * inter}, box of 64 rows, or
+                            // w_down as {inter, experts * hidden}, box of 128 rows
+  CUtensorMap acts;         // x as {hidden, tokens} or h as {inter, 2 * tokens * top_k},
+                            // boxes of 8 rows
+  DecodeArgs a;
+};
 
-// Weights are read once: keep them out of L1, where the activations live.
-__device__ __forceinline__ uint4 load_weights(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
+// Stages of one CTA. COLS: columns (tokens) a stage has room for; PLANES: 1 (x) or 2 (the two
+// halves of h). A k-block is 128 bytes of every weight row: 64 BF16 or 128 INT8 values, against
+// one or two 128-byte wide pieces of the activations.
+template <bool INT8, uint32_t COLS, uint32_t PLANES, uint32_t RESERVED>
+struct Ring {
+  static constexpr uint32_t kPieces = INT8 ? 2 : 1;
+  static constexpr uint32_t kBlockK = 64 * kPieces;
+  static constexpr uint32_t kPieceBytes = COLS * 128;
+  static constexpr uint32_t kStageBytes = kABytes + PLANES * kPieces * kPieceBytes;
+  static constexpr uint32_t kTwo = (kTwoPerSm - RESERVED) / kStageBytes;
+  static constexpr uint32_t kOne = (kOnePerSm - RESERVED) / kStageBytes;
+  // Two CTAs per SM if each keeps three stages: while one starts or ends, the other streams.
+  static constexpr uint32_t kCtasPerSm = kTwo >= 3 ? 2 : 1;
+  static constexpr uint32_t kStages = kCtasPerSm == 2 ? (kTwo < 6 ? kTwo : 6) : (kOne < 6 ? kOne : 6);
+  static_assert(kStages >= 2, "ring");
+};
 
-__device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
+// Barriers of a CTA (static shared memory).
+struct Barriers {
+  uint64_t full[6], empty[6];     // stage: bytes landed / MMAs done with it
+  uint64_t a_full[2], a_empty[2]; // INT8: converted weights in Tensor Memory / read by the MMAs
+  uint64_t d_full[2], d_empty[2]; // accumulator: complete / drained
+};
 
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
-      "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+struct Wait {
+  volatile uint32_t* abort_word;
+  __device__ __forceinline__ bool operator()(uint64_t& bar, uint32_t parity) const {
+    return ptx::mbar_wait(ptx::smem_addr(&bar), parity, abort_word, kWaitBudgetNs);
+  }
+};
+
+// Position in a ring of `N` slots: slot and the parity of its current use.
+template <uint32_t N>
+struct Cursor {
+  uint32_t slot = 0, parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
+__device__ __forceinline__ void report(const DecodeArgs& a, uint32_t site) {
+  if (a.status != nullptr) atomicCAS(a.status, 0u, 0x50000000u | site);
 }
 
 // Two signed bytes of `word` (selector 0x4140: bytes 0, 1; 0x4342: bytes 2, 3) -> BF16 pair,
@@ -74,46 +116,6 @@ __device__ __forceinline__ uint32_t int8_pair(uint32_t word, uint32_t selector) 
   return r;
 }
 
-// One step of one 16-row tile against one 8-column tile: 32 (BF16) or 64 (INT8) of k.
-// lo, hi: this lane's 16 bytes of rows g and g + 8; b: its 8 or 16 activations.
-template <bool INT8>
-struct Step {
-  static constexpr uint32_t kActs = INT8 ? 2 : 1;   // 16-byte loads of activations per lane
-  uint4 lo, hi;
-
-  __device__ __forceinline__ void multiply(float (&acc)[4], const uint4 (&b)[kActs]) const {
-    if constexpr (!INT8) {
-      mma_bf16(acc, lo.x, hi.x, lo.y, hi.y, b[0].x, b[0].y);
-      mma_bf16(acc, lo.z, hi.z, lo.w, hi.w, b[0].z, b[0].w);
-    } else {
-      mma_bf16(acc, int8_pair(lo.x, 0x4140), int8_pair(hi.x, 0x4140), int8_pair(lo.x, 0x4342),
-               int8_pair(hi.x, 0x4342), b[0].x, b[0].y);
-      mma_bf16(acc, int8_pair(lo.y, 0x4140), int8_pair(hi.y, 0x4140), int8_pair(lo.y, 0x4342),
-               int8_pair(hi.y, 0x4342), b[0].z, b[0].w);
-      mma_bf16(acc, int8_pair(lo.z, 0x4140), int8_pair(hi.z, 0x4140), int8_pair(lo.z, 0x4342),
-               int8_pair(hi.z, 0x4342), b[1].x, b[1].y);
-      mma_bf16(acc, int8_pair(lo.w, 0x4140), int8_pair(hi.w, 0x4140), int8_pair(lo.w, 0x4342),
-               int8_pair(hi.w, 0x4342), b[1].z, b[1].w);
-    }
-  }
-};
-
-// This lane's activations of one step: k = step * K + lane's share, zeros beyond `k_total`
-// (a multiple of the 8 or 16 values of a lane) and for a column without a row. Plain loads:
-// h is written by the first kernel while the second is already resident, so a load through the
-// read-only path, which the compiler may move above the wait between them, would be wrong.
-template <bool INT8>
-__device__ __forceinline__ void load_acts(uint4 (&b)[Step<INT8>::kActs], const uint16_t* row,
-                                          uint32_t k, uint32_t k_total) {
-  const bool live = row != nullptr && k < k_total;
-#pragma unroll
-  for (uint32_t i = 0; i < Step<INT8>::kActs; ++i) {
-    b[i] = live ? *reinterpret_cast<const uint4*>(row + k + 8 * i) : zero4();
-  }
-}
-
-__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
-
 __device__ __forceinline__ uint16_t to_bf16(float v) {
   uint16_t b;
   asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(b) : "f"(v));
@@ -124,446 +126,639 @@ __device__ __forceinline__ float from_bf16(uint16_t v) {
   return __uint_as_float(static_cast<uint32_t>(v) << 16);
 }
 
-// --------------------------------------------------- gate and up products --
+// ------------------------------------------------------------------- roles --
 
-// One CTA computes 16 * WR channels of one expert for all of its tokens: WR warps side by side
-// (16 gate and 16 up rows each), times WK warps that share the k range block by block.
-template <bool INT8, uint32_t NT, uint32_t WR, uint32_t WK>
-__global__ void __launch_bounds__(32 * WR * WK) decode_up_kernel(DecodeArgs a) {
-  using S = Step<INT8>;
-  constexpr uint32_t kStep = INT8 ? 64 : 32;         // k values per step
-  constexpr uint32_t kLane = INT8 ? 16 : 8;          // of which a lane holds these
-  extern __shared__ float4 partial[];                // [WK][WR][2][NT][32]
-  __shared__ uint16_t list_row[kMaxTokens];          // assignment of column p
-  __shared__ uint8_t list_token[kMaxTokens];
-  __shared__ float list_coef[kMaxTokens];
-  __shared__ uint32_t list_count, list_expert;
-
-  // let the second kernel's CTAs take their places as this grid's last CTAs run
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (warp == 0) {
-    // Tokens of this CTA's expert. By assignment: the expert's first one does the work.
-    const int64_t e = a.by_expert != 0 ? static_cast<int64_t>(blockIdx.y) : a.ids[blockIdx.y];
-    uint32_t count = 0, owner = 0;
-    if (e >= 0 && e < a.experts) {
-      for (uint32_t t0 = 0; t0 < a.tokens; t0 += 32) {
-        const uint32_t t = t0 + lane;
-        int first = -1;
-        float coef = 0.0f;
-        if (t < a.tokens) {
-          for (uint32_t j = 0; j < a.top_k; ++j) {
-            if (a.ids[t * a.top_k + j] == e) {   // twice: the sum of both weights
-              if (first < 0) first = static_cast<int>(t * a.top_k + j);
-              coef += a.coef[t * a.top_k + j];
+// MMA issuer: `blocks` k-blocks into the accumulator at `d_tmem` (n columns). Returns false
+// when a wait gave up. The warp is converged; one elected lane issues.
+template <bool INT8, uint32_t PLANES, typename R>
+__device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars, uint32_t ring,
+                                             Cursor<R::kStages>& stage, Cursor<2>& a_buf,
+                                             uint32_t tmem, uint32_t d_tmem, uint32_t n,
+                                             uint32_t blocks, uint64_t& done) {
+  const uint32_t idesc = ptx::make_bf16_idesc(kRows, n);
+  for (uint32_t b = 0; b < blocks; ++b) {
+    if (!wait(bars.full[stage.slot], stage.parity)) return false;
+    if (INT8 && !wait(bars.a_full[a_buf.slot], a_buf.parity)) return false;
+    ptx::tc_fence_after_sync();
+    const uint32_t at = ring + stage.slot * R::kStageBytes;
+    const uint64_t a_desc = ptx::make_kmajor_sw128_desc(at);
+    const uint32_t a_tmem = tmem + kTmemA + a_buf.slot * 64;
+    if (ptx::elect_one()) {
+#pragma unroll
+      for (uint32_t piece = 0; piece < R::kPieces; ++piece) {
+#pragma unroll
+        for (uint32_t ks = 0; ks < 4; ++ks) {
+#pragma unroll
+          for (uint32_t plane = 0; plane < PLANES; ++plane) {
+            const uint64_t b_desc = ptx::make_kmajor_sw128_desc(
+                at + kABytes + (plane * R::kPieces + piece) * R::kPieceBytes);
+            const uint32_t acc = (b | piece | ks | plane) != 0 ? 1u : 0u;
+            if constexpr (INT8) {
+              ptx::umma_bf16_ts(d_tmem, a_tmem + (piece * 4 + ks) * 8, b_desc + 2 * ks, idesc, acc);
+            } else {
+              ptx::umma_bf16_ss(d_tmem, a_desc + 2 * ks, b_desc + 2 * ks, idesc, acc);
             }
           }
         }
-        const uint32_t mask = __ballot_sync(kFullWarp, first >= 0);
-        if (count == 0 && mask != 0) {
-          owner = static_cast<uint32_t>(__shfl_sync(kFullWarp, first, __ffs(mask) - 1));
-        }
-        if (first >= 0) {
-          const uint32_t p = count + __popc(mask & ((1u << lane) - 1));
-          list_row[p] = static_cast<uint16_t>(first);
-          list_token[p] = static_cast<uint8_t>(t);
-          list_coef[p] = coef;
-        }
-        count += __popc(mask);
       }
-      if (a.by_expert == 0 && owner != blockIdx.y) count = 0;
+      ptx::umma_commit(ptx::smem_addr(&bars.empty[stage.slot]));
+      if (INT8) ptx::umma_commit(ptx::smem_addr(&bars.a_empty[a_buf.slot]));
+      if (b + 1 == blocks) ptx::umma_commit(ptx::smem_addr(&done));
+    }
+    __syncwarp();
+    stage.next();
+    a_buf.next();
+  }
+  return true;
+}
+
+// INT8: one warp's 32 rows of `blocks` k-blocks from shared memory to Tensor Memory as BF16.
+template <typename R>
+__device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars, uint32_t ring,
+                                               Cursor<R::kStages>& stage, Cursor<2>& a_buf,
+                                               uint32_t tmem, uint32_t quad, uint32_t lane,
+                                               uint32_t blocks) {
+  for (uint32_t b = 0; b < blocks; ++b) {
+    if (!wait(bars.full[stage.slot], stage.parity)) return false;
+    if (!wait(bars.a_empty[a_buf.slot], a_buf.parity ^ 1u)) return false;
+    ptx::tc_fence_after_sync();
+    const uint32_t row = ring + stage.slot * R::kStageBytes + (quad * 32 + lane) * 128;
+    const uint32_t to = tmem + kTmemA + a_buf.slot * 64 + ((quad * 32) << 16);
+#pragma unroll
+    for (uint32_t half = 0; half < 2; ++half) {
+      uint32_t v[32];
+#pragma unroll
+      for (uint32_t c = 0; c < 4; ++c) {
+        // 16-byte pieces of a 128-byte row are swizzled by the row's place in its group of 8
+        const uint4 w = ptx::ld_shared_v4(row + (((half * 4 + c) ^ (lane & 7)) << 4));
+        v[8 * c + 0] = int8_pair(w.x, 0x4140);
+        v[8 * c + 1] = int8_pair(w.x, 0x4342);
+        v[8 * c + 2] = int8_pair(w.y, 0x4140);
+        v[8 * c + 3] = int8_pair(w.y, 0x4342);
+        v[8 * c + 4] = int8_pair(w.z, 0x4140);
+        v[8 * c + 5] = int8_pair(w.z, 0x4342);
+        v[8 * c + 6] = int8_pair(w.w, 0x4140);
+        v[8 * c + 7] = int8_pair(w.w, 0x4342);
+      }
+      ptx::tmem_store_32x32(to + half * 32, v);
+    }
+    ptx::tmem_store_wait();
+    ptx::tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&bars.a_full[a_buf.slot]));
+    stage.next();
+    a_buf.next();
+  }
+  return true;
+}
+
+__device__ __forceinline__ void init_barriers(Barriers& bars) {
+  for (uint32_t s = 0; s < 6; ++s) {
+    ptx::mbar_init(ptx::smem_addr(&bars.full[s]), 1);
+    ptx::mbar_init(ptx::smem_addr(&bars.empty[s]), 1);
+  }
+  for (uint32_t b = 0; b < 2; ++b) {
+    ptx::mbar_init(ptx::smem_addr(&bars.a_full[b]), 4);    // converting warps
+    ptx::mbar_init(ptx::smem_addr(&bars.a_empty[b]), 1);
+    ptx::mbar_init(ptx::smem_addr(&bars.d_full[b]), 1);
+    ptx::mbar_init(ptx::smem_addr(&bars.d_empty[b]), 4);   // epilogue warps
+  }
+  ptx::fence_barrier_init();
+}
+
+// Copies and MMAs that an expired wait left behind land before their memory goes away.
+__device__ __forceinline__ void settle(volatile uint32_t* abort_word) {
+  if (*abort_word == 0) return;
+  const uint64_t start = ptx::global_timer_ns();
+  while (ptx::global_timer_ns() - start < 200000) __nanosleep(1000);
+}
+
+// --------------------------------------------------- gate and up products --
+
+constexpr uint32_t kUpThreads = 256;
+
+template <bool INT8, uint32_t COLS>
+using UpRing = Ring<INT8, COLS, 1, 0>;
+
+template <bool INT8, uint32_t COLS>
+constexpr uint32_t kUpSmem = UpRing<INT8, COLS>::kStages * UpRing<INT8, COLS>::kStageBytes + 1024;
+
+template <bool INT8, uint32_t COLS>
+constexpr uint32_t kUpTmem = INT8 ? 256 : (COLS < 32 ? 32 : COLS);
+
+// A cluster computes 64 channels of one expert for all of its tokens: the tile's rows 0-63
+// are the channels' gate rows, 64-127 their up rows. Activations come in boxes of 8 tokens, only
+// those that hold a token of the expert.
+template <bool INT8, uint32_t COLS>
+__global__ void __launch_bounds__(kUpThreads, (UpRing<INT8, COLS>::kCtasPerSm))
+decode_up_kernel(const __grid_constant__ DecodeParams p) {
+  using R = UpRing<INT8, COLS>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Barriers bars;
+  __shared__ uint32_t tmem_slot, abort_slot;
+  __shared__ uint32_t list_mask[2], list_base, list_expert;   // tokens of the expert
+  __shared__ float token_coef[kMaxTokens];
+  __shared__ uint8_t list_token[kMaxTokens], list_column[kMaxTokens];
+  const DecodeArgs& a = p.a;
+  const uint32_t ring = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Wait wait{&abort_slot};
+
+  if (warp == 0) {
+    if (lane == 0) {
+      ptx::tensormap_prefetch(&p.weights);
+      ptx::tensormap_prefetch(&p.acts);
+    }
+    // Tokens of this cluster's expert; rows of h in front of it (one per assignment to a
+    // lower id). By assignment: the expert's first one does the work.
+    const int64_t e = a.by_expert != 0 ? static_cast<int64_t>(blockIdx.y) : a.ids[blockIdx.y];
+    uint32_t mask[2] = {0, 0}, before = 0, owner = kFullWarp;
+    if (e >= 0 && e < a.experts) {
+#pragma unroll
+      for (uint32_t half = 0; half < 2; ++half) {
+        const uint32_t t = half * 32 + lane;
+        uint32_t first = kFullWarp;
+        float coef = 0.0f;
+        if (t < a.tokens) {
+          for (uint32_t j = 0; j < a.top_k; ++j) {
+            const uint32_t r = t * a.top_k + j;
+            const int64_t id = a.ids[r];
+            if (id == e) {                 // twice: the sum of both weights
+              if (first == kFullWarp) first = r;
+              coef += a.coef[r];
+            }
+            before += id >= 0 && id < e ? 1u : 0u;
+          }
+          token_coef[t] = coef;
+        }
+        mask[half] = __ballot_sync(kFullWarp, first != kFullWarp);
+        owner = min(owner, __reduce_min_sync(kFullWarp, first));
+      }
+      before = __reduce_add_sync(kFullWarp, before);
+      if (a.by_expert == 0 && owner != blockIdx.y) mask[0] = mask[1] = 0;
+    }
+    // column of a token in the tile: its place among the boxes that are loaded
+    uint32_t groups = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      if (((mask[i / 4] >> (8 * (i % 4))) & 0xffu) != 0) groups |= 1u << i;
+    }
+#pragma unroll
+    for (uint32_t half = 0; half < 2; ++half) {
+      if ((mask[half] >> lane) & 1u) {
+        const uint32_t t = half * 32 + lane;
+        const uint32_t at =
+            (half != 0 ? __popc(mask[0]) : 0) + __popc(mask[half] & ((1u << lane) - 1));
+        list_token[at] = static_cast<uint8_t>(t);
+        list_column[at] =
+            static_cast<uint8_t>(__popc(groups & ((1u << (t / 8)) - 1)) * 8 + t % 8);
+      }
     }
     if (lane == 0) {
-      list_count = count;
+      list_mask[0] = mask[0];
+      list_mask[1] = mask[1];
+      list_base = before;
       list_expert = static_cast<uint32_t>(e);
     }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      abort_slot = 0;
+      init_barriers(bars);
+    }
+    __syncwarp();
+    ptx::tmem_alloc(ptx::smem_addr(&tmem_slot), (kUpTmem<INT8, COLS>));
+    ptx::tmem_relinquish();
   }
+  ptx::tc_fence_before_sync();
   __syncthreads();
-  const uint32_t count = list_count;
-  if (count == 0) return;
+  ptx::tc_fence_after_sync();
+  // Let the second kernel's CTAs take their places as this grid's last CTAs run; not before
+  // this CTA has its Tensor Memory, which a waiting CTA of the second kernel would hold.
+  ptx::launch_dependents();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t mask[2] = {list_mask[0], list_mask[1]};
+  const uint32_t count = __popc(mask[0]) + __popc(mask[1]);
+  if (count == 0) {                        // the whole cluster: its CTAs share the expert
+    if (warp == 1) ptx::tmem_dealloc(tmem, (kUpTmem<INT8, COLS>));
+    return;
+  }
   const uint32_t expert = list_expert;
-  const uint32_t tiles = (count + 7) / 8;
-
-  const uint32_t g = lane >> 2, t = lane & 3;
-  const uint32_t wr = warp % WR, wk = warp / WR;
-  const uint32_t row0 = (blockIdx.x * WR + wr) * 16;
-  const size_t row_bytes = static_cast<size_t>(a.hidden) * (INT8 ? 1 : 2);
-  // rows beyond inter read the last one and are not stored
-  const uint32_t r_lo = min(row0 + g, a.inter - 1), r_hi = min(row0 + g + 8, a.inter - 1);
-  const size_t first_row = static_cast<size_t>(expert) * 2 * a.inter;
-  const uint8_t* const gate_lo = a.w1 + (first_row + r_lo) * row_bytes + 16 * t;
-  const uint8_t* const gate_hi = a.w1 + (first_row + r_hi) * row_bytes + 16 * t;
-  const size_t up_bytes = static_cast<size_t>(a.inter) * row_bytes;
-  const uint16_t* x_row[NT];
+  uint32_t groups = 0;
 #pragma unroll
-  for (uint32_t n = 0; n < NT; ++n) {
-    const uint32_t p = n * 8 + g;
-    x_row[n] = p < count ? a.x + static_cast<size_t>(list_token[p]) * a.hidden : nullptr;
+  for (uint32_t i = 0; i < 8; ++i) {
+    if (((mask[i / 4] >> (8 * (i % 4))) & 0xffu) != 0) groups |= 1u << i;
   }
+  const uint32_t boxes = __popc(groups);
+  const uint32_t n = (boxes + 1) / 2 * 16;         // columns of the MMA: a multiple of 16
 
-  float acc[2][NT][4];
+  const uint32_t rank = ptx::cluster_cta_rank(), ranks = ptx::cluster_cta_count();
+  const uint32_t channel0 = blockIdx.x / ranks * 64;
+  const uint32_t all_blocks = (a.hidden + R::kBlockK - 1) / R::kBlockK;
+  const uint32_t begin = all_blocks * rank / ranks, end = all_blocks * (rank + 1) / ranks;
+
+  if (warp == 0) {
+    Cursor<R::kStages> stage;
+    const uint32_t bytes = kABytes + boxes * R::kPieces * kGroup * 128;
+    const int32_t row = static_cast<int32_t>(expert * 2 * a.inter + channel0);
+    for (uint32_t b = begin; b < end; ++b) {
+      if (!wait(bars.empty[stage.slot], stage.parity ^ 1u)) {
+        if (lane == 0) report(a, 1);
+        break;
+      }
+      if (ptx::elect_one()) {
+        const uint32_t bar = ptx::smem_addr(&bars.full[stage.slot]);
+        const uint32_t at = ring + stage.slot * R::kStageBytes;
+        const int32_t k = static_cast<int32_t>(b * R::kBlockK);
+        ptx::mbar_arrive_expect_tx(bar, bytes);
+        ptx::tma_load_2d(at, &p.weights, bar, k, row);
+        ptx::tma_load_2d(at + kABytes / 2, &p.weights, bar, k,
+                         row + static_cast<int32_t>(a.inter));
+        uint32_t box = 0;
+        for (uint32_t left = groups; left != 0; left &= left - 1, ++box) {
+          const int32_t token = static_cast<int32_t>(kGroup * (__ffs(left) - 1));
 #pragma unroll
-  for (uint32_t m = 0; m < 2; ++m) {
-#pragma unroll
-    for (uint32_t n = 0; n < NT; ++n) {
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
-    }
-  }
-  const uint32_t steps = (a.hidden + kStep - 1) / kStep;
-  for (uint32_t s0 = wk * kUnroll; s0 < steps; s0 += WK * kUnroll) {
-    S w[kUnroll][2];
-#pragma unroll
-    for (uint32_t u = 0; u < kUnroll; ++u) {
-      const uint32_t k = (s0 + u) * kStep + t * kLane;
-      const size_t at = static_cast<size_t>(s0 + u) * kStepBytes;
-      const bool live = k < a.hidden;
-      w[u][0].lo = live ? load_weights(gate_lo + at) : zero4();
-      w[u][0].hi = live ? load_weights(gate_hi + at) : zero4();
-      w[u][1].lo = live ? load_weights(gate_lo + up_bytes + at) : zero4();
-      w[u][1].hi = live ? load_weights(gate_hi + up_bytes + at) : zero4();
-    }
-#pragma unroll
-    for (uint32_t u = 0; u < kUnroll; ++u) {
-      const uint32_t k = (s0 + u) * kStep + t * kLane;
-#pragma unroll
-      for (uint32_t n = 0; n < NT; ++n) {
-        if (n == 0 || n < tiles) {
-          uint4 b[S::kActs];
-          load_acts<INT8>(b, x_row[n], k, a.hidden);
-          w[u][0].multiply(acc[0][n], b);
-          w[u][1].multiply(acc[1][n], b);
+          for (uint32_t piece = 0; piece < R::kPieces; ++piece) {
+            ptx::tma_load_2d(at + kABytes + piece * R::kPieceBytes + box * kGroup * 128, &p.acts,
+                             bar, k + static_cast<int32_t>(64 * piece), token);
+          }
         }
       }
+      __syncwarp();
+      stage.next();
+    }
+  } else if (warp == 1) {
+    Cursor<R::kStages> stage;
+    Cursor<2> a_buf;
+    if (!issue_blocks<INT8, 1, R>(wait, bars, ring, stage, a_buf, tmem, tmem, n, end - begin,
+                                  bars.d_full[0])) {
+      if (lane == 0) report(a, 2);
+    }
+  } else if (warp >= 4) {
+    const uint32_t quad = warp & 3;
+    bool ok = true;
+    if constexpr (INT8) {
+      Cursor<R::kStages> stage;
+      Cursor<2> a_buf;
+      ok = convert_blocks<R>(wait, bars, ring, stage, a_buf, tmem, quad, lane, end - begin);
+      if (!ok && lane == 0) report(a, 3);
+    }
+    // Accumulator -> shared memory [column][row], over the ring: all of its bytes are used.
+    if (ok && wait(bars.d_full[0], 0)) {
+      ptx::tc_fence_after_sync();
+      const uint32_t to = ring + (quad * 32 + lane) * 4;
+#pragma unroll
+      for (uint32_t c = 0; c < COLS; c += 16) {
+        if (c < n) {
+          uint32_t v[16];
+          ptx::tmem_load_32x16(tmem + ((quad * 32) << 16) + c, v);
+          ptx::tmem_load_wait();
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) {
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + (c + i) * kRows * 4), "r"(v[i])
+                         : "memory");
+          }
+        }
+      }
+      ptx::tc_fence_before_sync();
+    } else if (lane == 0) {
+      report(a, 4);
     }
   }
+  __syncwarp();
+  settle(&abort_slot);
+  ptx::cluster_sync();
 
-  // Join the k shares in a fixed order and write weights * silu(gate) * up.
-  auto slot = [&](uint32_t k_share, uint32_t row_warp, uint32_t m, uint32_t n) {
-    return (((k_share * WR + row_warp) * 2 + m) * NT + n) * 32;
-  };
-#pragma unroll
-  for (uint32_t m = 0; m < 2; ++m) {
-#pragma unroll
-    for (uint32_t n = 0; n < NT; ++n) {
-      partial[slot(wk, wr, m, n) + lane] =
-          make_float4(acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]);
-    }
-  }
-  __syncthreads();
-  const float* const sums = reinterpret_cast<const float*>(partial);
-  for (uint32_t i = threadIdx.x; i < WR * tiles * 128; i += 32 * WR * WK) {
-    // element i: channel c of row group q, column p; rows run fastest
-    const uint32_t c = i % 16, p = (i / 16) % (tiles * 8), q = i / (16 * tiles * 8);
-    const uint32_t channel = (blockIdx.x * WR + q) * 16 + c;
-    if (p >= count || channel >= a.inter) continue;
-    // accumulator layout: lane (c % 8) * 4 + (p % 8) / 2, register 2 * (c / 8) + p % 2
-    const uint32_t in_tile = ((c % 8) * 4 + (p % 8) / 2) * 4 + 2 * (c / 8) + p % 2;
+  // Join the k shares in a fixed order; weights * silu(gate) * up in two BF16 halves.
+  for (uint32_t i = rank * kUpThreads + threadIdx.x; i < 64 * count; i += ranks * kUpThreads) {
+    const uint32_t c = i % 64, at = i / 64;
+    const uint32_t channel = channel0 + c;
+    if (channel >= a.inter) continue;
+    const uint32_t cell = ring + (list_column[at] * kRows + c) * 4;
     float gate = 0.0f, up = 0.0f;
-#pragma unroll
-    for (uint32_t s = 0; s < WK; ++s) {
-      gate += sums[slot(s, q, 0, p / 8) * 4 + in_tile];
-      up += sums[slot(s, q, 1, p / 8) * 4 + in_tile];
+    for (uint32_t s = 0; s < ranks; ++s) {
+      const uint32_t remote = ptx::map_to_cta(cell, s);
+      gate += ptx::ld_cluster_f32(remote);
+      up += ptx::ld_cluster_f32(remote + 64 * 4);
     }
     if constexpr (INT8) {
-      const float* const scale = a.s1 + first_row + channel;
+      const float* const scale = a.s1 + static_cast<size_t>(expert) * 2 * a.inter + channel;
       gate *= scale[0];
       up *= scale[a.inter];
     }
-    const float v = silu(gate) * up * list_coef[p];
+    const float v = gate / (1.0f + expf(-gate)) * up * token_coef[list_token[at]];
     // 16 significant bits in two BF16 numbers; an infinity has no remainder
     const uint16_t hi = to_bf16(v);
     const float rest = v - from_bf16(hi);
-    const size_t at = static_cast<size_t>(list_row[p]) * a.inter + channel;
-    a.h_hi[at] = hi;
-    a.h_lo[at] = to_bf16(isfinite(v) ? rest : 0.0f);
+    uint16_t* const to = a.h + static_cast<size_t>(list_base + at) * a.inter + channel;
+    to[0] = hi;
+    to[static_cast<size_t>(a.tokens) * a.top_k * a.inter] = to_bf16(isfinite(rest) ? rest : 0.0f);
+  }
+  ptx::fence_proxy_async_all();            // h is read by TMA
+  ptx::cluster_sync();                     // a neighbour may still read this CTA's tile
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem, (kUpTmem<INT8, COLS>));
   }
 }
 
 // ------------------------------------------------------------ down product --
 
-// A cluster computes 16 * MT * WR output channels for all tokens: WR warps side by side (MT
-// tiles of 16 rows each), and the chosen experts' k ranges, laid end to end, shared among
-// the cluster's CTAs x WK warps. Every warp sums into its own shared-memory tile [tokens][rows];
-// the tiles are joined in a fixed order, across the cluster through distributed shared memory.
-template <bool INT8, uint32_t NT, uint32_t MT, uint32_t WR, uint32_t WK>
-__global__ void __launch_bounds__(32 * WR * WK) decode_down_kernel(DecodeArgs a) {
-  using S = Step<INT8>;
-  constexpr uint32_t kStep = INT8 ? 64 : 32;
-  constexpr uint32_t kLane = INT8 ? 16 : 8;
-  constexpr uint32_t kRows = 16 * MT;                // rows of a warp
-  constexpr uint32_t kPitch = kRows + 8;             // floats between tokens of a tile
-  constexpr uint32_t kWarps = WR * WK;
-  extern __shared__ float4 dynamic[];
-  __shared__ uint32_t active_bits[BMOE_MOE_DECODE_MAX_EXPERTS / 32];
-  __shared__ uint16_t active[BMOE_MOE_DECODE_MAX_EXPERTS];
-  __shared__ uint32_t active_count;
-  __shared__ uint16_t list_row[kWarps][kMaxTokens];
-  __shared__ uint8_t list_token[kWarps][kMaxTokens];
-  float* const tile_all = reinterpret_cast<float*>(dynamic);      // [kWarps][tokens][kPitch]
-  int16_t* const ids = reinterpret_cast<int16_t*>(tile_all + kWarps * a.tokens * kPitch);
+template <bool INT8>
+constexpr uint32_t kDownThreads = INT8 ? 384 : 256;
 
+template <bool INT8, uint32_t COLS>
+using DownRing = Ring<INT8, COLS, 2, COLS * kRows * 4>;
+
+template <bool INT8, uint32_t COLS>
+constexpr uint32_t kDownTmem = INT8 ? 256 : 2 * COLS;
+
+// Lists in dynamic shared memory, per expert: token mask (8 bytes), assignments (4), and for
+// the chosen ones in ascending order id and first row of h (2 + 2).
+constexpr uint32_t kListBytes = 16;
+
+template <bool INT8, uint32_t COLS>
+uint32_t down_smem(uint32_t experts) {
+  using R = DownRing<INT8, COLS>;
+  return R::kStages * R::kStageBytes + COLS * kRows * 4 + experts * kListBytes + 1024;
+}
+
+// A cluster computes 128 output channels for all tokens: the chosen experts' k ranges, laid
+// end to end, are shared among its CTAs. A thread of the epilogue owns one channel and adds
+// every expert's accumulator columns to its tokens' sums in shared memory.
+template <bool INT8, uint32_t COLS>
+__global__ void __launch_bounds__(kDownThreads<INT8>, (DownRing<INT8, COLS>::kCtasPerSm))
+decode_down_kernel(const __grid_constant__ DecodeParams p) {
+  using R = DownRing<INT8, COLS>;
+  constexpr uint32_t kThreads = kDownThreads<INT8>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Barriers bars;
+  __shared__ uint32_t tmem_slot, abort_slot, active_count;
+  const DecodeArgs& a = p.a;
+  const uint32_t raw = ptx::smem_addr(smem_raw);
+  const uint32_t ring = (raw + 1023u) & ~1023u;
+  uint8_t* const behind = smem_raw + (ring - raw) + R::kStages * R::kStageBytes;
+  float* const sums = reinterpret_cast<float*>(behind);                  // [COLS][128]
+  uint32_t* const masks = reinterpret_cast<uint32_t*>(behind + COLS * kRows * 4);
+  uint32_t* const assigned = masks + 2 * a.experts;
+  uint16_t* const active = reinterpret_cast<uint16_t*>(assigned + a.experts);
+  uint16_t* const first_row = active + a.experts;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t assignments = a.tokens * a.top_k;
+  const Wait wait{&abort_slot};
 
-  // The chosen experts in ascending order.
-  if (threadIdx.x < BMOE_MOE_DECODE_MAX_EXPERTS / 32) active_bits[threadIdx.x] = 0;
-  for (uint32_t i = threadIdx.x; i < kWarps * a.tokens * kPitch; i += 32 * kWarps) {
-    tile_all[i] = 0.0f;
+  // Lists of the chosen experts; nothing here depends on the first kernel.
+  for (uint32_t i = threadIdx.x; i < 3 * a.experts; i += kThreads) masks[i] = 0;
+  for (uint32_t i = threadIdx.x; i < COLS * kRows; i += kThreads) sums[i] = 0.0f;
+  if (warp == 1) {
+    if (lane == 0) {
+      abort_slot = 0;
+      init_barriers(bars);
+    }
+    __syncwarp();
+    ptx::tmem_alloc(ptx::smem_addr(&tmem_slot), (kDownTmem<INT8, COLS>));
+    ptx::tmem_relinquish();
+  } else if (warp == 0 && lane == 0) {
+    ptx::tensormap_prefetch(&p.weights);
+    ptx::tensormap_prefetch(&p.acts);
   }
+  ptx::tc_fence_before_sync();
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < assignments; i += 32 * kWarps) {
+  ptx::tc_fence_after_sync();
+  for (uint32_t i = threadIdx.x; i < a.tokens * a.top_k; i += kThreads) {
     const int64_t e = a.ids[i];
-    const bool live = e >= 0 && e < a.experts;
-    ids[i] = live ? static_cast<int16_t>(e) : static_cast<int16_t>(-1);
-    if (live) atomicOr(&active_bits[e >> 5], 1u << (e & 31));
+    if (e >= 0 && e < a.experts) {
+      const uint32_t t = i / a.top_k;
+      atomicOr(&masks[2 * e + t / 32], 1u << (t % 32));
+      atomicAdd(&assigned[e], 1u);
+    }
   }
   __syncthreads();
   if (warp == 0) {
-    uint32_t bits = active_bits[lane];
-    uint32_t before = __popc(bits);
+    // experts lane * per ... of this lane: counts, then ids and rows behind a warp scan
+    const uint32_t per = (a.experts + 31) / 32;
+    const uint32_t from = min(lane * per, a.experts), to = min(from + per, a.experts);
+    uint32_t chosen = 0, rows = 0;
+    for (uint32_t e = from; e < to; ++e) {
+      chosen += assigned[e] != 0 ? 1u : 0u;
+      rows += assigned[e];
+    }
+    uint32_t chosen_end = chosen, rows_end = rows;
     for (uint32_t d = 1; d < 32; d <<= 1) {
-      const uint32_t v = __shfl_up_sync(kFullWarp, before, d);
-      if (lane >= d) before += v;
+      const uint32_t u = __shfl_up_sync(kFullWarp, chosen_end, d);
+      const uint32_t v = __shfl_up_sync(kFullWarp, rows_end, d);
+      if (lane >= d) {
+        chosen_end += u;
+        rows_end += v;
+      }
     }
-    if (lane == 31) active_count = before;
-    before -= __popc(bits);
-    while (bits != 0) {
-      active[before++] = static_cast<uint16_t>(lane * 32 + __ffs(bits) - 1);
-      bits &= bits - 1;
+    if (lane == 31) active_count = chosen_end;
+    uint32_t at = chosen_end - chosen, row = rows_end - rows;
+    for (uint32_t e = from; e < to; ++e) {
+      if (assigned[e] != 0) {
+        active[at] = static_cast<uint16_t>(e);
+        first_row[at] = static_cast<uint16_t>(row);
+        ++at;
+        row += assigned[e];
+      }
     }
   }
   __syncthreads();
-
-  uint32_t cta_rank, cta_count;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta_rank));
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(cta_count));
-  const uint32_t g = lane >> 2, t = lane & 3;
-  const uint32_t wr = warp % WR, wk = warp / WR;
-  const uint32_t group = blockIdx.x / cta_count;                  // of 16 * MT * WR rows
-  const uint32_t row0 = (group * WR + wr) * kRows;
-  const size_t row_bytes = static_cast<size_t>(a.inter) * (INT8 ? 1 : 2);
-  float* const tile = tile_all + warp * a.tokens * kPitch;
-
-  // This warp's share of the experts' k blocks, laid end to end.
-  const uint32_t steps = (a.inter + kStep - 1) / kStep;
-  const uint32_t blocks = (steps + kUnroll - 1) / kUnroll;        // of one expert
+  const uint32_t tmem = tmem_slot;
+  const uint32_t rank = ptx::cluster_cta_rank(), ranks = ptx::cluster_cta_count();
+  const uint32_t channel0 = blockIdx.x / ranks * kRows;
+  const uint32_t blocks = (a.inter + R::kBlockK - 1) / R::kBlockK;       // of one expert
   const uint32_t total = active_count * blocks;
-  const uint32_t workers = cta_count * WK, worker = cta_rank * WK + wk;
-  const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(total) * worker / workers);
-  const uint32_t end =
-      static_cast<uint32_t>(static_cast<uint64_t>(total) * (worker + 1) / workers);
+  const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(total) * rank / ranks);
+  const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(total) * (rank + 1) / ranks);
 
-  uint32_t row_of[MT][2];
+  // Columns of the expert at position `slot`, and how many of its blocks from `at` on are ours.
+  auto tokens_of = [&](uint32_t slot) {
+    const uint32_t e = active[slot];
+    return __popc(masks[2 * e]) + __popc(masks[2 * e + 1]);
+  };
+  auto run_of = [&](uint32_t at) { return min(end, (at / blocks + 1) * blocks) - at; };
+
+  if (warp == 0) {
+    const int32_t low_half = static_cast<int32_t>(a.tokens * a.top_k);
+    auto load_weights = [&](uint32_t at, uint32_t s) {
+      const uint32_t slot = at / blocks;
+      ptx::tma_load_2d(ring + s * R::kStageBytes, &p.weights, ptx::smem_addr(&bars.full[s]),
+                       static_cast<int32_t>((at - slot * blocks) * R::kBlockK),
+                       static_cast<int32_t>(active[slot] * a.hidden + channel0));
+    };
+    auto expect = [&](uint32_t at, uint32_t s) {
+      const uint32_t boxes = (tokens_of(at / blocks) + kGroup - 1) / kGroup;
+      ptx::mbar_arrive_expect_tx(ptx::smem_addr(&bars.full[s]),
+                                 kABytes + boxes * 2 * R::kPieces * kGroup * 128);
+    };
+    auto load_acts = [&](uint32_t at, uint32_t s) {
+      const uint32_t slot = at / blocks;
+      const uint32_t boxes = (tokens_of(slot) + kGroup - 1) / kGroup;
+      const int32_t k = static_cast<int32_t>((at - slot * blocks) * R::kBlockK);
+      const uint32_t to = ring + s * R::kStageBytes + kABytes;
+      const uint32_t bar = ptx::smem_addr(&bars.full[s]);
+      for (uint32_t box = 0; box < boxes; ++box) {
+        // rows beyond the expert's are other rows of h: columns that nobody reads
+        const int32_t row = static_cast<int32_t>(first_row[slot] + box * kGroup);
 #pragma unroll
-  for (uint32_t m = 0; m < MT; ++m) {
-    row_of[m][0] = min(row0 + m * 16 + g, a.hidden - 1);
-    row_of[m][1] = min(row0 + m * 16 + g + 8, a.hidden - 1);
-  }
-
-  bool waited = false;
-  uint32_t block = begin;
-  while (block < end) {
-    const uint32_t slot = block / blocks;
-    const uint32_t expert = active[slot];
-    const uint32_t stop = min(end, (slot + 1) * blocks);
-    // tokens of this expert, in ascending order (the first of two equal ids counts)
-    uint32_t count = 0;
-    __syncwarp();
-    for (uint32_t t0 = 0; t0 < a.tokens; t0 += 32) {
-      const uint32_t token = t0 + lane;
-      int first = -1;
-      if (token < a.tokens) {
-        for (uint32_t j = 0; j < a.top_k; ++j) {
-          if (first < 0 && ids[token * a.top_k + j] == static_cast<int>(expert)) {
-            first = static_cast<int>(token * a.top_k + j);
+        for (uint32_t plane = 0; plane < 2; ++plane) {
+#pragma unroll
+          for (uint32_t piece = 0; piece < R::kPieces; ++piece) {
+            ptx::tma_load_2d(
+                to + (plane * R::kPieces + piece) * R::kPieceBytes + box * kGroup * 128, &p.acts,
+                bar, k + static_cast<int32_t>(64 * piece),
+                row + (plane != 0 ? low_half : 0));
           }
         }
       }
-      const uint32_t mask = __ballot_sync(kFullWarp, first >= 0);
-      if (first >= 0) {
-        const uint32_t p = count + __popc(mask & ((1u << lane) - 1));
-        list_row[warp][p] = static_cast<uint16_t>(first);
-        list_token[warp][p] = static_cast<uint8_t>(token);
+    };
+    // The first stages' weights do not wait for the first kernel, their activations do.
+    const uint32_t ahead = min(begin + R::kStages, end);
+    if (ptx::elect_one()) {
+      for (uint32_t at = begin; at < ahead; ++at) {
+        expect(at, at - begin);
+        load_weights(at, at - begin);
       }
-      count += __popc(mask);
     }
     __syncwarp();
-    const uint32_t tiles = (count + 7) / 8;
-    size_t h_at[NT];
-    bool h_live[NT];
-#pragma unroll
-    for (uint32_t n = 0; n < NT; ++n) {
-      const uint32_t p = n * 8 + g;
-      h_live[n] = p < count;
-      h_at[n] = h_live[n] ? static_cast<size_t>(list_row[warp][p]) * a.inter : 0;
+    ptx::wait_for_previous_grid();
+    ptx::fence_proxy_async_all();
+    if (ptx::elect_one()) {
+      for (uint32_t at = begin; at < ahead; ++at) load_acts(at, at - begin);
     }
-    const uint8_t* w_at[MT][2];
-#pragma unroll
-    for (uint32_t m = 0; m < MT; ++m) {
-#pragma unroll
-      for (uint32_t i = 0; i < 2; ++i) {
-        w_at[m][i] = a.w2 + (static_cast<size_t>(expert) * a.hidden + row_of[m][i]) * row_bytes +
-                     16 * t;
+    __syncwarp();
+    Cursor<R::kStages> stage;
+    stage.parity = 1;                      // second use of every stage
+    for (uint32_t at = ahead; at < end; ++at) {
+      if (!wait(bars.empty[stage.slot], stage.parity ^ 1u)) {
+        if (lane == 0) report(a, 5);
+        break;
       }
-    }
-    float acc[MT][NT][4];
-#pragma unroll
-    for (uint32_t m = 0; m < MT; ++m) {
-#pragma unroll
-      for (uint32_t n = 0; n < NT; ++n) {
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
+      if (ptx::elect_one()) {
+        expect(at, stage.slot);
+        load_weights(at, stage.slot);
+        load_acts(at, stage.slot);
       }
+      __syncwarp();
+      stage.next();
     }
-    for (; block < stop; ++block) {
-      const uint32_t s0 = (block - slot * blocks) * kUnroll;
-      S w[kUnroll][MT];
-#pragma unroll
-      for (uint32_t u = 0; u < kUnroll; ++u) {
-        const uint32_t k = (s0 + u) * kStep + t * kLane;
-        const size_t at = static_cast<size_t>(s0 + u) * kStepBytes;
-#pragma unroll
-        for (uint32_t m = 0; m < MT; ++m) {
-          w[u][m].lo = k < a.inter ? load_weights(w_at[m][0] + at) : zero4();
-          w[u][m].hi = k < a.inter ? load_weights(w_at[m][1] + at) : zero4();
+  } else if (warp == 1) {
+    Cursor<R::kStages> stage;
+    Cursor<2> a_buf, d_buf;
+    for (uint32_t at = begin; at < end;) {
+      const uint32_t run = run_of(at);
+      const uint32_t n = (tokens_of(at / blocks) + 15) / 16 * 16;
+      if (!wait(bars.d_empty[d_buf.slot], d_buf.parity ^ 1u)) {
+        if (lane == 0) report(a, 6);
+        break;
+      }
+      ptx::tc_fence_after_sync();
+      if (!issue_blocks<INT8, 2, R>(wait, bars, ring, stage, a_buf, tmem,
+                                    tmem + d_buf.slot * COLS, n, run,
+                                    bars.d_full[d_buf.slot])) {
+        if (lane == 0) report(a, 7);
+        break;
+      }
+      d_buf.next();
+      at += run;
+    }
+  } else if (INT8 && warp >= 4 && warp < 8) {
+    Cursor<R::kStages> stage;
+    Cursor<2> a_buf;
+    if (!convert_blocks<R>(wait, bars, ring, stage, a_buf, tmem, warp & 3, lane, end - begin)) {
+      if (lane == 0) report(a, 8);
+    }
+  } else if (warp >= (INT8 ? 8 : 4)) {
+    const uint32_t quad = warp & 3;
+    const uint32_t row = quad * 32 + lane;
+    float* const mine = sums + row;
+    Cursor<2> d_buf;
+    for (uint32_t at = begin; at < end;) {
+      const uint32_t run = run_of(at);
+      const uint32_t e = active[at / blocks];
+      const uint32_t count = tokens_of(at / blocks);
+      unsigned long long left = static_cast<unsigned long long>(masks[2 * e + 1]) << 32 | masks[2 * e];
+      float scale = 1.0f;
+      if constexpr (INT8) {
+        if (channel0 + row < a.hidden) {
+          scale = a.s2[static_cast<size_t>(e) * a.hidden + channel0 + row];
         }
       }
-      if (!waited) {
-        // h comes from the first kernel; the weights above do not
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        waited = true;
+      if (!wait(bars.d_full[d_buf.slot], d_buf.parity)) {
+        if (lane == 0) report(a, 9);
+        break;
       }
+      ptx::tc_fence_after_sync();
+      const uint32_t from = tmem + ((quad * 32) << 16) + d_buf.slot * COLS;
 #pragma unroll
-      for (uint32_t u = 0; u < kUnroll; ++u) {
-        const uint32_t k = (s0 + u) * kStep + t * kLane;
+      for (uint32_t c = 0; c < COLS; c += 16) {
+        if (c < count) {
+          uint32_t v[16];
+          ptx::tmem_load_32x16(from + c, v);
+          ptx::tmem_load_wait();
 #pragma unroll
-        for (uint32_t n = 0; n < NT; ++n) {
-          if (n == 0 || n < tiles) {
-            uint4 b[S::kActs], rest[S::kActs];
-            load_acts<INT8>(b, h_live[n] ? a.h_hi + h_at[n] : nullptr, k, a.inter);
-            load_acts<INT8>(rest, h_live[n] ? a.h_lo + h_at[n] : nullptr, k, a.inter);
-#pragma unroll
-            for (uint32_t m = 0; m < MT; ++m) {
-              w[u][m].multiply(acc[m][n], b);
-              w[u][m].multiply(acc[m][n], rest);
+          for (uint32_t i = 0; i < 16; ++i) {
+            if (c + i < count) {
+              const uint32_t token = __ffsll(static_cast<long long>(left)) - 1;
+              left &= left - 1;
+              mine[token * kRows] = fmaf(__uint_as_float(v[i]), scale, mine[token * kRows]);
             }
           }
         }
       }
-    }
-    // into the warp's tile: columns p of this expert are tokens list_token[p]
-#pragma unroll
-    for (uint32_t m = 0; m < MT; ++m) {
-#pragma unroll
-      for (uint32_t n = 0; n < NT; ++n) {
-        if (n == 0 || n < tiles) {
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t p = n * 8 + 2 * t + (i & 1), half = i >> 1;
-            if (p < count) {
-              float v = acc[m][n][i];
-              if constexpr (INT8) {
-                v *= a.s2[static_cast<size_t>(expert) * a.hidden + row_of[m][half]];
-              }
-              tile[list_token[warp][p] * kPitch + m * 16 + g + 8 * half] += v;
-            }
-          }
-        }
-      }
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&bars.d_empty[d_buf.slot]));
+      d_buf.next();
+      at += run;
     }
   }
+  __syncwarp();
+  // No thread goes on before the first kernel has ended: out may be x, and this grid must
+  // not end first.
+  ptx::wait_for_previous_grid();
+  settle(&abort_slot);
+  ptx::cluster_sync();
 
-  // A warp without a share waits as well: this grid must not end before the first one.
-  if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  // Join the WK warps of this CTA, then the cluster's CTAs, each in ascending order.
-  __syncthreads();
-  constexpr uint32_t kCtaRows = kRows * WR;
-  const uint32_t cells = a.tokens * kCtaRows;
-  if constexpr (WK > 1) {
-    for (uint32_t i = threadIdx.x; i < cells; i += 32 * kWarps) {
-      const uint32_t token = i / kCtaRows, row = i % kCtaRows;
-      const uint32_t at = token * kPitch + row % kRows;
-      float sum = 0.0f;
-#pragma unroll
-      for (uint32_t s = 0; s < WK; ++s) {
-        sum += tile_all[(s * WR + row / kRows) * a.tokens * kPitch + at];
-      }
-      tile_all[row / kRows * a.tokens * kPitch + at] = sum;
-    }
-  }
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  const uint32_t tile_smem = static_cast<uint32_t>(__cvta_generic_to_shared(tile_all));
-  for (uint32_t i = cta_rank * 32 * kWarps + threadIdx.x; i < cells;
-       i += cta_count * 32 * kWarps) {
-    const uint32_t token = i / kCtaRows, row = i % kCtaRows;
-    const uint32_t channel = group * kCtaRows + row;
-    const uint32_t at =
-        tile_smem + 4 * ((row / kRows * a.tokens + token) * kPitch + row % kRows);
+  // Join the cluster's CTAs in a fixed order.
+  const uint32_t sums_smem = ptx::smem_addr(sums);
+  for (uint32_t i = rank * kThreads + threadIdx.x; i < a.tokens * kRows; i += ranks * kThreads) {
+    const uint32_t channel = channel0 + i % kRows;
     float sum = 0.0f;
-    for (uint32_t c = 0; c < cta_count; ++c) {
-      uint32_t remote;
-      float v;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(c));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
-      sum += v;
+    for (uint32_t s = 0; s < ranks; ++s) {
+      sum += ptx::ld_cluster_f32(ptx::map_to_cta(sums_smem + i * 4, s));
     }
-    if (channel < a.hidden) a.out[static_cast<size_t>(token) * a.hidden + channel] = to_bf16(sum);
+    if (channel < a.hidden) {
+      a.out[static_cast<size_t>(i / kRows) * a.hidden + channel] = to_bf16(sum);
+    }
   }
-  // nobody leaves while a neighbour still reads its tile
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  ptx::cluster_sync();                     // a neighbour may still read this CTA's sums
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem, (kDownTmem<INT8, COLS>));
+  }
 }
 
 // ------------------------------------------------------------------ launch --
 
-template <bool INT8, uint32_t NT, uint32_t WR, uint32_t WK>
-constexpr uint32_t up_smem() {
-  return WK * WR * 2 * NT * 32 * sizeof(float4);
+// CTAs along k: up to 8 (the portable cluster size) while the grid leaves room and every CTA
+// keeps two k-blocks.
+uint32_t split_of(uint64_t tiles, uint32_t blocks, uint32_t room) {
+  uint32_t split = 1;
+  while (split < 8 && tiles * split * 2 <= room && split * 4 <= blocks) split *= 2;
+  return split;
 }
 
-template <uint32_t MT, uint32_t WR, uint32_t WK>
-uint32_t down_smem(uint32_t tokens, uint32_t top_k) {
-  return WR * WK * tokens * (16 * MT + 8) * 4 + (tokens * top_k * 2 + 15) / 16 * 16;
-}
-
-// Opt-in shared memory is an attribute of a function on a device; setting it is cheap and
-// the same value every time, so every launch does it and nothing is cached.
 template <typename Kernel>
-cudaError_t allow_smem(Kernel kernel, uint32_t bytes) {
-  return bytes <= 48u * 1024u - 8192u
-             ? cudaSuccess
-             : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(bytes));
-}
-
-template <bool INT8, uint32_t NT, uint32_t MT, uint32_t WR, uint32_t WK>
-cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t stream) {
-  const uint32_t sms = device_sm_count();
-  {
-    constexpr uint32_t smem = up_smem<INT8, NT, WR, WK>();
-    const auto kernel = decode_up_kernel<INT8, NT, WR, WK>;
-    cudaError_t rc = allow_smem(kernel, smem);
-    if (rc != cudaSuccess) return rc;
-    const uint32_t slots = a.by_expert != 0 ? a.experts : a.tokens * a.top_k;
-    kernel<<<dim3((a.inter + 16 * WR - 1) / (16 * WR), slots), 32 * WR * WK, smem, stream>>>(a);
-    rc = cudaPeekAtLastError();
-    if (rc != cudaSuccess) return rc;
-  }
-  const uint32_t smem = down_smem<MT, WR, WK>(a.tokens, a.top_k);
-  const auto kernel = decode_down_kernel<INT8, NT, MT, WR, WK>;
-  cudaError_t rc = allow_smem(kernel, smem);
+cudaError_t launch_cluster(Kernel kernel, dim3 grid, uint32_t threads, uint32_t smem,
+                           uint32_t cluster, bool after_previous, const DecodeParams& params,
+                           cudaStream_t stream) {
+  // an attribute of the function on the current device: set per launch, nothing is cached
+  cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        static_cast<int>(smem));
   if (rc != cudaSuccess) return rc;
-  // enough CTAs for two per SM, in clusters of at most 8
-  const uint32_t groups = (a.hidden + 16 * MT * WR - 1) / (16 * MT * WR);
-  uint32_t cluster = 1;
-  while (cluster < 8 && groups * cluster < 2 * sms) cluster *= 2;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(groups * cluster);
-  config.blockDim = dim3(32 * WR * WK);
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attribute[2];
@@ -574,38 +769,60 @@ cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t stream) {
   attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
-  config.numAttrs = 2;
-  rc = cudaLaunchKernelEx(&config, kernel, a);
+  config.numAttrs = after_previous ? 2 : 1;
+  rc = cudaLaunchKernelEx(&config, kernel, params);
   return rc != cudaSuccess ? rc : cudaPeekAtLastError();
 }
 
-template <bool INT8>
-cudaError_t dispatch_decode(const DecodeArgs& a, cudaStream_t stream) {
-  if (a.tokens <= 8) return launch_decode<INT8, 1, 2, 1, 8>(a, stream);
-  if (a.tokens <= 32) return launch_decode<INT8, 4, 2, 2, 4>(a, stream);
-  return launch_decode<INT8, 8, 2, 4, 2>(a, stream);
+template <bool INT8, uint32_t COLS>
+cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cudaStream_t stream) {
+  const DecodeArgs& a = up.a;
+  const uint32_t sms = device_sm_count();
+  using U = UpRing<INT8, COLS>;
+  using D = DownRing<INT8, COLS>;
+  const uint32_t slots = a.by_expert != 0 ? a.experts : a.tokens * a.top_k;
+  const uint32_t tiles = (a.inter + 63) / 64;
+  uint32_t split = split_of(static_cast<uint64_t>(tiles) * slots,
+                            (a.hidden + U::kBlockK - 1) / U::kBlockK, 2 * U::kCtasPerSm * sms);
+  cudaError_t rc =
+      launch_cluster(decode_up_kernel<INT8, COLS>, dim3(tiles * split, slots), kUpThreads,
+                     kUpSmem<INT8, COLS>, split, false, up, stream);
+  if (rc != cudaSuccess) return rc;
+  const uint32_t groups = (a.hidden + kRows - 1) / kRows;
+  const uint64_t blocks =
+      static_cast<uint64_t>((a.inter + D::kBlockK - 1) / D::kBlockK) *
+      (slots < a.tokens * a.top_k ? slots : a.tokens * a.top_k);
+  split = split_of(groups, blocks < 64 ? static_cast<uint32_t>(blocks) : 64u,
+                   2 * D::kCtasPerSm * sms);
+  return launch_cluster(decode_down_kernel<INT8, COLS>, dim3(groups * split),
+                        kDownThreads<INT8>, down_smem<INT8, COLS>(a.experts), split, true, down,
+                        stream);
 }
 
-template <bool INT8, uint32_t NT, uint32_t MT, uint32_t WR, uint32_t WK>
+template <bool INT8>
+cudaError_t dispatch_decode(const DecodeParams& up, const DecodeParams& down,
+                            cudaStream_t stream) {
+  // columns that a stage has room for: what the tokens need
+  if (up.a.tokens <= 16) return launch_decode<INT8, 16>(up, down, stream);
+  if (up.a.tokens <= 32) return launch_decode<INT8, 32>(up, down, stream);
+  return launch_decode<INT8, 64>(up, down, stream);
+}
+
+template <bool INT8, uint32_t COLS>
 cudaError_t preload_decode() {
-  const cudaError_t rc = preload_one(decode_up_kernel<INT8, NT, WR, WK>);
-  return rc == cudaSuccess ? preload_one(decode_down_kernel<INT8, NT, MT, WR, WK>) : rc;
+  const cudaError_t rc = preload_one(decode_up_kernel<INT8, COLS>);
+  return rc == cudaSuccess ? preload_one(decode_down_kernel<INT8, COLS>) : rc;
 }
 
 template <bool INT8>
 cudaError_t preload_decode_type() {
-  cudaError_t rc = preload_decode<INT8, 1, 2, 1, 8>();
-  if (rc == cudaSuccess) rc = preload_decode<INT8, 4, 2, 2, 4>();
-  if (rc == cudaSuccess) rc = preload_decode<INT8, 8, 2, 4, 2>();
+  cudaError_t rc = preload_decode<INT8, 16>();
+  if (rc == cudaSuccess) rc = preload_decode<INT8, 32>();
+  if (rc == cudaSuccess) rc = preload_decode<INT8, 64>();
   return rc;
 }
 
 bool unaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
-
-// Bytes of one BF16 plane of h.
-uint64_t plane_bytes(uint32_t tokens, uint32_t top_k, uint32_t inter) {
-  return (static_cast<uint64_t>(tokens) * top_k * inter * 2 + 255) / 256 * 256;
-}
 
 }  // namespace
 
@@ -617,7 +834,7 @@ cudaError_t preload_decode_kernels() {
 }  // namespace bmoe
 
 extern "C" uint64_t bmoe_moe_decode_workspace(uint32_t tokens, uint32_t top_k, uint32_t inter) {
-  return 2 * bmoe::plane_bytes(tokens, top_k, inter);
+  return (2ull * tokens * top_k * inter * sizeof(uint16_t) + 255) / 256 * 256;
 }
 
 extern "C" int bmoe_moe_decode(const bmoe_moe_decode_args* args) {
@@ -645,26 +862,37 @@ extern "C" int bmoe_moe_decode(const bmoe_moe_decode_args* args) {
       (int8 && (a.gate_up_scale_dev == nullptr || a.down_scale_dev == nullptr))) {
     return BMOE_INVALID_ARGUMENT;
   }
-  bmoe::DecodeArgs k;
-  k.x = static_cast<const uint16_t*>(a.x_dev);
-  k.w1 = static_cast<const uint8_t*>(a.w_gate_up_dev);
-  k.w2 = static_cast<const uint8_t*>(a.w_down_dev);
+  bmoe::DecodeParams up;
+  bmoe::DecodeArgs& k = up.a;
   k.s1 = a.gate_up_scale_dev;
   k.s2 = a.down_scale_dev;
   k.ids = a.expert_ids_dev;
   k.coef = a.weights_dev;
   k.out = static_cast<uint16_t*>(a.out_dev);
-  k.h_hi = static_cast<uint16_t*>(a.workspace_dev);
-  k.h_lo = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(a.workspace_dev) +
-                                       bmoe::plane_bytes(a.tokens, a.top_k, a.inter));
+  k.h = static_cast<uint16_t*>(a.workspace_dev);
+  k.status = a.status_dev;
   k.tokens = a.tokens;
   k.top_k = a.top_k;
   k.experts = a.experts;
   k.hidden = a.hidden;
   k.inter = a.inter;
   k.by_expert = a.experts <= a.tokens * a.top_k ? 1u : 0u;
+  bmoe::DecodeParams down;
+  down.a = k;
+  const bmoe::Elem weight = int8 ? bmoe::Elem::kByte : bmoe::Elem::kBf16;
+  if (!bmoe::encode_matrix(&up.weights, a.w_gate_up_dev, 2ull * a.experts * a.inter, a.hidden, 64,
+                           weight) ||
+      !bmoe::encode_matrix(&up.acts, a.x_dev, a.tokens, a.hidden, bmoe::kGroup,
+                           bmoe::Elem::kBf16) ||
+      !bmoe::encode_matrix(&down.weights, a.w_down_dev,
+                           static_cast<uint64_t>(a.experts) * a.hidden, a.inter, bmoe::kRows,
+                           weight) ||
+      !bmoe::encode_matrix(&down.acts, a.workspace_dev, 2ull * a.tokens * a.top_k, a.inter,
+                           bmoe::kGroup, bmoe::Elem::kBf16)) {
+    return BMOE_CUDA_ERROR;
+  }
   const cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
-  const cudaError_t rc = int8 ? bmoe::dispatch_decode<true>(k, stream)
-                              : bmoe::dispatch_decode<false>(k, stream);
+  const cudaError_t rc = int8 ? bmoe::dispatch_decode<true>(up, down, stream)
+                              : bmoe::dispatch_decode<false>(up, down, stream);
   return rc == cudaSuccess ? BMOE_OK : BMOE_CUDA_ERROR;
 }
