@@ -10,10 +10,12 @@
 // keeps enough bytes in flight to hold HBM busy while CTAs come and go.
 //   warp 0     TMA producer
 //   warp 1     MMA issuer (one elected lane), Tensor Memory
-//   warps 4-7  BF16 weights: epilogue
-//              INT8 weights: shared memory -> BF16 -> Tensor Memory, the A operand of the
-//              MMA (a signed byte is a BF16 value, so the conversion is exact); the first
-//              kernel's epilogue; the second kernel has warps 8-11 for it
+//   warps 4-7  epilogue (BF16 weights)
+//   warps 4-11 INT8 weights: shared memory -> BF16 -> Tensor Memory, the A operand of the
+//              MMA (a signed byte is a BF16 value, so the conversion is exact). The first
+//              kernel's warps 4-7 are its epilogue afterwards, the second has warps 12-15
+// h keeps 16 significant bits as two BF16 numbers whose products are added: the upper and
+// the lower halves of the tokens are separate columns of the same MMA.
 // Few tiles are split along k over the CTAs of a cluster, joined in a fixed order through
 // distributed shared memory: no atomics, the same bits on every run.
 #include <cuda.h>
@@ -36,7 +38,7 @@ constexpr uint32_t kABytes = kRows * 128;        // one k-block of weights: 128 
 constexpr uint32_t kGroup = 8;                   // tokens of one activation box
 constexpr uint32_t kTwoPerSm = 108u * 1024u;     // shared memory of a CTA that shares its SM
 constexpr uint32_t kOnePerSm = 208u * 1024u;
-constexpr uint32_t kTmemA = 128;                 // first column of the INT8 A operand
+constexpr uint32_t kTmemA = 128;                 // columns of the INT8 A operand, in front
 constexpr uint64_t kWaitBudgetNs = 1000000000ull;
 
 struct DecodeArgs {
@@ -66,8 +68,8 @@ template <bool INT8, uint32_t COLS, uint32_t PLANES, uint32_t RESERVED>
 struct Ring {
   static constexpr uint32_t kPieces = INT8 ? 2 : 1;
   static constexpr uint32_t kBlockK = 64 * kPieces;
-  static constexpr uint32_t kPieceBytes = COLS * 128;
-  static constexpr uint32_t kStageBytes = kABytes + PLANES * kPieces * kPieceBytes;
+  static constexpr uint32_t kPieceBytes = PLANES * COLS * 128;
+  static constexpr uint32_t kStageBytes = kABytes + kPieces * kPieceBytes;
   static constexpr uint32_t kTwo = (kTwoPerSm - RESERVED) / kStageBytes;
   static constexpr uint32_t kOne = (kOnePerSm - RESERVED) / kStageBytes;
   // Two CTAs per SM if each keeps three stages: while one starts or ends, the other streams.
@@ -130,7 +132,7 @@ __device__ __forceinline__ float from_bf16(uint16_t v) {
 
 // MMA issuer: `blocks` k-blocks into the accumulator at `d_tmem` (n columns). Returns false
 // when a wait gave up. The warp is converged; one elected lane issues.
-template <bool INT8, uint32_t PLANES, typename R>
+template <bool INT8, typename R>
 __device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars, uint32_t ring,
                                              Cursor<R::kStages>& stage, Cursor<2>& a_buf,
                                              uint32_t tmem, uint32_t d_tmem, uint32_t n,
@@ -142,22 +144,19 @@ __device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars, u
     ptx::tc_fence_after_sync();
     const uint32_t at = ring + stage.slot * R::kStageBytes;
     const uint64_t a_desc = ptx::make_kmajor_sw128_desc(at);
-    const uint32_t a_tmem = tmem + kTmemA + a_buf.slot * 64;
+    const uint32_t a_tmem = tmem + a_buf.slot * (kTmemA / 2);
     if (ptx::elect_one()) {
 #pragma unroll
       for (uint32_t piece = 0; piece < R::kPieces; ++piece) {
+        const uint64_t b_desc =
+            ptx::make_kmajor_sw128_desc(at + kABytes + piece * R::kPieceBytes);
 #pragma unroll
         for (uint32_t ks = 0; ks < 4; ++ks) {
-#pragma unroll
-          for (uint32_t plane = 0; plane < PLANES; ++plane) {
-            const uint64_t b_desc = ptx::make_kmajor_sw128_desc(
-                at + kABytes + (plane * R::kPieces + piece) * R::kPieceBytes);
-            const uint32_t acc = (b | piece | ks | plane) != 0 ? 1u : 0u;
-            if constexpr (INT8) {
-              ptx::umma_bf16_ts(d_tmem, a_tmem + (piece * 4 + ks) * 8, b_desc + 2 * ks, idesc, acc);
-            } else {
-              ptx::umma_bf16_ss(d_tmem, a_desc + 2 * ks, b_desc + 2 * ks, idesc, acc);
-            }
+          const uint32_t acc = (b | piece | ks) != 0 ? 1u : 0u;
+          if constexpr (INT8) {
+            ptx::umma_bf16_ts(d_tmem, a_tmem + (piece * 4 + ks) * 8, b_desc + 2 * ks, idesc, acc);
+          } else {
+            ptx::umma_bf16_ss(d_tmem, a_desc + 2 * ks, b_desc + 2 * ks, idesc, acc);
           }
         }
       }
@@ -172,36 +171,34 @@ __device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars, u
   return true;
 }
 
-// INT8: one warp's 32 rows of `blocks` k-blocks from shared memory to Tensor Memory as BF16.
+// INT8: half of one warp's 32 rows of `blocks` k-blocks from shared memory to Tensor Memory as
+// BF16. Two warps share 32 rows: one alone measured half the rate HBM delivers.
 template <typename R>
 __device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars, uint32_t ring,
                                                Cursor<R::kStages>& stage, Cursor<2>& a_buf,
-                                               uint32_t tmem, uint32_t quad, uint32_t lane,
-                                               uint32_t blocks) {
+                                               uint32_t tmem, uint32_t quad, uint32_t half,
+                                               uint32_t lane, uint32_t blocks) {
   for (uint32_t b = 0; b < blocks; ++b) {
     if (!wait(bars.full[stage.slot], stage.parity)) return false;
     if (!wait(bars.a_empty[a_buf.slot], a_buf.parity ^ 1u)) return false;
     ptx::tc_fence_after_sync();
     const uint32_t row = ring + stage.slot * R::kStageBytes + (quad * 32 + lane) * 128;
-    const uint32_t to = tmem + kTmemA + a_buf.slot * 64 + ((quad * 32) << 16);
+    const uint32_t to = tmem + a_buf.slot * (kTmemA / 2) + ((quad * 32) << 16);
+    uint32_t v[32];
 #pragma unroll
-    for (uint32_t half = 0; half < 2; ++half) {
-      uint32_t v[32];
-#pragma unroll
-      for (uint32_t c = 0; c < 4; ++c) {
-        // 16-byte pieces of a 128-byte row are swizzled by the row's place in its group of 8
-        const uint4 w = ptx::ld_shared_v4(row + (((half * 4 + c) ^ (lane & 7)) << 4));
-        v[8 * c + 0] = int8_pair(w.x, 0x4140);
-        v[8 * c + 1] = int8_pair(w.x, 0x4342);
-        v[8 * c + 2] = int8_pair(w.y, 0x4140);
-        v[8 * c + 3] = int8_pair(w.y, 0x4342);
-        v[8 * c + 4] = int8_pair(w.z, 0x4140);
-        v[8 * c + 5] = int8_pair(w.z, 0x4342);
-        v[8 * c + 6] = int8_pair(w.w, 0x4140);
-        v[8 * c + 7] = int8_pair(w.w, 0x4342);
-      }
-      ptx::tmem_store_32x32(to + half * 32, v);
+    for (uint32_t c = 0; c < 4; ++c) {
+      // 16-byte pieces of a 128-byte row are swizzled by the row's place in its group of 8
+      const uint4 w = ptx::ld_shared_v4(row + (((half * 4 + c) ^ (lane & 7)) << 4));
+      v[8 * c + 0] = int8_pair(w.x, 0x4140);
+      v[8 * c + 1] = int8_pair(w.x, 0x4342);
+      v[8 * c + 2] = int8_pair(w.y, 0x4140);
+      v[8 * c + 3] = int8_pair(w.y, 0x4342);
+      v[8 * c + 4] = int8_pair(w.z, 0x4140);
+      v[8 * c + 5] = int8_pair(w.z, 0x4342);
+      v[8 * c + 6] = int8_pair(w.w, 0x4140);
+      v[8 * c + 7] = int8_pair(w.w, 0x4342);
     }
+    ptx::tmem_store_32x32(to + half * 32, v);
     ptx::tmem_store_wait();
     ptx::tc_fence_before_sync();
     __syncwarp();
@@ -218,7 +215,7 @@ __device__ __forceinline__ void init_barriers(Barriers& bars) {
     ptx::mbar_init(ptx::smem_addr(&bars.empty[s]), 1);
   }
   for (uint32_t b = 0; b < 2; ++b) {
-    ptx::mbar_init(ptx::smem_addr(&bars.a_full[b]), 4);    // converting warps
+    ptx::mbar_init(ptx::smem_addr(&bars.a_full[b]), 8);    // converting warps
     ptx::mbar_init(ptx::smem_addr(&bars.a_empty[b]), 1);
     ptx::mbar_init(ptx::smem_addr(&bars.d_full[b]), 1);
     ptx::mbar_init(ptx::smem_addr(&bars.d_empty[b]), 4);   // epilogue warps
@@ -235,7 +232,8 @@ __device__ __forceinline__ void settle(volatile uint32_t* abort_word) {
 
 // --------------------------------------------------- gate and up products --
 
-constexpr uint32_t kUpThreads = 256;
+template <bool INT8>
+constexpr uint32_t kUpThreads = INT8 ? 384 : 256;
 
 template <bool INT8, uint32_t COLS>
 using UpRing = Ring<INT8, COLS, 1, 0>;
@@ -250,7 +248,7 @@ constexpr uint32_t kUpTmem = INT8 ? 256 : (COLS < 32 ? 32 : COLS);
 // are the channels' gate rows, 64-127 their up rows. Activations come in boxes of 8 tokens, only
 // those that hold a token of the expert.
 template <bool INT8, uint32_t COLS>
-__global__ void __launch_bounds__(kUpThreads, (UpRing<INT8, COLS>::kCtasPerSm))
+__global__ void __launch_bounds__(kUpThreads<INT8>, (UpRing<INT8, COLS>::kCtasPerSm))
 decode_up_kernel(const __grid_constant__ DecodeParams p) {
   using R = UpRing<INT8, COLS>;
   extern __shared__ uint8_t smem_raw[];
@@ -348,6 +346,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
   for (uint32_t i = 0; i < 8; ++i) {
     if (((mask[i / 4] >> (8 * (i % 4))) & 0xffu) != 0) groups |= 1u << i;
   }
+  const uint32_t d_tmem = tmem + (INT8 ? kTmemA : 0);
   const uint32_t boxes = __popc(groups);
   const uint32_t n = (boxes + 1) / 2 * 16;         // columns of the MMA: a multiple of 16
 
@@ -389,8 +388,8 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
   } else if (warp == 1) {
     Cursor<R::kStages> stage;
     Cursor<2> a_buf;
-    if (!issue_blocks<INT8, 1, R>(wait, bars, ring, stage, a_buf, tmem, tmem, n, end - begin,
-                                  bars.d_full[0])) {
+    if (!issue_blocks<INT8, R>(wait, bars, ring, stage, a_buf, tmem, d_tmem, n, end - begin,
+                               bars.d_full[0])) {
       if (lane == 0) report(a, 2);
     }
   } else if (warp >= 4) {
@@ -399,18 +398,20 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
     if constexpr (INT8) {
       Cursor<R::kStages> stage;
       Cursor<2> a_buf;
-      ok = convert_blocks<R>(wait, bars, ring, stage, a_buf, tmem, quad, lane, end - begin);
+      ok = convert_blocks<R>(wait, bars, ring, stage, a_buf, tmem, quad, (warp - 4) / 4, lane,
+                             end - begin);
       if (!ok && lane == 0) report(a, 3);
     }
     // Accumulator -> shared memory [column][row], over the ring: all of its bytes are used.
-    if (ok && wait(bars.d_full[0], 0)) {
+    if (warp >= 8) {
+    } else if (ok && wait(bars.d_full[0], 0)) {
       ptx::tc_fence_after_sync();
       const uint32_t to = ring + (quad * 32 + lane) * 4;
 #pragma unroll
       for (uint32_t c = 0; c < COLS; c += 16) {
         if (c < n) {
           uint32_t v[16];
-          ptx::tmem_load_32x16(tmem + ((quad * 32) << 16) + c, v);
+          ptx::tmem_load_32x16(d_tmem + ((quad * 32) << 16) + c, v);
           ptx::tmem_load_wait();
 #pragma unroll
           for (uint32_t i = 0; i < 16; ++i) {
@@ -429,7 +430,8 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
   ptx::cluster_sync();
 
   // Join the k shares in a fixed order; weights * silu(gate) * up in two BF16 halves.
-  for (uint32_t i = rank * kUpThreads + threadIdx.x; i < 64 * count; i += ranks * kUpThreads) {
+  for (uint32_t i = rank * kUpThreads<INT8> + threadIdx.x; i < 64 * count;
+       i += ranks * kUpThreads<INT8>) {
     const uint32_t c = i % 64, at = i / 64;
     const uint32_t channel = channel0 + c;
     if (channel >= a.inter) continue;
@@ -464,13 +466,13 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
 // ------------------------------------------------------------ down product --
 
 template <bool INT8>
-constexpr uint32_t kDownThreads = INT8 ? 384 : 256;
+constexpr uint32_t kDownThreads = INT8 ? 512 : 256;
 
 template <bool INT8, uint32_t COLS>
 using DownRing = Ring<INT8, COLS, 2, COLS * kRows * 4>;
 
 template <bool INT8, uint32_t COLS>
-constexpr uint32_t kDownTmem = INT8 ? 256 : 2 * COLS;
+constexpr uint32_t kDownTmem = INT8 ? (COLS == 64 ? 512 : 256) : 4 * COLS;
 
 // Lists in dynamic shared memory, per expert: token mask (8 bytes), assignments (4), and for
 // the chosen ones in ascending order id and first row of h (2 + 2).
@@ -565,6 +567,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
   const uint32_t tmem = tmem_slot;
   const uint32_t rank = ptx::cluster_cta_rank(), ranks = ptx::cluster_cta_count();
   const uint32_t channel0 = blockIdx.x / ranks * kRows;
+  const uint32_t d_tmem = tmem + (INT8 ? kTmemA : 0);
   const uint32_t blocks = (a.inter + R::kBlockK - 1) / R::kBlockK;       // of one expert
   const uint32_t total = active_count * blocks;
   const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(total) * rank / ranks);
@@ -604,8 +607,8 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
 #pragma unroll
           for (uint32_t piece = 0; piece < R::kPieces; ++piece) {
             ptx::tma_load_2d(
-                to + (plane * R::kPieces + piece) * R::kPieceBytes + box * kGroup * 128, &p.acts,
-                bar, k + static_cast<int32_t>(64 * piece),
+                to + piece * R::kPieceBytes + (plane * boxes + box) * kGroup * 128, &p.acts, bar,
+                k + static_cast<int32_t>(64 * piece),
                 row + (plane != 0 ? low_half : 0));
           }
         }
@@ -646,28 +649,29 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
     Cursor<2> a_buf, d_buf;
     for (uint32_t at = begin; at < end;) {
       const uint32_t run = run_of(at);
-      const uint32_t n = (tokens_of(at / blocks) + 15) / 16 * 16;
+      const uint32_t n = (tokens_of(at / blocks) + kGroup - 1) / kGroup * 2 * kGroup;
       if (!wait(bars.d_empty[d_buf.slot], d_buf.parity ^ 1u)) {
         if (lane == 0) report(a, 6);
         break;
       }
       ptx::tc_fence_after_sync();
-      if (!issue_blocks<INT8, 2, R>(wait, bars, ring, stage, a_buf, tmem,
-                                    tmem + d_buf.slot * COLS, n, run,
-                                    bars.d_full[d_buf.slot])) {
+      if (!issue_blocks<INT8, R>(wait, bars, ring, stage, a_buf, tmem,
+                                 d_tmem + d_buf.slot * 2 * COLS, n, run,
+                                 bars.d_full[d_buf.slot])) {
         if (lane == 0) report(a, 7);
         break;
       }
       d_buf.next();
       at += run;
     }
-  } else if (INT8 && warp >= 4 && warp < 8) {
+  } else if (INT8 && warp >= 4 && warp < 12) {
     Cursor<R::kStages> stage;
     Cursor<2> a_buf;
-    if (!convert_blocks<R>(wait, bars, ring, stage, a_buf, tmem, warp & 3, lane, end - begin)) {
+    if (!convert_blocks<R>(wait, bars, ring, stage, a_buf, tmem, warp & 3, (warp - 4) / 4, lane,
+                           end - begin)) {
       if (lane == 0) report(a, 8);
     }
-  } else if (warp >= (INT8 ? 8 : 4)) {
+  } else if (warp >= (INT8 ? 12 : 4)) {
     const uint32_t quad = warp & 3;
     const uint32_t row = quad * 32 + lane;
     float* const mine = sums + row;
@@ -688,20 +692,20 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
         break;
       }
       ptx::tc_fence_after_sync();
-      const uint32_t from = tmem + ((quad * 32) << 16) + d_buf.slot * COLS;
+      const uint32_t from = d_tmem + ((quad * 32) << 16) + d_buf.slot * 2 * COLS;
+      const uint32_t boxes = (count + kGroup - 1) / kGroup;
+      for (uint32_t c = 0; c < boxes * kGroup; c += kGroup) {
+        uint32_t upper[kGroup], lower[kGroup];
+        ptx::tmem_load_32x8(from + c, upper);
+        ptx::tmem_load_32x8(from + boxes * kGroup + c, lower);
+        ptx::tmem_load_wait();
 #pragma unroll
-      for (uint32_t c = 0; c < COLS; c += 16) {
-        if (c < count) {
-          uint32_t v[16];
-          ptx::tmem_load_32x16(from + c, v);
-          ptx::tmem_load_wait();
-#pragma unroll
-          for (uint32_t i = 0; i < 16; ++i) {
-            if (c + i < count) {
-              const uint32_t token = __ffsll(static_cast<long long>(left)) - 1;
-              left &= left - 1;
-              mine[token * kRows] = fmaf(__uint_as_float(v[i]), scale, mine[token * kRows]);
-            }
+        for (uint32_t i = 0; i < kGroup; ++i) {
+          if (c + i < count) {
+            const uint32_t token = __ffsll(static_cast<long long>(left)) - 1;
+            left &= left - 1;
+            const float v = __uint_as_float(upper[i]) + __uint_as_float(lower[i]);
+            mine[token * kRows] = fmaf(v, scale, mine[token * kRows]);
           }
         }
       }
@@ -785,7 +789,7 @@ cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cuda
   uint32_t split = split_of(static_cast<uint64_t>(tiles) * slots,
                             (a.hidden + U::kBlockK - 1) / U::kBlockK, 2 * U::kCtasPerSm * sms);
   cudaError_t rc =
-      launch_cluster(decode_up_kernel<INT8, COLS>, dim3(tiles * split, slots), kUpThreads,
+      launch_cluster(decode_up_kernel<INT8, COLS>, dim3(tiles * split, slots), kUpThreads<INT8>,
                      kUpSmem<INT8, COLS>, split, false, up, stream);
   if (rc != cudaSuccess) return rc;
   const uint32_t groups = (a.hidden + kRows - 1) / kRows;

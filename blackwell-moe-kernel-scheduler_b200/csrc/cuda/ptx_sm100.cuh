@@ -385,6 +385,16 @@ __device__ __forceinline__ void tmem_load_32x16(uint32_t taddr, uint32_t (&v)[16
       : "memory");
 }
 
+// The same for 8 columns.
+__device__ __forceinline__ void tmem_load_32x8(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
+        "=r"(v[6]), "=r"(v[7])
+      : "r"(taddr)
+      : "memory");
+}
+
 // Warp-collective: writes 32 lanes x 32 consecutive 32-bit columns starting at taddr.
 __device__ __forceinline__ void tmem_store_32x32(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
