@@ -36,8 +36,9 @@ constexpr uint32_t kMaxTokens = BMOE_MOE_DECODE_MAX_TOKENS;
 constexpr uint32_t kRows = 128;                  // weight rows of a tile
 constexpr uint32_t kABytes = kRows * 128;        // one k-block of weights: 128 bytes of a row
 constexpr uint32_t kGroup = 8;                   // tokens of one activation box
-constexpr uint32_t kTwoPerSm = 108u * 1024u;     // shared memory of a CTA that shares its SM
-constexpr uint32_t kOnePerSm = 208u * 1024u;
+constexpr uint32_t kTwoPerSm = 110u * 1024u;     // dynamic shared memory of a CTA that shares
+constexpr uint32_t kOnePerSm = 222u * 1024u;     // its SM, and of one that does not
+constexpr uint32_t kMaxStages = 12;
 constexpr uint32_t kTmemA = 128;                 // columns of the INT8 A operand, in front
 constexpr uint64_t kWaitBudgetNs = 1000000000ull;
 
@@ -61,26 +62,30 @@ struct DecodeParams {
   DecodeArgs a;
 };
 
-// Stages of one CTA. COLS: columns (tokens) a stage has room for; PLANES: 1 (x) or 2 (the two
-// halves of h). A k-block is 128 bytes of every weight row: 64 BF16 or 128 INT8 values, against
-// one or two 128-byte wide pieces of the activations.
-template <bool INT8, uint32_t COLS, uint32_t PLANES, uint32_t RESERVED>
-struct Ring {
+// A k-block is 128 bytes of every weight row: 64 BF16 or 128 INT8 values, against one or two
+// 128-byte wide pieces of the activations.
+template <bool INT8>
+struct Block {
   static constexpr uint32_t kPieces = INT8 ? 2 : 1;
-  static constexpr uint32_t kBlockK = 64 * kPieces;
-  static constexpr uint32_t kPieceBytes = PLANES * COLS * 128;
-  static constexpr uint32_t kStageBytes = kABytes + kPieces * kPieceBytes;
-  static constexpr uint32_t kTwo = (kTwoPerSm - RESERVED) / kStageBytes;
-  static constexpr uint32_t kOne = (kOnePerSm - RESERVED) / kStageBytes;
-  // Two CTAs per SM if each keeps three stages: while one starts or ends, the other streams.
-  static constexpr uint32_t kCtasPerSm = kTwo >= 3 ? 2 : 1;
-  static constexpr uint32_t kStages = kCtasPerSm == 2 ? (kTwo < 6 ? kTwo : 6) : (kOne < 6 ? kOne : 6);
-  static_assert(kStages >= 2, "ring");
+  static constexpr uint32_t kK = 64 * kPieces;
+};
+
+// Stages of one CTA: the columns that its experts really need decide how many fit.
+template <bool INT8>
+struct Ring {
+  uint32_t base, piece_bytes, stage_bytes, stages;
+  // columns: a multiple of 16, at least as many as any MMA of the CTA has
+  __device__ __forceinline__ Ring(uint32_t at, uint32_t bytes, uint32_t columns)
+      : base(at),
+        piece_bytes(columns * 128),
+        stage_bytes(kABytes + Block<INT8>::kPieces * columns * 128),
+        stages(min(bytes / stage_bytes, kMaxStages)) {}
+  __device__ __forceinline__ uint32_t at(uint32_t slot) const { return base + slot * stage_bytes; }
 };
 
 // Barriers of a CTA (static shared memory).
 struct Barriers {
-  uint64_t full[6], empty[6];     // stage: bytes landed / MMAs done with it
+  uint64_t full[kMaxStages], empty[kMaxStages];   // stage: bytes landed / MMAs done with it
   uint64_t a_full[2], a_empty[2]; // INT8: converted weights in Tensor Memory / read by the MMAs
   uint64_t d_full[2], d_empty[2]; // accumulator: complete / drained
 };
@@ -92,12 +97,11 @@ struct Wait {
   }
 };
 
-// Position in a ring of `N` slots: slot and the parity of its current use.
-template <uint32_t N>
+// Position in a ring of slots: slot and the parity of its current use.
 struct Cursor {
   uint32_t slot = 0, parity = 0;
-  __device__ __forceinline__ void next() {
-    if (++slot == N) {
+  __device__ __forceinline__ void next(uint32_t slots) {
+    if (++slot == slots) {
       slot = 0;
       parity ^= 1u;
     }
@@ -110,7 +114,9 @@ __device__ __forceinline__ void report(const DecodeArgs& a, uint32_t site) {
 
 // Two signed bytes of `word` (selector 0x4140: bytes 0, 1; 0x4342: bytes 2, 3) -> BF16 pair,
 // exact. With v = 128 + (b & 127) as the bits 0x4300 | (b & 0x7f), and 128 or 256 as the bits
-// 0x4300 | (b & 0x80), the signed value is their difference.
+// 0x4300 | (b & 0x80), the signed value is their difference. (One permutation and three FMAs
+// do it without the masks: f = bits 0x43 u of u = b + 128, q = f / 2 - 128, value
+// q - max(0, -q); measured 11 % more cycles per block.)
 __device__ __forceinline__ uint32_t int8_pair(uint32_t word, uint32_t selector) {
   const uint32_t both = __byte_perm(word, 0x43434343u, selector);
   uint32_t r;
@@ -132,9 +138,9 @@ __device__ __forceinline__ float from_bf16(uint16_t v) {
 
 // MMA issuer: `blocks` k-blocks into the accumulator at `d_tmem` (n columns). Returns false
 // when a wait gave up. The warp is converged; one elected lane issues.
-template <bool INT8, typename R>
-__device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars, uint32_t ring,
-                                             Cursor<R::kStages>& stage, Cursor<2>& a_buf,
+template <bool INT8>
+__device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars,
+                                             const Ring<INT8>& ring, Cursor& stage, Cursor& a_buf,
                                              uint32_t tmem, uint32_t d_tmem, uint32_t n,
                                              uint32_t blocks, uint64_t& done) {
   const uint32_t idesc = ptx::make_bf16_idesc(kRows, n);
@@ -142,14 +148,14 @@ __device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars, u
     if (!wait(bars.full[stage.slot], stage.parity)) return false;
     if (INT8 && !wait(bars.a_full[a_buf.slot], a_buf.parity)) return false;
     ptx::tc_fence_after_sync();
-    const uint32_t at = ring + stage.slot * R::kStageBytes;
+    const uint32_t at = ring.at(stage.slot);
     const uint64_t a_desc = ptx::make_kmajor_sw128_desc(at);
     const uint32_t a_tmem = tmem + a_buf.slot * (kTmemA / 2);
     if (ptx::elect_one()) {
 #pragma unroll
-      for (uint32_t piece = 0; piece < R::kPieces; ++piece) {
+      for (uint32_t piece = 0; piece < Block<INT8>::kPieces; ++piece) {
         const uint64_t b_desc =
-            ptx::make_kmajor_sw128_desc(at + kABytes + piece * R::kPieceBytes);
+            ptx::make_kmajor_sw128_desc(at + kABytes + piece * ring.piece_bytes);
 #pragma unroll
         for (uint32_t ks = 0; ks < 4; ++ks) {
           const uint32_t acc = (b | piece | ks) != 0 ? 1u : 0u;
@@ -165,24 +171,23 @@ __device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars, u
       if (b + 1 == blocks) ptx::umma_commit(ptx::smem_addr(&done));
     }
     __syncwarp();
-    stage.next();
-    a_buf.next();
+    stage.next(ring.stages);
+    a_buf.next(2);
   }
   return true;
 }
 
 // INT8: half of one warp's 32 rows of `blocks` k-blocks from shared memory to Tensor Memory as
 // BF16. Two warps share 32 rows: one alone measured half the rate HBM delivers.
-template <typename R>
-__device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars, uint32_t ring,
-                                               Cursor<R::kStages>& stage, Cursor<2>& a_buf,
-                                               uint32_t tmem, uint32_t quad, uint32_t half,
+__device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars,
+                                               const Ring<true>& ring, uint32_t tmem, uint32_t quad, uint32_t half,
                                                uint32_t lane, uint32_t blocks) {
+  Cursor stage, a_buf;
   for (uint32_t b = 0; b < blocks; ++b) {
     if (!wait(bars.full[stage.slot], stage.parity)) return false;
     if (!wait(bars.a_empty[a_buf.slot], a_buf.parity ^ 1u)) return false;
     ptx::tc_fence_after_sync();
-    const uint32_t row = ring + stage.slot * R::kStageBytes + (quad * 32 + lane) * 128;
+    const uint32_t row = ring.at(stage.slot) + (quad * 32 + lane) * 128;
     const uint32_t to = tmem + a_buf.slot * (kTmemA / 2) + ((quad * 32) << 16);
     uint32_t v[32];
 #pragma unroll
@@ -203,14 +208,14 @@ __device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars,
     ptx::tc_fence_before_sync();
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&bars.a_full[a_buf.slot]));
-    stage.next();
-    a_buf.next();
+    stage.next(ring.stages);
+    a_buf.next(2);
   }
   return true;
 }
 
 __device__ __forceinline__ void init_barriers(Barriers& bars) {
-  for (uint32_t s = 0; s < 6; ++s) {
+  for (uint32_t s = 0; s < kMaxStages; ++s) {
     ptx::mbar_init(ptx::smem_addr(&bars.full[s]), 1);
     ptx::mbar_init(ptx::smem_addr(&bars.empty[s]), 1);
   }
@@ -230,16 +235,30 @@ __device__ __forceinline__ void settle(volatile uint32_t* abort_word) {
   while (ptx::global_timer_ns() - start < 200000) __nanosleep(1000);
 }
 
+// The word at the same shared-memory address of every CTA of the cluster, summed in the order
+// of their ranks; all loads are in flight together.
+__device__ __forceinline__ float sum_over_cluster(uint32_t address, uint32_t ranks) {
+  float part[8];
+  if (ranks == 1) {
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(part[0]) : "r"(address) : "memory");
+    return part[0];
+  }
+#pragma unroll
+  for (uint32_t s = 0; s < 8; ++s) {
+    part[s] = s < ranks ? ptx::ld_cluster_f32(ptx::map_to_cta(address, s)) : 0.0f;
+  }
+  float sum = part[0];
+#pragma unroll
+  for (uint32_t s = 1; s < 8; ++s) {
+    if (s < ranks) sum += part[s];
+  }
+  return sum;
+}
+
 // --------------------------------------------------- gate and up products --
 
 template <bool INT8>
 constexpr uint32_t kUpThreads = INT8 ? 384 : 256;
-
-template <bool INT8, uint32_t COLS>
-using UpRing = Ring<INT8, COLS, 1, 0>;
-
-template <bool INT8, uint32_t COLS>
-constexpr uint32_t kUpSmem = UpRing<INT8, COLS>::kStages * UpRing<INT8, COLS>::kStageBytes + 1024;
 
 template <bool INT8, uint32_t COLS>
 constexpr uint32_t kUpTmem = INT8 ? 256 : (COLS < 32 ? 32 : COLS);
@@ -248,17 +267,17 @@ constexpr uint32_t kUpTmem = INT8 ? 256 : (COLS < 32 ? 32 : COLS);
 // are the channels' gate rows, 64-127 their up rows. Activations come in boxes of 8 tokens, only
 // those that hold a token of the expert.
 template <bool INT8, uint32_t COLS>
-__global__ void __launch_bounds__(kUpThreads<INT8>, (UpRing<INT8, COLS>::kCtasPerSm))
-decode_up_kernel(const __grid_constant__ DecodeParams p) {
-  using R = UpRing<INT8, COLS>;
+__global__ void __launch_bounds__(kUpThreads<INT8>, 2)
+decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
+  constexpr uint32_t kPieces = Block<INT8>::kPieces, kBlockK = Block<INT8>::kK;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Barriers bars;
   __shared__ uint32_t tmem_slot, abort_slot;
   __shared__ uint32_t list_mask[2], list_base, list_expert;   // tokens of the expert
-  __shared__ float token_coef[kMaxTokens];
+  __shared__ float list_coef[kMaxTokens], channel_scale[2][64];
   __shared__ uint8_t list_token[kMaxTokens], list_column[kMaxTokens];
   const DecodeArgs& a = p.a;
-  const uint32_t ring = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Wait wait{&abort_slot};
 
@@ -272,27 +291,21 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
     const int64_t e = a.by_expert != 0 ? static_cast<int64_t>(blockIdx.y) : a.ids[blockIdx.y];
     uint32_t mask[2] = {0, 0}, before = 0, owner = kFullWarp;
     if (e >= 0 && e < a.experts) {
-#pragma unroll
-      for (uint32_t half = 0; half < 2; ++half) {
-        const uint32_t t = half * 32 + lane;
-        uint32_t first = kFullWarp;
-        float coef = 0.0f;
-        if (t < a.tokens) {
-          for (uint32_t j = 0; j < a.top_k; ++j) {
-            const uint32_t r = t * a.top_k + j;
-            const int64_t id = a.ids[r];
-            if (id == e) {                 // twice: the sum of both weights
-              if (first == kFullWarp) first = r;
-              coef += a.coef[r];
-            }
-            before += id >= 0 && id < e ? 1u : 0u;
-          }
-          token_coef[t] = coef;
+#pragma unroll 4
+      for (uint32_t r = lane; r < a.tokens * a.top_k; r += 32) {
+        const int64_t id = a.ids[r];
+        if (id == e) {
+          const uint32_t t = r / a.top_k;
+          mask[0] |= t < 32 ? 1u << t : 0u;
+          mask[1] |= t < 32 ? 0u : 1u << (t - 32);
+          owner = min(owner, r);
         }
-        mask[half] = __ballot_sync(kFullWarp, first != kFullWarp);
-        owner = min(owner, __reduce_min_sync(kFullWarp, first));
+        before += id >= 0 && id < e ? 1u : 0u;
       }
+      mask[0] = __reduce_or_sync(kFullWarp, mask[0]);
+      mask[1] = __reduce_or_sync(kFullWarp, mask[1]);
       before = __reduce_add_sync(kFullWarp, before);
+      owner = __reduce_min_sync(kFullWarp, owner);
       if (a.by_expert == 0 && owner != blockIdx.y) mask[0] = mask[1] = 0;
     }
     // column of a token in the tile: its place among the boxes that are loaded
@@ -349,15 +362,16 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
   const uint32_t d_tmem = tmem + (INT8 ? kTmemA : 0);
   const uint32_t boxes = __popc(groups);
   const uint32_t n = (boxes + 1) / 2 * 16;         // columns of the MMA: a multiple of 16
+  const Ring<INT8> ring(base, ring_bytes, n);
 
   const uint32_t rank = ptx::cluster_cta_rank(), ranks = ptx::cluster_cta_count();
   const uint32_t channel0 = blockIdx.x / ranks * 64;
-  const uint32_t all_blocks = (a.hidden + R::kBlockK - 1) / R::kBlockK;
+  const uint32_t all_blocks = (a.hidden + kBlockK - 1) / kBlockK;
   const uint32_t begin = all_blocks * rank / ranks, end = all_blocks * (rank + 1) / ranks;
 
   if (warp == 0) {
-    Cursor<R::kStages> stage;
-    const uint32_t bytes = kABytes + boxes * R::kPieces * kGroup * 128;
+    Cursor stage;
+    const uint32_t bytes = kABytes + boxes * kPieces * kGroup * 128;
     const int32_t row = static_cast<int32_t>(expert * 2 * a.inter + channel0);
     for (uint32_t b = begin; b < end; ++b) {
       if (!wait(bars.empty[stage.slot], stage.parity ^ 1u)) {
@@ -366,8 +380,8 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
       }
       if (ptx::elect_one()) {
         const uint32_t bar = ptx::smem_addr(&bars.full[stage.slot]);
-        const uint32_t at = ring + stage.slot * R::kStageBytes;
-        const int32_t k = static_cast<int32_t>(b * R::kBlockK);
+        const uint32_t at = ring.at(stage.slot);
+        const int32_t k = static_cast<int32_t>(b * kBlockK);
         ptx::mbar_arrive_expect_tx(bar, bytes);
         ptx::tma_load_2d(at, &p.weights, bar, k, row);
         ptx::tma_load_2d(at + kABytes / 2, &p.weights, bar, k,
@@ -376,37 +390,51 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
         for (uint32_t left = groups; left != 0; left &= left - 1, ++box) {
           const int32_t token = static_cast<int32_t>(kGroup * (__ffs(left) - 1));
 #pragma unroll
-          for (uint32_t piece = 0; piece < R::kPieces; ++piece) {
-            ptx::tma_load_2d(at + kABytes + piece * R::kPieceBytes + box * kGroup * 128, &p.acts,
+          for (uint32_t piece = 0; piece < kPieces; ++piece) {
+            ptx::tma_load_2d(at + kABytes + piece * ring.piece_bytes + box * kGroup * 128, &p.acts,
                              bar, k + static_cast<int32_t>(64 * piece), token);
           }
         }
       }
       __syncwarp();
-      stage.next();
+      stage.next(ring.stages);
     }
   } else if (warp == 1) {
-    Cursor<R::kStages> stage;
-    Cursor<2> a_buf;
-    if (!issue_blocks<INT8, R>(wait, bars, ring, stage, a_buf, tmem, d_tmem, n, end - begin,
-                               bars.d_full[0])) {
+    Cursor stage, a_buf;
+    if (!issue_blocks<INT8>(wait, bars, ring, stage, a_buf, tmem, d_tmem, n, end - begin,
+                            bars.d_full[0])) {
       if (lane == 0) report(a, 2);
+    }
+  } else if (warp == 2) {
+    // weight of every listed token: the sum where it names the expert twice
+    for (uint32_t at = lane; at < count; at += 32) {
+      const uint32_t t = list_token[at];
+      float coef = 0.0f;
+      for (uint32_t j = 0; j < a.top_k; ++j) {
+        if (a.ids[t * a.top_k + j] == static_cast<int64_t>(expert)) coef += a.coef[t * a.top_k + j];
+      }
+      list_coef[at] = coef;
+    }
+  } else if (warp == 3) {
+    if constexpr (INT8) {
+      for (uint32_t c = lane; c < 64 && channel0 + c < a.inter; c += 32) {
+        const float* const scale = a.s1 + static_cast<size_t>(expert) * 2 * a.inter + channel0 + c;
+        channel_scale[0][c] = scale[0];
+        channel_scale[1][c] = scale[a.inter];
+      }
     }
   } else if (warp >= 4) {
     const uint32_t quad = warp & 3;
     bool ok = true;
     if constexpr (INT8) {
-      Cursor<R::kStages> stage;
-      Cursor<2> a_buf;
-      ok = convert_blocks<R>(wait, bars, ring, stage, a_buf, tmem, quad, (warp - 4) / 4, lane,
-                             end - begin);
+      ok = convert_blocks(wait, bars, ring, tmem, quad, (warp - 4) / 4, lane, end - begin);
       if (!ok && lane == 0) report(a, 3);
     }
     // Accumulator -> shared memory [column][row], over the ring: all of its bytes are used.
     if (warp >= 8) {
     } else if (ok && wait(bars.d_full[0], 0)) {
       ptx::tc_fence_after_sync();
-      const uint32_t to = ring + (quad * 32 + lane) * 4;
+      const uint32_t to = base + (quad * 32 + lane) * 4;
 #pragma unroll
       for (uint32_t c = 0; c < COLS; c += 16) {
         if (c < n) {
@@ -427,7 +455,11 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
   }
   __syncwarp();
   settle(&abort_slot);
-  ptx::cluster_sync();
+  if (ranks > 1) {
+    ptx::cluster_sync();
+  } else {
+    __syncthreads();
+  }
 
   // Join the k shares in a fixed order; weights * silu(gate) * up in two BF16 halves.
   for (uint32_t i = rank * kUpThreads<INT8> + threadIdx.x; i < 64 * count;
@@ -435,19 +467,13 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
     const uint32_t c = i % 64, at = i / 64;
     const uint32_t channel = channel0 + c;
     if (channel >= a.inter) continue;
-    const uint32_t cell = ring + (list_column[at] * kRows + c) * 4;
-    float gate = 0.0f, up = 0.0f;
-    for (uint32_t s = 0; s < ranks; ++s) {
-      const uint32_t remote = ptx::map_to_cta(cell, s);
-      gate += ptx::ld_cluster_f32(remote);
-      up += ptx::ld_cluster_f32(remote + 64 * 4);
-    }
+    const uint32_t cell = base + (list_column[at] * kRows + c) * 4;
+    float gate = sum_over_cluster(cell, ranks), up = sum_over_cluster(cell + 64 * 4, ranks);
     if constexpr (INT8) {
-      const float* const scale = a.s1 + static_cast<size_t>(expert) * 2 * a.inter + channel;
-      gate *= scale[0];
-      up *= scale[a.inter];
+      gate *= channel_scale[0][c];
+      up *= channel_scale[1][c];
     }
-    const float v = gate / (1.0f + expf(-gate)) * up * token_coef[list_token[at]];
+    const float v = gate / (1.0f + expf(-gate)) * up * list_coef[at];
     // 16 significant bits in two BF16 numbers; an infinity has no remainder
     const uint16_t hi = to_bf16(v);
     const float rest = v - from_bf16(hi);
@@ -455,8 +481,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p) {
     to[0] = hi;
     to[static_cast<size_t>(a.tokens) * a.top_k * a.inter] = to_bf16(isfinite(rest) ? rest : 0.0f);
   }
-  ptx::fence_proxy_async_all();            // h is read by TMA
-  ptx::cluster_sync();                     // a neighbour may still read this CTA's tile
+  if (ranks > 1) ptx::cluster_sync_relaxed();   // a neighbour may still read this CTA's tile
   if (warp == 1) {
     ptx::tc_fence_after_sync();
     ptx::tmem_dealloc(tmem, (kUpTmem<INT8, COLS>));
@@ -469,38 +494,29 @@ template <bool INT8>
 constexpr uint32_t kDownThreads = INT8 ? 512 : 256;
 
 template <bool INT8, uint32_t COLS>
-using DownRing = Ring<INT8, COLS, 2, COLS * kRows * 4>;
-
-template <bool INT8, uint32_t COLS>
 constexpr uint32_t kDownTmem = INT8 ? (COLS == 64 ? 512 : 256) : 4 * COLS;
 
 // Lists in dynamic shared memory, per expert: token mask (8 bytes), assignments (4), and for
 // the chosen ones in ascending order id and first row of h (2 + 2).
 constexpr uint32_t kListBytes = 16;
 
-template <bool INT8, uint32_t COLS>
-uint32_t down_smem(uint32_t experts) {
-  using R = DownRing<INT8, COLS>;
-  return R::kStages * R::kStageBytes + COLS * kRows * 4 + experts * kListBytes + 1024;
-}
-
 // A cluster computes 128 output channels for all tokens: the chosen experts' k ranges, laid
 // end to end, are shared among its CTAs. A thread of the epilogue owns one channel and adds
 // every expert's accumulator columns to its tokens' sums in shared memory.
 template <bool INT8, uint32_t COLS>
-__global__ void __launch_bounds__(kDownThreads<INT8>, (DownRing<INT8, COLS>::kCtasPerSm))
-decode_down_kernel(const __grid_constant__ DecodeParams p) {
-  using R = DownRing<INT8, COLS>;
+__global__ void __launch_bounds__(kDownThreads<INT8>, 2)
+decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
+  constexpr uint32_t kPieces = Block<INT8>::kPieces, kBlockK = Block<INT8>::kK;
   constexpr uint32_t kThreads = kDownThreads<INT8>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Barriers bars;
   __shared__ uint32_t tmem_slot, abort_slot, active_count;
   const DecodeArgs& a = p.a;
   const uint32_t raw = ptx::smem_addr(smem_raw);
-  const uint32_t ring = (raw + 1023u) & ~1023u;
-  uint8_t* const behind = smem_raw + (ring - raw) + R::kStages * R::kStageBytes;
-  float* const sums = reinterpret_cast<float*>(behind);                  // [COLS][128]
-  uint32_t* const masks = reinterpret_cast<uint32_t*>(behind + COLS * kRows * 4);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* const behind = smem_raw + (base - raw) + ring_bytes;
+  float* const sums = reinterpret_cast<float*>(behind);                  // [tokens][128]
+  uint32_t* const masks = reinterpret_cast<uint32_t*>(behind + a.tokens * kRows * 4);
   uint32_t* const assigned = masks + 2 * a.experts;
   uint16_t* const active = reinterpret_cast<uint16_t*>(assigned + a.experts);
   uint16_t* const first_row = active + a.experts;
@@ -509,7 +525,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
 
   // Lists of the chosen experts; nothing here depends on the first kernel.
   for (uint32_t i = threadIdx.x; i < 3 * a.experts; i += kThreads) masks[i] = 0;
-  for (uint32_t i = threadIdx.x; i < COLS * kRows; i += kThreads) sums[i] = 0.0f;
+  for (uint32_t i = threadIdx.x; i < a.tokens * kRows; i += kThreads) sums[i] = 0.0f;
   if (warp == 1) {
     if (lane == 0) {
       abort_slot = 0;
@@ -568,7 +584,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
   const uint32_t rank = ptx::cluster_cta_rank(), ranks = ptx::cluster_cta_count();
   const uint32_t channel0 = blockIdx.x / ranks * kRows;
   const uint32_t d_tmem = tmem + (INT8 ? kTmemA : 0);
-  const uint32_t blocks = (a.inter + R::kBlockK - 1) / R::kBlockK;       // of one expert
+  const uint32_t blocks = (a.inter + kBlockK - 1) / kBlockK;             // of one expert
   const uint32_t total = active_count * blocks;
   const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(total) * rank / ranks);
   const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(total) * (rank + 1) / ranks);
@@ -579,25 +595,29 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
     return __popc(masks[2 * e]) + __popc(masks[2 * e + 1]);
   };
   auto run_of = [&](uint32_t at) { return min(end, (at / blocks + 1) * blocks) - at; };
+  // boxes of 8 rows of h for the expert, once for each half of h
+  auto boxes_of = [&](uint32_t slot) { return (tokens_of(slot) + kGroup - 1) / kGroup; };
+  uint32_t most = 1;
+  for (uint32_t at = begin; at < end; at += run_of(at)) most = max(most, boxes_of(at / blocks));
+  const Ring<INT8> ring(base, ring_bytes, most * 2 * kGroup);
 
   if (warp == 0) {
     const int32_t low_half = static_cast<int32_t>(a.tokens * a.top_k);
     auto load_weights = [&](uint32_t at, uint32_t s) {
       const uint32_t slot = at / blocks;
-      ptx::tma_load_2d(ring + s * R::kStageBytes, &p.weights, ptx::smem_addr(&bars.full[s]),
-                       static_cast<int32_t>((at - slot * blocks) * R::kBlockK),
+      ptx::tma_load_2d(ring.at(s), &p.weights, ptx::smem_addr(&bars.full[s]),
+                       static_cast<int32_t>((at - slot * blocks) * kBlockK),
                        static_cast<int32_t>(active[slot] * a.hidden + channel0));
     };
     auto expect = [&](uint32_t at, uint32_t s) {
-      const uint32_t boxes = (tokens_of(at / blocks) + kGroup - 1) / kGroup;
       ptx::mbar_arrive_expect_tx(ptx::smem_addr(&bars.full[s]),
-                                 kABytes + boxes * 2 * R::kPieces * kGroup * 128);
+                                 kABytes + boxes_of(at / blocks) * 2 * kPieces * kGroup * 128);
     };
     auto load_acts = [&](uint32_t at, uint32_t s) {
       const uint32_t slot = at / blocks;
-      const uint32_t boxes = (tokens_of(slot) + kGroup - 1) / kGroup;
-      const int32_t k = static_cast<int32_t>((at - slot * blocks) * R::kBlockK);
-      const uint32_t to = ring + s * R::kStageBytes + kABytes;
+      const uint32_t boxes = boxes_of(slot);
+      const int32_t k = static_cast<int32_t>((at - slot * blocks) * kBlockK);
+      const uint32_t to = ring.at(s) + kABytes;
       const uint32_t bar = ptx::smem_addr(&bars.full[s]);
       for (uint32_t box = 0; box < boxes; ++box) {
         // rows beyond the expert's are other rows of h: columns that nobody reads
@@ -605,9 +625,9 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
 #pragma unroll
         for (uint32_t plane = 0; plane < 2; ++plane) {
 #pragma unroll
-          for (uint32_t piece = 0; piece < R::kPieces; ++piece) {
+          for (uint32_t piece = 0; piece < kPieces; ++piece) {
             ptx::tma_load_2d(
-                to + piece * R::kPieceBytes + (plane * boxes + box) * kGroup * 128, &p.acts, bar,
+                to + piece * ring.piece_bytes + (plane * boxes + box) * kGroup * 128, &p.acts, bar,
                 k + static_cast<int32_t>(64 * piece),
                 row + (plane != 0 ? low_half : 0));
           }
@@ -615,7 +635,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
       }
     };
     // The first stages' weights do not wait for the first kernel, their activations do.
-    const uint32_t ahead = min(begin + R::kStages, end);
+    const uint32_t ahead = min(begin + ring.stages, end);
     if (ptx::elect_one()) {
       for (uint32_t at = begin; at < ahead; ++at) {
         expect(at, at - begin);
@@ -629,7 +649,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
       for (uint32_t at = begin; at < ahead; ++at) load_acts(at, at - begin);
     }
     __syncwarp();
-    Cursor<R::kStages> stage;
+    Cursor stage;
     stage.parity = 1;                      // second use of every stage
     for (uint32_t at = ahead; at < end; ++at) {
       if (!wait(bars.empty[stage.slot], stage.parity ^ 1u)) {
@@ -642,40 +662,38 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
         load_acts(at, stage.slot);
       }
       __syncwarp();
-      stage.next();
+      stage.next(ring.stages);
     }
   } else if (warp == 1) {
-    Cursor<R::kStages> stage;
-    Cursor<2> a_buf, d_buf;
+    Cursor stage, a_buf, d_buf;
     for (uint32_t at = begin; at < end;) {
       const uint32_t run = run_of(at);
-      const uint32_t n = (tokens_of(at / blocks) + kGroup - 1) / kGroup * 2 * kGroup;
+      const uint32_t n = boxes_of(at / blocks) * 2 * kGroup;
       if (!wait(bars.d_empty[d_buf.slot], d_buf.parity ^ 1u)) {
         if (lane == 0) report(a, 6);
         break;
       }
       ptx::tc_fence_after_sync();
-      if (!issue_blocks<INT8, R>(wait, bars, ring, stage, a_buf, tmem,
-                                 d_tmem + d_buf.slot * 2 * COLS, n, run,
-                                 bars.d_full[d_buf.slot])) {
+      if (!issue_blocks<INT8>(wait, bars, ring, stage, a_buf, tmem,
+                              d_tmem + d_buf.slot * 2 * COLS, n, run,
+                              bars.d_full[d_buf.slot])) {
         if (lane == 0) report(a, 7);
         break;
       }
-      d_buf.next();
+      d_buf.next(2);
       at += run;
     }
   } else if (INT8 && warp >= 4 && warp < 12) {
-    Cursor<R::kStages> stage;
-    Cursor<2> a_buf;
-    if (!convert_blocks<R>(wait, bars, ring, stage, a_buf, tmem, warp & 3, (warp - 4) / 4, lane,
-                           end - begin)) {
-      if (lane == 0) report(a, 8);
+    if constexpr (INT8) {
+      if (!convert_blocks(wait, bars, ring, tmem, warp & 3, (warp - 4) / 4, lane, end - begin)) {
+        if (lane == 0) report(a, 8);
+      }
     }
   } else if (warp >= (INT8 ? 12 : 4)) {
     const uint32_t quad = warp & 3;
     const uint32_t row = quad * 32 + lane;
     float* const mine = sums + row;
-    Cursor<2> d_buf;
+    Cursor d_buf;
     for (uint32_t at = begin; at < end;) {
       const uint32_t run = run_of(at);
       const uint32_t e = active[at / blocks];
@@ -693,7 +711,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
       }
       ptx::tc_fence_after_sync();
       const uint32_t from = d_tmem + ((quad * 32) << 16) + d_buf.slot * 2 * COLS;
-      const uint32_t boxes = (count + kGroup - 1) / kGroup;
+      const uint32_t boxes = boxes_of(at / blocks);
       for (uint32_t c = 0; c < boxes * kGroup; c += kGroup) {
         uint32_t upper[kGroup], lower[kGroup];
         ptx::tmem_load_32x8(from + c, upper);
@@ -712,7 +730,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
       ptx::tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&bars.d_empty[d_buf.slot]));
-      d_buf.next();
+      d_buf.next(2);
       at += run;
     }
   }
@@ -721,21 +739,22 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
   // not end first.
   ptx::wait_for_previous_grid();
   settle(&abort_slot);
-  ptx::cluster_sync();
+  if (ranks > 1) {
+    ptx::cluster_sync();
+  } else {
+    __syncthreads();
+  }
 
   // Join the cluster's CTAs in a fixed order.
   const uint32_t sums_smem = ptx::smem_addr(sums);
   for (uint32_t i = rank * kThreads + threadIdx.x; i < a.tokens * kRows; i += ranks * kThreads) {
     const uint32_t channel = channel0 + i % kRows;
-    float sum = 0.0f;
-    for (uint32_t s = 0; s < ranks; ++s) {
-      sum += ptx::ld_cluster_f32(ptx::map_to_cta(sums_smem + i * 4, s));
-    }
+    const float sum = sum_over_cluster(sums_smem + i * 4, ranks);
     if (channel < a.hidden) {
       a.out[static_cast<size_t>(i / kRows) * a.hidden + channel] = to_bf16(sum);
     }
   }
-  ptx::cluster_sync();                     // a neighbour may still read this CTA's sums
+  if (ranks > 1) ptx::cluster_sync_relaxed();   // a neighbour may still read this CTA's sums
   if (warp == 1) {
     ptx::tc_fence_after_sync();
     ptx::tmem_dealloc(tmem, (kDownTmem<INT8, COLS>));
@@ -744,19 +763,19 @@ decode_down_kernel(const __grid_constant__ DecodeParams p) {
 
 // ------------------------------------------------------------------ launch --
 
-// CTAs along k: up to 8 (the portable cluster size) while the grid leaves room and every CTA
-// keeps two k-blocks.
-uint32_t split_of(uint64_t tiles, uint32_t blocks, uint32_t room) {
+// CTAs along k: up to `most` while the grid leaves room and every CTA keeps two k-blocks.
+uint32_t split_of(uint64_t tiles, uint64_t blocks, uint32_t room, uint32_t most) {
   uint32_t split = 1;
-  while (split < 8 && tiles * split * 2 <= room && split * 4 <= blocks) split *= 2;
+  while (split < most && tiles * split * 2 <= room && split * 4 <= blocks) split *= 2;
   return split;
 }
 
 template <typename Kernel>
-cudaError_t launch_cluster(Kernel kernel, dim3 grid, uint32_t threads, uint32_t smem,
-                           uint32_t cluster, bool after_previous, const DecodeParams& params,
-                           cudaStream_t stream) {
+cudaError_t launch_cluster(Kernel kernel, dim3 grid, uint32_t threads, uint32_t ring_bytes,
+                           uint32_t reserved, uint32_t cluster, bool after_previous,
+                           const DecodeParams& params, cudaStream_t stream) {
   // an attribute of the function on the current device: set per launch, nothing is cached
+  const uint32_t smem = 1024 + ring_bytes + reserved;
   cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         static_cast<int>(smem));
   if (rc != cudaSuccess) return rc;
@@ -774,33 +793,38 @@ cudaError_t launch_cluster(Kernel kernel, dim3 grid, uint32_t threads, uint32_t 
   attribute[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
   config.numAttrs = after_previous ? 2 : 1;
-  rc = cudaLaunchKernelEx(&config, kernel, params);
+  rc = cudaLaunchKernelEx(&config, kernel, params, ring_bytes);
   return rc != cudaSuccess ? rc : cudaPeekAtLastError();
 }
 
 template <bool INT8, uint32_t COLS>
 cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cudaStream_t stream) {
+  constexpr uint32_t kPieces = Block<INT8>::kPieces, kBlockK = Block<INT8>::kK;
   const DecodeArgs& a = up.a;
   const uint32_t sms = device_sm_count();
-  using U = UpRing<INT8, COLS>;
-  using D = DownRing<INT8, COLS>;
-  const uint32_t slots = a.by_expert != 0 ? a.experts : a.tokens * a.top_k;
+  const uint32_t assignments = a.tokens * a.top_k;
+  const uint32_t slots = a.by_expert != 0 ? a.experts : assignments;
+  // Two CTAs per SM: one streams while the other starts or ends.
   const uint32_t tiles = (a.inter + 63) / 64;
   uint32_t split = split_of(static_cast<uint64_t>(tiles) * slots,
-                            (a.hidden + U::kBlockK - 1) / U::kBlockK, 2 * U::kCtasPerSm * sms);
+                            (a.hidden + kBlockK - 1) / kBlockK, 4 * sms, 8);
   cudaError_t rc =
       launch_cluster(decode_up_kernel<INT8, COLS>, dim3(tiles * split, slots), kUpThreads<INT8>,
-                     kUpSmem<INT8, COLS>, split, false, up, stream);
+                     kTwoPerSm - 1024, 0, split, false, up, stream);
   if (rc != cudaSuccess) return rc;
+  // The sums of many tokens leave less for the ring: two CTAs per SM if three stages fit at
+  // twice the average number of an expert's tokens, else one, in clusters of 4 (of 8 with an
+  // SM each, fewer fit at once).
   const uint32_t groups = (a.hidden + kRows - 1) / kRows;
-  const uint64_t blocks =
-      static_cast<uint64_t>((a.inter + D::kBlockK - 1) / D::kBlockK) *
-      (slots < a.tokens * a.top_k ? slots : a.tokens * a.top_k);
-  split = split_of(groups, blocks < 64 ? static_cast<uint32_t>(blocks) : 64u,
-                   2 * D::kCtasPerSm * sms);
-  return launch_cluster(decode_down_kernel<INT8, COLS>, dim3(groups * split),
-                        kDownThreads<INT8>, down_smem<INT8, COLS>(a.experts), split, true, down,
-                        stream);
+  const uint32_t reserved = (a.tokens * kRows * 4 + a.experts * kListBytes + 15) / 16 * 16;
+  const uint32_t twice = 2 * assignments / a.experts + kGroup;
+  const uint32_t columns = (twice < a.tokens ? twice : a.tokens) / kGroup * 2 * kGroup;
+  const bool two = kTwoPerSm - 1024 >= reserved + 3 * (kABytes + kPieces * columns * 128);
+  split = split_of(groups, static_cast<uint64_t>((a.inter + kBlockK - 1) / kBlockK) * slots,
+                   two ? 2 * sms : sms, two ? 8 : 4);
+  return launch_cluster(decode_down_kernel<INT8, COLS>, dim3(groups * split), kDownThreads<INT8>,
+                        (two ? kTwoPerSm : kOnePerSm) - 1024 - reserved, reserved, split, true,
+                        down, stream);
 }
 
 template <bool INT8>
