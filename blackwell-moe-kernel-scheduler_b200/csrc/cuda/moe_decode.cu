@@ -177,39 +177,46 @@ __device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars,
   return true;
 }
 
-// INT8: half of one warp's 32 rows of `blocks` k-blocks from shared memory to Tensor Memory as
-// BF16. Two warps share 32 rows: one alone measured half the rate HBM delivers.
+// INT8: one warp's 32 rows of every second of `blocks` k-blocks (`turn` 0 or 1, and that buffer)
+// from shared memory to Tensor Memory as BF16. A block takes a warp some 800 cycles, most of
+// them latency, so two groups of four warps take turns.
 __device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars,
-                                               const Ring<true>& ring, uint32_t tmem, uint32_t quad, uint32_t half,
+                                               const Ring<true>& ring, uint32_t tmem, uint32_t quad, uint32_t turn,
                                                uint32_t lane, uint32_t blocks) {
-  Cursor stage, a_buf;
-  for (uint32_t b = 0; b < blocks; ++b) {
+  Cursor stage;
+  uint32_t a_parity = 0;
+  if (turn != 0) stage.next(ring.stages);
+  const uint32_t to = tmem + turn * (kTmemA / 2) + ((quad * 32) << 16);
+  for (uint32_t b = turn; b < blocks; b += 2) {
     if (!wait(bars.full[stage.slot], stage.parity)) return false;
-    if (!wait(bars.a_empty[a_buf.slot], a_buf.parity ^ 1u)) return false;
+    if (!wait(bars.a_empty[turn], a_parity ^ 1u)) return false;
     ptx::tc_fence_after_sync();
     const uint32_t row = ring.at(stage.slot) + (quad * 32 + lane) * 128;
-    const uint32_t to = tmem + a_buf.slot * (kTmemA / 2) + ((quad * 32) << 16);
-    uint32_t v[32];
 #pragma unroll
-    for (uint32_t c = 0; c < 4; ++c) {
-      // 16-byte pieces of a 128-byte row are swizzled by the row's place in its group of 8
-      const uint4 w = ptx::ld_shared_v4(row + (((half * 4 + c) ^ (lane & 7)) << 4));
-      v[8 * c + 0] = int8_pair(w.x, 0x4140);
-      v[8 * c + 1] = int8_pair(w.x, 0x4342);
-      v[8 * c + 2] = int8_pair(w.y, 0x4140);
-      v[8 * c + 3] = int8_pair(w.y, 0x4342);
-      v[8 * c + 4] = int8_pair(w.z, 0x4140);
-      v[8 * c + 5] = int8_pair(w.z, 0x4342);
-      v[8 * c + 6] = int8_pair(w.w, 0x4140);
-      v[8 * c + 7] = int8_pair(w.w, 0x4342);
+    for (uint32_t half = 0; half < 2; ++half) {
+      uint32_t v[32];
+#pragma unroll
+      for (uint32_t c = 0; c < 4; ++c) {
+        // 16-byte pieces of a 128-byte row are swizzled by the row's place in its group of 8
+        const uint4 w = ptx::ld_shared_v4(row + (((half * 4 + c) ^ (lane & 7)) << 4));
+        v[8 * c + 0] = int8_pair(w.x, 0x4140);
+        v[8 * c + 1] = int8_pair(w.x, 0x4342);
+        v[8 * c + 2] = int8_pair(w.y, 0x4140);
+        v[8 * c + 3] = int8_pair(w.y, 0x4342);
+        v[8 * c + 4] = int8_pair(w.z, 0x4140);
+        v[8 * c + 5] = int8_pair(w.z, 0x4342);
+        v[8 * c + 6] = int8_pair(w.w, 0x4140);
+        v[8 * c + 7] = int8_pair(w.w, 0x4342);
+      }
+      ptx::tmem_store_32x32(to + half * 32, v);
     }
-    ptx::tmem_store_32x32(to + half * 32, v);
     ptx::tmem_store_wait();
     ptx::tc_fence_before_sync();
     __syncwarp();
-    if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&bars.a_full[a_buf.slot]));
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&bars.a_full[turn]));
     stage.next(ring.stages);
-    a_buf.next(2);
+    stage.next(ring.stages);
+    a_parity ^= 1u;
   }
   return true;
 }
@@ -220,7 +227,7 @@ __device__ __forceinline__ void init_barriers(Barriers& bars) {
     ptx::mbar_init(ptx::smem_addr(&bars.empty[s]), 1);
   }
   for (uint32_t b = 0; b < 2; ++b) {
-    ptx::mbar_init(ptx::smem_addr(&bars.a_full[b]), 8);    // converting warps
+    ptx::mbar_init(ptx::smem_addr(&bars.a_full[b]), 4);    // converting warps
     ptx::mbar_init(ptx::smem_addr(&bars.a_empty[b]), 1);
     ptx::mbar_init(ptx::smem_addr(&bars.d_full[b]), 1);
     ptx::mbar_init(ptx::smem_addr(&bars.d_empty[b]), 4);   // epilogue warps
