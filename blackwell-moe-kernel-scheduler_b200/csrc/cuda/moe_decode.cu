@@ -55,10 +55,10 @@ struct DecodeArgs {
 };
 
 struct DecodeParams {
-  CUtensorMap weights;      // w_gate_up as {hidden, experts * 2 * inter}, box of 64 rows, or
-                            // w_down as {inter, experts * hidden}, box of 128 rows
-  CUtensorMap acts;         // x as {hidden, tokens} or h as {inter, 2 * tokens * top_k},
-                            // boxes of 8 rows
+  CUtensorMap weights;      // w_gate_up as {hidden, inter, 2 * experts}, box 128 B x 64 x 2, or
+                            // w_down as {inter, hidden, experts}, box 128 B x 128
+  CUtensorMap acts[kMaxTokens / kGroup];   // boxes of 8, 16, ... rows: x as {hidden, tokens},
+                                           // h as {inter, rows, 2}, both halves in one box
   DecodeArgs a;
 };
 
@@ -271,8 +271,9 @@ template <bool INT8, uint32_t COLS>
 constexpr uint32_t kUpTmem = INT8 ? 256 : (COLS < 32 ? 32 : COLS);
 
 // A cluster computes 64 channels of one expert for all of its tokens: the tile's rows 0-63
-// are the channels' gate rows, 64-127 their up rows. Activations come in boxes of 8 tokens, only
-// those that hold a token of the expert.
+// are the channels' gate rows, 64-127 their up rows. The activations of a k-block are one box per
+// piece (every load takes the producer some 60 cycles to issue): the groups of 8 tokens from
+// the expert's first to its last.
 template <bool INT8, uint32_t COLS>
 __global__ void __launch_bounds__(kUpThreads<INT8>, 2)
 decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
@@ -282,7 +283,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
   __shared__ uint32_t tmem_slot, abort_slot;
   __shared__ uint32_t list_mask[2], list_base, list_expert;   // tokens of the expert
   __shared__ float list_coef[kMaxTokens], channel_scale[2][64];
-  __shared__ uint8_t list_token[kMaxTokens], list_column[kMaxTokens];
+  __shared__ uint8_t list_token[kMaxTokens];
   const DecodeArgs& a = p.a;
   const uint32_t base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -291,7 +292,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
   if (warp == 0) {
     if (lane == 0) {
       ptx::tensormap_prefetch(&p.weights);
-      ptx::tensormap_prefetch(&p.acts);
+      ptx::tensormap_prefetch(&p.acts[0]);
     }
     // Tokens of this cluster's expert; rows of h in front of it (one per assignment to a
     // lower id). By assignment: the expert's first one does the work.
@@ -315,12 +316,6 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
       owner = __reduce_min_sync(kFullWarp, owner);
       if (a.by_expert == 0 && owner != blockIdx.y) mask[0] = mask[1] = 0;
     }
-    // column of a token in the tile: its place among the boxes that are loaded
-    uint32_t groups = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-      if (((mask[i / 4] >> (8 * (i % 4))) & 0xffu) != 0) groups |= 1u << i;
-    }
 #pragma unroll
     for (uint32_t half = 0; half < 2; ++half) {
       if ((mask[half] >> lane) & 1u) {
@@ -328,8 +323,6 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
         const uint32_t at =
             (half != 0 ? __popc(mask[0]) : 0) + __popc(mask[half] & ((1u << lane) - 1));
         list_token[at] = static_cast<uint8_t>(t);
-        list_column[at] =
-            static_cast<uint8_t>(__popc(groups & ((1u << (t / 8)) - 1)) * 8 + t % 8);
       }
     }
     if (lane == 0) {
@@ -361,13 +354,9 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
     return;
   }
   const uint32_t expert = list_expert;
-  uint32_t groups = 0;
-#pragma unroll
-  for (uint32_t i = 0; i < 8; ++i) {
-    if (((mask[i / 4] >> (8 * (i % 4))) & 0xffu) != 0) groups |= 1u << i;
-  }
   const uint32_t d_tmem = tmem + (INT8 ? kTmemA : 0);
-  const uint32_t boxes = __popc(groups);
+  const uint32_t token0 = list_token[0] / kGroup * kGroup;
+  const uint32_t boxes = list_token[count - 1] / kGroup - token0 / kGroup + 1;
   const uint32_t n = (boxes + 1) / 2 * 16;         // columns of the MMA: a multiple of 16
   const Ring<INT8> ring(base, ring_bytes, n);
 
@@ -379,7 +368,6 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
   if (warp == 0) {
     Cursor stage;
     const uint32_t bytes = kABytes + boxes * kPieces * kGroup * 128;
-    const int32_t row = static_cast<int32_t>(expert * 2 * a.inter + channel0);
     for (uint32_t b = begin; b < end; ++b) {
       if (!wait(bars.empty[stage.slot], stage.parity ^ 1u)) {
         if (lane == 0) report(a, 1);
@@ -390,17 +378,12 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
         const uint32_t at = ring.at(stage.slot);
         const int32_t k = static_cast<int32_t>(b * kBlockK);
         ptx::mbar_arrive_expect_tx(bar, bytes);
-        ptx::tma_load_2d(at, &p.weights, bar, k, row);
-        ptx::tma_load_2d(at + kABytes / 2, &p.weights, bar, k,
-                         row + static_cast<int32_t>(a.inter));
-        uint32_t box = 0;
-        for (uint32_t left = groups; left != 0; left &= left - 1, ++box) {
-          const int32_t token = static_cast<int32_t>(kGroup * (__ffs(left) - 1));
+        ptx::tma_load_3d(at, &p.weights, bar, k, static_cast<int32_t>(channel0),
+                         static_cast<int32_t>(2 * expert));
 #pragma unroll
-          for (uint32_t piece = 0; piece < kPieces; ++piece) {
-            ptx::tma_load_2d(at + kABytes + piece * ring.piece_bytes + box * kGroup * 128, &p.acts,
-                             bar, k + static_cast<int32_t>(64 * piece), token);
-          }
+        for (uint32_t piece = 0; piece < kPieces; ++piece) {
+          ptx::tma_load_2d(at + kABytes + piece * ring.piece_bytes, &p.acts[boxes - 1], bar,
+                           k + static_cast<int32_t>(64 * piece), static_cast<int32_t>(token0));
         }
       }
       __syncwarp();
@@ -474,7 +457,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
     const uint32_t c = i % 64, at = i / 64;
     const uint32_t channel = channel0 + c;
     if (channel >= a.inter) continue;
-    const uint32_t cell = base + (list_column[at] * kRows + c) * 4;
+    const uint32_t cell = base + ((list_token[at] - token0) * kRows + c) * 4;
     float gate = sum_over_cluster(cell, ranks), up = sum_over_cluster(cell + 64 * 4, ranks);
     if constexpr (INT8) {
       gate *= channel_scale[0][c];
@@ -543,7 +526,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
     ptx::tmem_relinquish();
   } else if (warp == 0 && lane == 0) {
     ptx::tensormap_prefetch(&p.weights);
-    ptx::tensormap_prefetch(&p.acts);
+    ptx::tensormap_prefetch(&p.acts[0]);
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
@@ -602,19 +585,18 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
     return __popc(masks[2 * e]) + __popc(masks[2 * e + 1]);
   };
   auto run_of = [&](uint32_t at) { return min(end, (at / blocks + 1) * blocks) - at; };
-  // boxes of 8 rows of h for the expert, once for each half of h
+  // rows of h that are loaded for the expert, in groups of 8
   auto boxes_of = [&](uint32_t slot) { return (tokens_of(slot) + kGroup - 1) / kGroup; };
   uint32_t most = 1;
   for (uint32_t at = begin; at < end; at += run_of(at)) most = max(most, boxes_of(at / blocks));
   const Ring<INT8> ring(base, ring_bytes, most * 2 * kGroup);
 
   if (warp == 0) {
-    const int32_t low_half = static_cast<int32_t>(a.tokens * a.top_k);
     auto load_weights = [&](uint32_t at, uint32_t s) {
       const uint32_t slot = at / blocks;
-      ptx::tma_load_2d(ring.at(s), &p.weights, ptx::smem_addr(&bars.full[s]),
+      ptx::tma_load_3d(ring.at(s), &p.weights, ptx::smem_addr(&bars.full[s]),
                        static_cast<int32_t>((at - slot * blocks) * kBlockK),
-                       static_cast<int32_t>(active[slot] * a.hidden + channel0));
+                       static_cast<int32_t>(channel0), active[slot]);
     };
     auto expect = [&](uint32_t at, uint32_t s) {
       ptx::mbar_arrive_expect_tx(ptx::smem_addr(&bars.full[s]),
@@ -624,21 +606,12 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
       const uint32_t slot = at / blocks;
       const uint32_t boxes = boxes_of(slot);
       const int32_t k = static_cast<int32_t>((at - slot * blocks) * kBlockK);
-      const uint32_t to = ring.at(s) + kABytes;
-      const uint32_t bar = ptx::smem_addr(&bars.full[s]);
-      for (uint32_t box = 0; box < boxes; ++box) {
+#pragma unroll
+      for (uint32_t piece = 0; piece < kPieces; ++piece) {
         // rows beyond the expert's are other rows of h: columns that nobody reads
-        const int32_t row = static_cast<int32_t>(first_row[slot] + box * kGroup);
-#pragma unroll
-        for (uint32_t plane = 0; plane < 2; ++plane) {
-#pragma unroll
-          for (uint32_t piece = 0; piece < kPieces; ++piece) {
-            ptx::tma_load_2d(
-                to + piece * ring.piece_bytes + (plane * boxes + box) * kGroup * 128, &p.acts, bar,
-                k + static_cast<int32_t>(64 * piece),
-                row + (plane != 0 ? low_half : 0));
-          }
-        }
+        ptx::tma_load_3d(ring.at(s) + kABytes + piece * ring.piece_bytes, &p.acts[boxes - 1],
+                         ptx::smem_addr(&bars.full[s]), k + static_cast<int32_t>(64 * piece),
+                         first_row[slot], 0);
       }
     };
     // The first stages' weights do not wait for the first kernel, their activations do.
@@ -857,6 +830,36 @@ cudaError_t preload_decode_type() {
   return rc;
 }
 
+bool encode_maps(DecodeParams& up, DecodeParams& down, const bmoe_moe_decode_args& a, bool int8) {
+  const Elem weight = int8 ? Elem::kByte : Elem::kBf16;
+  const uint64_t elem = int8 ? 1 : 2;
+  const uint32_t line = int8 ? 128 : 64;
+  const uint64_t hidden = a.hidden, inter = a.inter;
+  const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.top_k;
+  {
+    const uint64_t dims[3] = {hidden, inter, 2ull * a.experts};
+    const uint64_t strides[2] = {hidden * elem, inter * hidden * elem};
+    const uint32_t box[3] = {line, 64, 2};
+    if (!encode_box(&up.weights, a.w_gate_up_dev, weight, 3, dims, strides, box)) return false;
+  }
+  {
+    const uint64_t dims[3] = {inter, hidden, a.experts};
+    const uint64_t strides[2] = {inter * elem, hidden * inter * elem};
+    const uint32_t box[3] = {line, kRows, 1};
+    if (!encode_box(&down.weights, a.w_down_dev, weight, 3, dims, strides, box)) return false;
+  }
+  const uint64_t x_dims[2] = {hidden, a.tokens}, x_strides[1] = {hidden * 2};
+  const uint64_t h_dims[3] = {inter, rows, 2}, h_strides[2] = {inter * 2, rows * inter * 2};
+  for (uint32_t g = 0; g * kGroup < a.tokens; ++g) {
+    const uint32_t box[3] = {64, (g + 1) * kGroup, 2};
+    if (!encode_box(&up.acts[g], a.x_dev, Elem::kBf16, 2, x_dims, x_strides, box) ||
+        !encode_box(&down.acts[g], a.workspace_dev, Elem::kBf16, 3, h_dims, h_strides, box)) {
+      return false;
+    }
+  }
+  return true;
+}
+
 bool unaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
 }  // namespace
@@ -869,7 +872,7 @@ cudaError_t preload_decode_kernels() {
 }  // namespace bmoe
 
 extern "C" uint64_t bmoe_moe_decode_workspace(uint32_t tokens, uint32_t top_k, uint32_t inter) {
-  return (2ull * tokens * top_k * inter * sizeof(uint16_t) + 255) / 256 * 256;
+  return (2ull * tokens * top_k * inter * sizeof(uint16_t) + 255) / 256 * 256;   // h's halves
 }
 
 extern "C" int bmoe_moe_decode(const bmoe_moe_decode_args* args) {
@@ -914,18 +917,7 @@ extern "C" int bmoe_moe_decode(const bmoe_moe_decode_args* args) {
   k.by_expert = a.experts <= a.tokens * a.top_k ? 1u : 0u;
   bmoe::DecodeParams down;
   down.a = k;
-  const bmoe::Elem weight = int8 ? bmoe::Elem::kByte : bmoe::Elem::kBf16;
-  if (!bmoe::encode_matrix(&up.weights, a.w_gate_up_dev, 2ull * a.experts * a.inter, a.hidden, 64,
-                           weight) ||
-      !bmoe::encode_matrix(&up.acts, a.x_dev, a.tokens, a.hidden, bmoe::kGroup,
-                           bmoe::Elem::kBf16) ||
-      !bmoe::encode_matrix(&down.weights, a.w_down_dev,
-                           static_cast<uint64_t>(a.experts) * a.hidden, a.inter, bmoe::kRows,
-                           weight) ||
-      !bmoe::encode_matrix(&down.acts, a.workspace_dev, 2ull * a.tokens * a.top_k, a.inter,
-                           bmoe::kGroup, bmoe::Elem::kBf16)) {
-    return BMOE_CUDA_ERROR;
-  }
+  if (!bmoe::encode_maps(up, down, a, int8)) return BMOE_CUDA_ERROR;
   const cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
   const cudaError_t rc = int8 ? bmoe::dispatch_decode<true>(up, down, stream)
                               : bmoe::dispatch_decode<false>(up, down, stream);

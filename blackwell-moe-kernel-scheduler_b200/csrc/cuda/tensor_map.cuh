@@ -55,4 +55,29 @@ inline bool encode_matrix(CUtensorMap* map, const void* base, uint64_t rows, uin
   return rc == CUDA_SUCCESS;
 }
 
+// Box of a tensor of `rank` dimensions, innermost first: box[0] elements are 128 bytes of
+// contiguous memory (SWIZZLE_128B), strides[i] the bytes between neighbours of dimension i + 1,
+// each a multiple of the one before.
+inline bool encode_box(CUtensorMap* map, const void* base, Elem type, uint32_t rank,
+                       const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  EncodeTiledFn encode = encode_tiled_fn();
+  if (encode == nullptr || rank > 5) return false;
+  const CUtensorMapDataType kind =
+      type == Elem::kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                         : (type == Elem::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_UINT8);
+  cuuint64_t size[5], stride[4];
+  cuuint32_t extent[5];
+  const cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
+  for (uint32_t i = 0; i < rank; ++i) {
+    size[i] = dims[i];
+    extent[i] = box[i];
+    if (i + 1 < rank) stride[i] = strides[i];
+  }
+  return encode(map, kind, rank, const_cast<void*>(base), size, stride, extent, elem_strides,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace bmoe
