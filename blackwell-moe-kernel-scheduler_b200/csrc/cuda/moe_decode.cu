@@ -750,15 +750,23 @@ uint32_t split_of(uint64_t tiles, uint64_t blocks, uint32_t room, uint32_t most)
   return split;
 }
 
-template <typename Kernel>
-cudaError_t launch_cluster(Kernel kernel, dim3 grid, uint32_t threads, uint32_t ring_bytes,
-                           uint32_t reserved, uint32_t cluster, bool after_previous,
-                           const DecodeParams& params, cudaStream_t stream) {
-  // an attribute of the function on the current device: set per launch, nothing is cached
-  const uint32_t smem = 1024 + ring_bytes + reserved;
-  cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        static_cast<int>(smem));
+using DecodeKernel = void (*)(const DecodeParams, uint32_t);
+
+template <DecodeKernel kernel>
+cudaError_t launch_cluster(dim3 grid, uint32_t threads, uint32_t ring_bytes, uint32_t reserved,
+                           uint32_t cluster, bool after_previous, const DecodeParams& params,
+                           cudaStream_t stream) {
+  // The opt-in shared-memory size is a per-device function attribute.
+  static bool configured[64] = {};
+  int device = 0;
+  cudaError_t rc = cudaGetDevice(&device);
   if (rc != cudaSuccess) return rc;
+  if (device < 0 || device >= 64 || !configured[device]) {
+    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOnePerSm);
+    if (rc != cudaSuccess) return rc;
+    if (device >= 0 && device < 64) configured[device] = true;
+  }
+  const uint32_t smem = 1024 + ring_bytes + reserved;
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = dim3(threads);
@@ -789,8 +797,8 @@ cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cuda
   uint32_t split = split_of(static_cast<uint64_t>(tiles) * slots,
                             (a.hidden + kBlockK - 1) / kBlockK, 4 * sms, 8);
   cudaError_t rc =
-      launch_cluster(decode_up_kernel<INT8, COLS>, dim3(tiles * split, slots), kUpThreads<INT8>,
-                     kTwoPerSm - 1024, 0, split, false, up, stream);
+      launch_cluster<decode_up_kernel<INT8, COLS>>(dim3(tiles * split, slots), kUpThreads<INT8>,
+                                                   kTwoPerSm - 1024, 0, split, false, up, stream);
   if (rc != cudaSuccess) return rc;
   // The sums of many tokens leave less for the ring: two CTAs per SM if three stages fit at
   // twice the average number of an expert's tokens, else one, in clusters of 4 (of 8 with an
@@ -802,9 +810,9 @@ cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cuda
   const bool two = kTwoPerSm - 1024 >= reserved + 3 * (kABytes + kPieces * columns * 128);
   split = split_of(groups, static_cast<uint64_t>((a.inter + kBlockK - 1) / kBlockK) * slots,
                    two ? 2 * sms : sms, two ? 8 : 4);
-  return launch_cluster(decode_down_kernel<INT8, COLS>, dim3(groups * split), kDownThreads<INT8>,
-                        (two ? kTwoPerSm : kOnePerSm) - 1024 - reserved, reserved, split, true,
-                        down, stream);
+  return launch_cluster<decode_down_kernel<INT8, COLS>>(
+      dim3(groups * split), kDownThreads<INT8>, (two ? kTwoPerSm : kOnePerSm) - 1024 - reserved,
+      reserved, split, true, down, stream);
 }
 
 template <bool INT8>

@@ -13,8 +13,6 @@
 namespace bmoe {
 namespace {
 
-constexpr uint32_t kQuantThreads = 256;
-
 struct QuantizeArgs {
   const void* src;
   const int64_t* index;
@@ -26,6 +24,8 @@ struct QuantizeArgs {
   uint32_t cols;
 };
 
+constexpr uint32_t kUnit = 16;            // values a thread takes at a time: one 16-byte store
+
 // max of |values| that keeps a NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -33,51 +33,153 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-__device__ __forceinline__ float load_value(const float* p) { return *p; }
-__device__ __forceinline__ float load_value(const uint16_t* p) {
-  return __uint_as_float(static_cast<uint32_t>(*p) << 16);
-}
+// One unit in its own type.
+template <typename T>
+struct Unit {
+  static constexpr uint32_t kVectors = kUnit * sizeof(T) / 16;
+  uint4 v[kVectors];
 
-// Nearest integer, ties to even; what is not a number becomes -127 (the row's scale then
-// says NaN or inf).
-__device__ __forceinline__ int8_t to_int8(float v) {
-  const int q = __float2int_rn(fminf(fmaxf(v, -127.0f), 127.0f));
-  return static_cast<int8_t>(q);
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (uint32_t i = 0; i < kVectors; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (uint32_t i = 0; i < kVectors; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ float at(uint32_t i) const {
+    const uint32_t word = i * sizeof(T) / 4;
+    const uint4& four = v[word / 4];
+    const uint32_t bits =
+        word % 4 == 0 ? four.x : (word % 4 == 1 ? four.y : (word % 4 == 2 ? four.z : four.w));
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(bits);
+    } else {
+      return __uint_as_float(i % 2 == 0 ? bits << 16 : bits & 0xffff0000u);
+    }
+  }
+};
+
+// Nearest integer, ties to even, as the low byte of the result: 1.5 * 2^23 + v has it there for
+// |v| <= 127 (an FP32 addition rounds to nearest even at that magnitude). What is not a number
+// becomes -127; the row's scale then says NaN or inf.
+__device__ __forceinline__ uint32_t to_int8_bits(float v) {
+  return __float_as_uint(fminf(fmaxf(v, -127.0f), 127.0f) + 12582912.0f);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantizeArgs a) {
-  __shared__ float partial[kQuantThreads / 32];
-  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const int64_t from = a.index != nullptr ? a.index[r] : static_cast<int64_t>(r);
-    if (from < 0 || static_cast<uint64_t>(from) >= a.src_rows) continue;
-    const T* const row = static_cast<const T*>(a.src) + static_cast<uint64_t>(from) * a.src_stride;
-    float largest = 0.0f;
-    for (uint32_t c = threadIdx.x; c < a.cols; c += kQuantThreads) {
-      largest = max_nan(largest, fabsf(load_value(row + c)));
-    }
-    for (uint32_t d = 16; d > 0; d >>= 1) {
-      largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, d));
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) partial[threadIdx.x >> 5] = largest;
-    __syncthreads();
-    for (uint32_t w = 0; w < kQuantThreads / 32; ++w) largest = max_nan(largest, partial[w]);
-    largest = max_nan(largest, 0x1p-100f);
-    const float inverse = 127.0f * (1.0f / largest);
-    for (uint32_t c = threadIdx.x; c < a.cols; c += kQuantThreads) {
-      a.dst[r * a.cols + c] = to_int8(load_value(row + c) * inverse);
-    }
-    if (threadIdx.x == 0) a.scale[r] = largest / 127.0f;
+__device__ __forceinline__ void store_unit(int8_t* to, const Unit<T>& unit, float inverse) {
+  uint32_t word[4];
+#pragma unroll
+  for (uint32_t w = 0; w < 4; ++w) {
+    const uint32_t b0 = to_int8_bits(unit.at(4 * w) * inverse);
+    const uint32_t b1 = to_int8_bits(unit.at(4 * w + 1) * inverse);
+    const uint32_t b2 = to_int8_bits(unit.at(4 * w + 2) * inverse);
+    const uint32_t b3 = to_int8_bits(unit.at(4 * w + 3) * inverse);
+    word[w] = __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
   }
+  *reinterpret_cast<uint4*>(to) = make_uint4(word[0], word[1], word[2], word[3]);
+}
+
+// WARPS warps share a row; a CTA of one-warp rows holds four of them. A thread keeps HELD units
+// in registers between the maximum and the conversion, so a row is read once; what is
+// beyond (rows of more than 65536 values) is read again.
+template <typename T, uint32_t WARPS, uint32_t HELD>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS)
+quantize_rows_kernel(QuantizeArgs a) {
+  __shared__ float partial[WARPS];
+  constexpr uint32_t kThreads = 32 * WARPS;
+  const uint64_t r =
+      WARPS == 1 ? static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (r >= a.rows) return;
+  const uint32_t thread = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t from = a.index != nullptr ? a.index[r] : static_cast<int64_t>(r);
+  if (from < 0 || static_cast<uint64_t>(from) >= a.src_rows) return;
+  const T* const row = static_cast<const T*>(a.src) + static_cast<uint64_t>(from) * a.src_stride;
+  int8_t* const to = a.dst + r * a.cols;
+  const uint32_t units = a.cols / kUnit;
+
+  Unit<T> held[HELD];
+#pragma unroll
+  for (uint32_t i = 0; i < HELD; ++i) {
+    const uint32_t u = i * kThreads + thread;
+    if (u < units) {
+      held[i].load(row + u * kUnit);
+    } else {
+      held[i].clear();
+    }
+  }
+  float largest = 0x1p-100f;
+#pragma unroll
+  for (uint32_t i = 0; i < HELD; ++i) {
+#pragma unroll
+    for (uint32_t j = 0; j < kUnit; ++j) largest = max_nan(largest, fabsf(held[i].at(j)));
+  }
+  for (uint32_t u = HELD * kThreads + thread; u < units; u += kThreads) {
+    Unit<T> unit;
+    unit.load(row + u * kUnit);
+#pragma unroll
+    for (uint32_t j = 0; j < kUnit; ++j) largest = max_nan(largest, fabsf(unit.at(j)));
+  }
+#pragma unroll
+  for (uint32_t d = 16; d > 0; d >>= 1) {
+    largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, d));
+  }
+  if constexpr (WARPS > 1) {
+    if ((thread & 31) == 0) partial[thread >> 5] = largest;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < WARPS; ++w) largest = max_nan(largest, partial[w]);
+  }
+  const float inverse = 127.0f * (1.0f / largest);
+#pragma unroll
+  for (uint32_t i = 0; i < HELD; ++i) {
+    const uint32_t u = i * kThreads + thread;
+    if (u < units) store_unit(to + u * kUnit, held[i], inverse);
+  }
+  for (uint32_t u = HELD * kThreads + thread; u < units; u += kThreads) {
+    Unit<T> unit;
+    unit.load(row + u * kUnit);
+    store_unit(to + u * kUnit, unit, inverse);
+  }
+  if (thread == 0) a.scale[r] = largest / 127.0f;
+}
+
+template <typename T, uint32_t WARPS, uint32_t HELD>
+cudaError_t launch_quantize(const QuantizeArgs& a, cudaStream_t stream) {
+  const uint64_t grid = WARPS == 1 ? (a.rows + 3) / 4 : a.rows;
+  quantize_rows_kernel<T, WARPS, HELD>
+      <<<static_cast<uint32_t>(grid), WARPS == 1 ? 128 : 32 * WARPS, 0, stream>>>(a);
+  return cudaPeekAtLastError();
+}
+
+// Threads by the length of a row: about four units (64 values) each.
+template <typename T>
+cudaError_t dispatch_quantize(const QuantizeArgs& a, cudaStream_t stream) {
+  if (a.cols <= 512) return launch_quantize<T, 1, 1>(a, stream);
+  if (a.cols <= 2048) return launch_quantize<T, 1, 4>(a, stream);
+  if (a.cols <= 4096) return launch_quantize<T, 4, 2>(a, stream);
+  if (a.cols <= 8192) return launch_quantize<T, 4, 4>(a, stream);
+  if (a.cols <= 16384) return launch_quantize<T, 8, 4>(a, stream);
+  return launch_quantize<T, 32, 4>(a, stream);
+}
+
+template <typename T>
+cudaError_t preload_quantize() {
+  cudaError_t rc = preload_one(quantize_rows_kernel<T, 1, 1>);
+  if (rc == cudaSuccess) rc = preload_one(quantize_rows_kernel<T, 1, 4>);
+  if (rc == cudaSuccess) rc = preload_one(quantize_rows_kernel<T, 4, 2>);
+  if (rc == cudaSuccess) rc = preload_one(quantize_rows_kernel<T, 4, 4>);
+  if (rc == cudaSuccess) rc = preload_one(quantize_rows_kernel<T, 8, 4>);
+  if (rc == cudaSuccess) rc = preload_one(quantize_rows_kernel<T, 32, 4>);
+  return rc;
 }
 
 }  // namespace
 
 cudaError_t preload_quantize_kernels() {
-  cudaError_t rc = preload_one(quantize_rows_kernel<uint16_t>);
-  if (rc == cudaSuccess) rc = preload_one(quantize_rows_kernel<float>);
-  return rc;
+  const cudaError_t rc = preload_quantize<uint16_t>();
+  return rc == cudaSuccess ? preload_quantize<float>() : rc;
 }
 
 }  // namespace bmoe
@@ -90,6 +192,7 @@ extern "C" int bmoe_quantize_rows(const bmoe_quantize_rows_args* args) {
   }
   const uint32_t elem = a.src_type == BMOE_TYPE_BF16 ? 2u : 4u;
   if (a.cols == 0 || a.cols % 16 != 0 ||
+      a.rows > 0x7fffffffull ||
       (a.src_stride != 0 && (a.src_stride < a.cols || a.src_stride % (16 / elem) != 0))) {
     return BMOE_INVALID_ARGUMENT;
   }
@@ -109,13 +212,8 @@ extern "C" int bmoe_quantize_rows(const bmoe_quantize_rows_args* args) {
   k.src_rows = a.src_rows;
   k.src_stride = a.src_stride != 0 ? a.src_stride : a.cols;
   k.cols = a.cols;
-  const uint64_t resident = 8ull * bmoe::device_sm_count();
-  const uint32_t grid = static_cast<uint32_t>(a.rows < resident ? a.rows : resident);
   const cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
-  if (elem == 2) {
-    bmoe::quantize_rows_kernel<uint16_t><<<grid, bmoe::kQuantThreads, 0, stream>>>(k);
-  } else {
-    bmoe::quantize_rows_kernel<float><<<grid, bmoe::kQuantThreads, 0, stream>>>(k);
-  }
-  return cudaPeekAtLastError() == cudaSuccess ? BMOE_OK : BMOE_CUDA_ERROR;
+  const cudaError_t rc = elem == 2 ? bmoe::dispatch_quantize<uint16_t>(k, stream)
+                                   : bmoe::dispatch_quantize<float>(k, stream);
+  return rc == cudaSuccess ? BMOE_OK : BMOE_CUDA_ERROR;
 }

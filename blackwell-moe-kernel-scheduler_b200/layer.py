@@ -20,34 +20,46 @@ from . import _capi
 _ROW_TYPES = {torch.bfloat16: _capi.TYPE_BF16, torch.float32: _capi.TYPE_FP32}
 _WEIGHT_TYPES = {torch.bfloat16: _capi.TYPE_BF16, torch.int8: _capi.TYPE_INT8}
 _NO_GUARD = contextlib.nullcontext()
+# the raw handle of a device's current stream, without building a Stream object
+_current_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _require(condition, message: str) -> None:
-    if not condition:
-        raise ValueError(message)
+def _on(index: int):
+    """Context in which device ``index`` is the current one."""
+    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-def _on(device):
-    """Context in which ``device`` is the current one."""
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _stream(stream, device) -> int | None:
+def _raw_stream(stream, index: int) -> int | None:
     if stream is None:
-        stream = torch.cuda.current_stream(device)
+        return _current_raw_stream(index) or None
     return int(getattr(stream, "cuda_stream", stream)) or None
 
 
-def _check_rows(x, name: str) -> None:
-    _require(x.is_cuda, f"{name}: the engine has no CPU path, a CUDA tensor is needed")
-    _require(x.dim() == 2 and x.dtype in _ROW_TYPES, f"{name}: BF16 or FP32 [rows, columns]")
-    _require(x.stride(1) == 1 or x.shape[1] <= 1, f"{name}: columns must be contiguous")
+def _is(x, dtype, shape, index: int) -> bool:
+    """``x`` is a contiguous tensor of that type and shape on CUDA device ``index``."""
+    return (x.dtype is dtype and x.shape == shape and x.is_cuda and x.get_device() == index
+            and x.is_contiguous())
 
 
-def _check(x, name: str, dtype, shape, device) -> None:
-    _require(x.dtype is dtype and x.device == device and tuple(x.shape) == tuple(shape)
-             and x.is_contiguous(),
-             f"{name}: contiguous {dtype} {list(shape)} on {device} needed")
+def _need(x, name: str, dtype, shape, index: int) -> None:
+    if not _is(x, dtype, shape, index):
+        raise ValueError(f"{name}: contiguous {dtype} {list(shape)} on cuda:{index} needed, got "
+                         f"{x.dtype} {list(x.shape)} on {x.device}")
+
+
+def _rows(x, name: str):
+    """Rows, columns, row stride and device of a row matrix with contiguous columns."""
+    if not x.is_cuda:
+        raise ValueError(f"{name}: the engine has no CPU path, a CUDA tensor is needed")
+    if x.dim() != 2 or x.dtype not in _ROW_TYPES:
+        raise ValueError(f"{name}: BF16 or FP32 [rows, columns] needed")
+    rows, cols = x.shape
+    stride, inner = x.stride()
+    if inner != 1 and cols > 1:
+        raise ValueError(f"{name}: columns must be contiguous")
+    if rows > 1 and stride < cols:
+        raise ValueError(f"{name}: rows must not overlap")
+    return rows, cols, stride if rows > 1 else 0, x.get_device()
 
 
 def route_topk(logits, top_k: int, *, scoring: str = "softmax", renormalize: bool = False,
@@ -59,27 +71,24 @@ def route_topk(logits, top_k: int, *, scoring: str = "softmax", renormalize: boo
     lower id. ``scoring`` "softmax" or "sigmoid"; ``bias`` [experts] float32 is added to a
     sigmoid score for the choice only; ``renormalize`` divides by the sum over the chosen.
     Experts at -inf or NaN are never chosen; a token left with fewer gets id -1, weight 0."""
-    _check_rows(logits, "logits")
-    _require(scoring in _capi.SCORINGS, f"unknown scoring: {scoring}")
-    tokens, experts = logits.shape
-    device = logits.device
+    tokens, experts, row_stride, index = _rows(logits, "logits")
+    if scoring not in _capi.SCORINGS:
+        raise ValueError(f"unknown scoring: {scoring}")
     if bias is not None:
-        _check(bias, "bias", torch.float32, (experts,), device)
-    with _on(device):
+        _need(bias, "bias", torch.float32, (experts,), index)
+    with _on(index):
         if expert_ids is None:
-            expert_ids = torch.empty(tokens, top_k, dtype=torch.int64, device=device)
+            expert_ids = torch.empty(tokens, top_k, dtype=torch.int64, device=logits.device)
         else:
-            _check(expert_ids, "expert_ids", torch.int64, (tokens, top_k), device)
+            _need(expert_ids, "expert_ids", torch.int64, (tokens, top_k), index)
         if weights is None:
-            weights = torch.empty(tokens, top_k, dtype=torch.float32, device=device)
+            weights = torch.empty(tokens, top_k, dtype=torch.float32, device=logits.device)
         else:
-            _check(weights, "weights", torch.float32, (tokens, top_k), device)
-        _require(tokens <= 1 or logits.stride(0) >= experts, "logits: rows must not overlap")
+            _need(weights, "weights", torch.float32, (tokens, top_k), index)
         args = _capi.RouteTopkArgs(
             logits.data_ptr(), None if bias is None else bias.data_ptr(), expert_ids.data_ptr(),
-            weights.data_ptr(), tokens, logits.stride(0) if tokens > 1 else 0, experts, top_k,
-            _ROW_TYPES[logits.dtype], _capi.SCORINGS[scoring], int(renormalize), scale,
-            _stream(stream, device))
+            weights.data_ptr(), tokens, row_stride, experts, top_k, _ROW_TYPES[logits.dtype],
+            _capi.SCORINGS[scoring], int(renormalize), scale, _raw_stream(stream, index))
         _capi.check(_capi.load().bmoe_route_topk(C.byref(args)), "bmoe_route_topk")
     return expert_ids, weights
 
@@ -90,28 +99,24 @@ def quantize_rows(x, index=None, *, out=None, scale=None, stream=None):
     Returns ``(q int8, scale float32)`` with ``x[i] ~ q[i] * scale[i]``: the A operand and
     ``row_scale`` of an INT8 product. With ``index`` (int64) output row i is row
     ``index[i]``; an index outside ``x`` leaves its output row untouched."""
-    _check_rows(x, "x")
-    device = x.device
-    src_rows, cols = x.shape
+    src_rows, cols, row_stride, device = _rows(x, "x")
     rows = src_rows
     if index is not None:
-        _require(index.dim() == 1, "index: one dimension")
-        rows = index.shape[0]
-        _check(index, "index", torch.int64, (rows,), device)
-    _require(src_rows <= 1 or x.stride(0) >= cols, "x: rows must not overlap")
+        rows = index.numel()
+        _need(index, "index", torch.int64, (rows,), device)
     with _on(device):
         if out is None:
-            out = torch.empty(rows, cols, dtype=torch.int8, device=device)
+            out = torch.empty(rows, cols, dtype=torch.int8, device=x.device)
         else:
-            _check(out, "out", torch.int8, (rows, cols), device)
+            _need(out, "out", torch.int8, (rows, cols), device)
         if scale is None:
-            scale = torch.empty(rows, dtype=torch.float32, device=device)
+            scale = torch.empty(rows, dtype=torch.float32, device=x.device)
         else:
-            _check(scale, "scale", torch.float32, (rows,), device)
+            _need(scale, "scale", torch.float32, (rows,), device)
         args = _capi.QuantizeRowsArgs(
             x.data_ptr(), None if index is None else index.data_ptr(), out.data_ptr(),
-            scale.data_ptr(), rows, src_rows, x.stride(0) if src_rows > 1 else 0, cols,
-            _ROW_TYPES[x.dtype], _stream(stream, device))
+            scale.data_ptr(), rows, src_rows, row_stride, cols, _ROW_TYPES[x.dtype],
+            _raw_stream(stream, device))
         _capi.check(_capi.load().bmoe_quantize_rows(C.byref(args)), "bmoe_quantize_rows")
     return out, scale
 
@@ -134,45 +139,45 @@ def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
 
     ``workspace``: contiguous uint8 tensor of ``moe_decode_workspace`` bytes, for callers that
     keep one; calls that may overlap need one each."""
-    _require(x.is_cuda, "x: the engine has no CPU path, a CUDA tensor is needed")
-    device = x.device
-    _require(x.dim() == 2 and w_gate_up.dim() == 3 and expert_ids.dim() == 2,
-             "x [tokens, hidden], w_gate_up [experts, 2 * inter, hidden], "
-             "expert_ids [tokens, top_k] needed")
-    tokens, hidden = x.shape
-    experts, both = w_gate_up.shape[:2]
-    inter, top_k = both // 2, expert_ids.shape[1]
+    if not x.is_cuda:
+        raise ValueError("x: the engine has no CPU path, a CUDA tensor is needed")
+    if x.dim() != 2 or w_gate_up.dim() != 3 or expert_ids.dim() != 2:
+        raise ValueError("x [tokens, hidden], w_gate_up [experts, 2 * inter, hidden] and "
+                         "expert_ids [tokens, top_k] needed")
     kind = w_gate_up.dtype
-    _require(kind in _WEIGHT_TYPES and both % 2 == 0, "w_gate_up: BF16 or INT8, 2 * inter rows")
-    _check(x, "x", torch.bfloat16, (tokens, hidden), device)
-    _check(w_gate_up, "w_gate_up", kind, (experts, 2 * inter, hidden), device)
-    _check(w_down, "w_down", kind, (experts, hidden, inter), device)
-    _check(expert_ids, "expert_ids", torch.int64, (tokens, top_k), device)
-    _check(weights, "weights", torch.float32, (tokens, top_k), device)
-    if kind is torch.int8:
-        _require(gate_up_scale is not None and down_scale is not None,
-                 "INT8 weights need gate_up_scale and down_scale")
-        _check(gate_up_scale, "gate_up_scale", torch.float32, (experts, 2 * inter), device)
-        _check(down_scale, "down_scale", torch.float32, (experts, hidden), device)
-    else:
-        _require(gate_up_scale is None and down_scale is None, "BF16 weights have no scales")
+    if kind not in _WEIGHT_TYPES:
+        raise ValueError("w_gate_up: BF16 or INT8 weights")
+    int8 = kind is torch.int8
+    if int8 != (gate_up_scale is not None) or int8 != (down_scale is not None):
+        raise ValueError("INT8 weights have gate_up_scale and down_scale, BF16 weights none")
+    index = x.get_device()
+    tokens, hidden = x.shape
+    experts, both, _ = w_gate_up.shape
+    inter, top_k = both // 2, expert_ids.shape[1]
+    _need(x, "x", torch.bfloat16, (tokens, hidden), index)
+    _need(w_gate_up, "w_gate_up", kind, (experts, 2 * inter, hidden), index)
+    _need(w_down, "w_down", kind, (experts, hidden, inter), index)
+    _need(expert_ids, "expert_ids", torch.int64, (tokens, top_k), index)
+    _need(weights, "weights", torch.float32, (tokens, top_k), index)
+    if int8:
+        _need(gate_up_scale, "gate_up_scale", torch.float32, (experts, 2 * inter), index)
+        _need(down_scale, "down_scale", torch.float32, (experts, hidden), index)
     lib = _capi.load()
-    with _on(device):
+    with _on(index):
         if out is None:
-            out = torch.empty(tokens, hidden, dtype=torch.bfloat16, device=device)
+            out = torch.empty_like(x)
         else:
-            _check(out, "out", torch.bfloat16, (tokens, hidden), device)
+            _need(out, "out", torch.bfloat16, (tokens, hidden), index)
         if workspace is None:
-            need = lib.bmoe_moe_decode_workspace(tokens, top_k, inter)
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            workspace = torch.empty(lib.bmoe_moe_decode_workspace(tokens, top_k, inter),
+                                    dtype=torch.uint8, device=x.device)
         else:
-            _require(workspace.dtype is torch.uint8 and workspace.device == device
-                     and workspace.is_contiguous(), "workspace: contiguous uint8 tensor")
+            _need(workspace, "workspace", torch.uint8, (workspace.numel(),), index)
         args = _capi.MoeDecodeArgs(
             x.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(),
-            None if gate_up_scale is None else gate_up_scale.data_ptr(),
-            None if down_scale is None else down_scale.data_ptr(), expert_ids.data_ptr(),
-            weights.data_ptr(), out.data_ptr(), workspace.data_ptr(), workspace.numel(),
-            tokens, top_k, experts, hidden, inter, _WEIGHT_TYPES[kind], _stream(stream, device))
+            gate_up_scale.data_ptr() if int8 else None, down_scale.data_ptr() if int8 else None,
+            expert_ids.data_ptr(), weights.data_ptr(), out.data_ptr(), workspace.data_ptr(),
+            workspace.numel(), tokens, top_k, experts, hidden, inter, _WEIGHT_TYPES[kind],
+            _raw_stream(stream, index))
         _capi.check(lib.bmoe_moe_decode(C.byref(args)), "bmoe_moe_decode")
     return out

@@ -186,7 +186,7 @@ def quantize_oracle(x):
 
 @pytest.mark.parametrize("rows,cols", [
     (1, 16), (3, 48), (5, 512), (2, 2048), (300, 272), (7, 7168), (4, 4112), (2, 16384),
-    (3, 20000), (2, 40016), (2500, 64)])
+    (3, 20000), (2, 40016), (2500, 64), (9, 3008), (2, 70016), (6, 6400)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_quantize_rows(engine, rows, cols, dtype):
     g = gen(rows + cols)

@@ -59,6 +59,7 @@ def quantize_args(cap, **change):
     (dict(src_dev=None), "INVALID_ARGUMENT"),
     (dict(dst_dev=None), "INVALID_ARGUMENT"),
     (dict(scale_dev=None), "INVALID_ARGUMENT"),
+    (dict(rows=1 << 31, src_rows=1 << 31), "INVALID_ARGUMENT"),
     (dict(rows=5), "INVALID_ARGUMENT"),                # no index: row i is source row i
     (dict(rows=0, src_dev=None), "OK"),
 ])
