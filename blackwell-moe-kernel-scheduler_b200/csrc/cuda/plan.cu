@@ -81,19 +81,26 @@ struct bmoe_plan {
   cudaStream_t default_stream = nullptr;
   cudaStream_t setup_stream = nullptr;
   cudaStream_t last_stream = nullptr;
-  cudaEvent_t setup_done = nullptr;
   int device = -1;
 
   // One metadata block, filled by a single copy from pinned staging memory:
   //   [0, 256) queue words   [256, 512) DeviceStatus
   //   [512, ...) counts uint32 [experts]   then CUtensorMap [3][experts] (128-aligned)
   DeviceBlock meta;
-  PinnedBlock staging;
+  // Two staging areas take turns, so that a re-plan waits for the set-up before the last one
+  // only: with one area the host would wait until the stream has reached the previous
+  // set-up, i.e. until the launch before it has finished, and the GPU would idle meanwhile.
+  struct Setup {
+    PinnedBlock staging;
+    cudaEvent_t done = nullptr;
+  } setup[2];
+  uint32_t turn = 0;   // the area of the current plan
   DeviceBlock worklist;   // bmoe_tile [capacity]
   DeviceBlock workspace;  // worklist builder arrays
 
-  // What the B descriptors in the staging area were encoded for (reused while the
-  // expert's weight pointer, the shape and the box do not change).
+  // B descriptors and what they were encoded for (reused while the expert's weight pointer,
+  // the shape and the box do not change).
+  std::vector<CUtensorMap> b_maps;
   std::vector<const void*> b_encoded_for;
   uint32_t b_key_n = 0, b_key_k = 0, b_key_box = 0, b_key_experts = 0, b_key_type = 0;
   bool needs_push = false;   // results_pushed: run() only after set_push
@@ -108,12 +115,14 @@ struct bmoe_plan {
 
   void release_all() {
     meta.release();
-    staging.release();
+    for (Setup& s : setup) {
+      s.staging.release();
+      if (s.done != nullptr) cudaEventDestroy(s.done);
+      s.done = nullptr;
+    }
     b_encoded_for.clear();
     worklist.release();
     workspace.release();
-    if (setup_done != nullptr) cudaEventDestroy(setup_done);
-    setup_done = nullptr;
     ready = false;
   }
 };
@@ -286,6 +295,7 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
   }
   if (packed && !dev_counts && routed_rows > a.packed_rows) return BMOE_INVALID_ARGUMENT;
   plan->stats.active_experts = active;
+  const cudaStream_t previous_stream = plan->setup_stream;
   plan->default_stream = static_cast<cudaStream_t>(a.stream);
   plan->setup_stream = plan->default_stream;
   plan->last_stream = plan->default_stream;
@@ -364,23 +374,29 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
   const size_t off_scales = off_maps + map_bytes;
   const size_t meta_bytes =
       off_scales + (int8 ? 2 * sizeof(float*) * static_cast<size_t>(a.experts) : 0);
-  const void* const staging_before = plan->staging.ptr;
-  if (!plan->meta.reserve(meta_bytes) || !plan->staging.reserve(meta_bytes) ||
+  bmoe_plan::Setup& before = plan->setup[plan->turn];
+  plan->turn ^= 1u;
+  bmoe_plan::Setup& setup = plan->setup[plan->turn];
+  // on another stream than the last set-up, this one follows it
+  if (before.done != nullptr && previous_stream != plan->setup_stream &&
+      cudaStreamWaitEvent(plan->setup_stream, before.done, 0) != cudaSuccess) {
+    return BMOE_CUDA_ERROR;
+  }
+  if (setup.done == nullptr) {
+    if (cudaEventCreateWithFlags(&setup.done, cudaEventDisableTiming) != cudaSuccess) {
+      return BMOE_CUDA_ERROR;
+    }
+  } else if (cudaEventSynchronize(setup.done) != cudaSuccess) {
+    // the copy of the set-up before the last one still reads this staging area
+    return BMOE_CUDA_ERROR;
+  }
+  if (!plan->meta.reserve(meta_bytes) || !setup.staging.reserve(meta_bytes) ||
       !plan->worklist.reserve(sizeof(bmoe_tile) * static_cast<size_t>(tiles)) ||
       !plan->workspace.reserve(layout.bytes)) {
     return BMOE_CUDA_ERROR;
   }
-  if (plan->setup_done == nullptr) {
-    if (cudaEventCreateWithFlags(&plan->setup_done, cudaEventDisableTiming) != cudaSuccess) {
-      return BMOE_CUDA_ERROR;
-    }
-  } else if (cudaEventSynchronize(plan->setup_done) != cudaSuccess) {
-    // the previous set-up copy still reads the staging area
-    return BMOE_CUDA_ERROR;
-  }
-  const bool staging_moved = plan->staging.ptr != staging_before;
-  cudaStream_t stream = plan->setup_stream;
-  uint8_t* const stage = static_cast<uint8_t*>(plan->staging.ptr);
+  const cudaStream_t stream = plan->setup_stream;
+  uint8_t* const stage = static_cast<uint8_t*>(setup.staging.ptr);
   uint8_t* const meta = static_cast<uint8_t*>(plan->meta.ptr);
 
   // ---- queue and status words, counts, one TMA descriptor triple per active expert ----
@@ -394,15 +410,17 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
   CUtensorMap* const maps_a = reinterpret_cast<CUtensorMap*>(stage + off_maps);
   CUtensorMap* const maps_b = maps_a + a.experts;
   CUtensorMap* const maps_d = maps_b + a.experts;
-  // B descriptors survive in the staging area from the previous initialize when the
-  // layout of that area, the shape and the box are the same; only experts whose weight
-  // pointer changed are encoded again.
+  // B descriptors survive from the previous initialize when the shape and the box are the
+  // same; only experts whose weight pointer changed are encoded again.
   const uint32_t b_box = tile_n / cta_group;
-  const bool b_cache_valid = !staging_moved && plan->b_key_experts == a.experts &&
+  const bool b_cache_valid = plan->b_key_experts == a.experts &&
                              plan->b_key_n == a.n && plan->b_key_k == a.k &&
                              plan->b_key_box == b_box && plan->b_key_type == a.data_type &&
                              plan->b_encoded_for.size() == a.experts;
-  if (!b_cache_valid) plan->b_encoded_for.assign(a.experts, nullptr);
+  if (!b_cache_valid) {
+    plan->b_encoded_for.assign(a.experts, nullptr);
+    plan->b_maps.resize(a.experts);
+  }
   plan->b_key_experts = a.experts;
   plan->b_key_n = a.n;
   plan->b_key_k = a.k;
@@ -427,16 +445,19 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
       if (!packed || e != 0) std::memset(&maps_a[e], 0, sizeof(CUtensorMap));
       std::memset(&maps_b[e], 0, sizeof(CUtensorMap));
       std::memset(&maps_d[e], 0, sizeof(CUtensorMap));
-      plan->b_encoded_for[e] = nullptr;
       continue;
     }
     if (!packed && !encode_matrix(&maps_a[e], a.a[e], rows, a.k, a_box_rows, operand)) {
       return BMOE_CUDA_ERROR;
     }
     if (plan->b_encoded_for[e] != a.b[e]) {
-      if (!encode_matrix(&maps_b[e], a.b[e], a.n, a.k, b_box, operand)) return BMOE_CUDA_ERROR;
+      if (!encode_matrix(&plan->b_maps[e], a.b[e], a.n, a.k, b_box, operand)) {
+        plan->b_encoded_for[e] = nullptr;
+        return BMOE_CUDA_ERROR;
+      }
       plan->b_encoded_for[e] = a.b[e];
     }
+    maps_b[e] = plan->b_maps[e];
     if (!pushed && !encode_matrix(&maps_d[e], a.d[e], rows, a.n, 32,
                                   out_f32 ? Elem::kF32 : Elem::kBf16)) {
       return BMOE_CUDA_ERROR;
@@ -468,7 +489,7 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
                                static_cast<bmoe_tile*>(plan->worklist.ptr), tiles,
                                plan->workspace.ptr, stream);
   if (rc != BMOE_OK) return rc;
-  if (cudaEventRecord(plan->setup_done, stream) != cudaSuccess) return BMOE_CUDA_ERROR;
+  if (cudaEventRecord(setup.done, stream) != cudaSuccess) return BMOE_CUDA_ERROR;
 
   // ---- launch parameters ----
   const CUtensorMap* const dev_maps = reinterpret_cast<const CUtensorMap*>(meta + off_maps);
@@ -638,7 +659,7 @@ int bmoe_plan_run(bmoe_plan* plan, void* stream) {
   cudaStream_t s = stream == nullptr ? plan->default_stream
                                      : static_cast<cudaStream_t>(stream);
   if (s != plan->setup_stream &&
-      cudaStreamWaitEvent(s, plan->setup_done, 0) != cudaSuccess) {
+      cudaStreamWaitEvent(s, plan->setup[plan->turn].done, 0) != cudaSuccess) {
     return BMOE_CUDA_ERROR;
   }
   const cudaError_t err =
