@@ -26,10 +26,11 @@ struct QuantizeArgs {
 
 constexpr uint32_t kUnit = 16;            // values a thread takes at a time: one 16-byte store
 
-// max of |values| that keeps a NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// Without their sign, floats have the order of their bits, NaN above infinity: the largest
+// |value| of a row is an integer maximum, two BF16 values at a time.
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
@@ -47,6 +48,22 @@ struct Unit {
 #pragma unroll
     for (uint32_t i = 0; i < kVectors; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
   }
+  // Running maximum of |values|, as bits: of pairs for BF16.
+  __device__ __forceinline__ uint32_t raise(uint32_t most) const {
+#pragma unroll
+    for (uint32_t i = 0; i < kVectors; ++i) {
+      const uint32_t words[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (uint32_t w = 0; w < 4; ++w) {
+        if constexpr (sizeof(T) == 4) {
+          most = max(most, words[w] & 0x7fffffffu);
+        } else {
+          most = max_pair(most, words[w] & 0x7fff7fffu);
+        }
+      }
+    }
+    return most;
+  }
   __device__ __forceinline__ float at(uint32_t i) const {
     const uint32_t word = i * sizeof(T) / 4;
     const uint4& four = v[word / 4];
@@ -60,11 +77,12 @@ struct Unit {
   }
 };
 
-// Nearest integer, ties to even, as the low byte of the result: 1.5 * 2^23 + v has it there for
-// |v| <= 127 (an FP32 addition rounds to nearest even at that magnitude). What is not a number
-// becomes -127; the row's scale then says NaN or inf.
-__device__ __forceinline__ uint32_t to_int8_bits(float v) {
-  return __float_as_uint(fminf(fmaxf(v, -127.0f), 127.0f) + 12582912.0f);
+// Nearest integer, ties to even, as the low byte of the result: 1.5 * 2^23 + v has it there (an
+// FP32 addition rounds to nearest even at that magnitude). |v| is at most 127 and a few
+// roundings, so the integer is at most 127. What is not a number becomes -1; the row's scale
+// then says NaN or inf. The product is rounded by itself (no fused multiply-add).
+__device__ __forceinline__ uint32_t to_int8_bits(float v, float inverse) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(v, inverse), 12582912.0f));
 }
 
 template <typename T>
@@ -72,10 +90,10 @@ __device__ __forceinline__ void store_unit(int8_t* to, const Unit<T>& unit, floa
   uint32_t word[4];
 #pragma unroll
   for (uint32_t w = 0; w < 4; ++w) {
-    const uint32_t b0 = to_int8_bits(unit.at(4 * w) * inverse);
-    const uint32_t b1 = to_int8_bits(unit.at(4 * w + 1) * inverse);
-    const uint32_t b2 = to_int8_bits(unit.at(4 * w + 2) * inverse);
-    const uint32_t b3 = to_int8_bits(unit.at(4 * w + 3) * inverse);
+    const uint32_t b0 = to_int8_bits(unit.at(4 * w), inverse);
+    const uint32_t b1 = to_int8_bits(unit.at(4 * w + 1), inverse);
+    const uint32_t b2 = to_int8_bits(unit.at(4 * w + 2), inverse);
+    const uint32_t b3 = to_int8_bits(unit.at(4 * w + 3), inverse);
     word[w] = __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
   }
   *reinterpret_cast<uint4*>(to) = make_uint4(word[0], word[1], word[2], word[3]);
@@ -87,7 +105,7 @@ __device__ __forceinline__ void store_unit(int8_t* to, const Unit<T>& unit, floa
 template <typename T, uint32_t WARPS, uint32_t HELD>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS)
 quantize_rows_kernel(QuantizeArgs a) {
-  __shared__ float partial[WARPS];
+  __shared__ uint32_t partial[WARPS];
   constexpr uint32_t kThreads = 32 * WARPS;
   const uint64_t r =
       WARPS == 1 ? static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
@@ -109,29 +127,25 @@ quantize_rows_kernel(QuantizeArgs a) {
       held[i].clear();
     }
   }
-  float largest = 0x1p-100f;
+  uint32_t most = 0;
 #pragma unroll
-  for (uint32_t i = 0; i < HELD; ++i) {
-#pragma unroll
-    for (uint32_t j = 0; j < kUnit; ++j) largest = max_nan(largest, fabsf(held[i].at(j)));
-  }
+  for (uint32_t i = 0; i < HELD; ++i) most = held[i].raise(most);
   for (uint32_t u = HELD * kThreads + thread; u < units; u += kThreads) {
     Unit<T> unit;
     unit.load(row + u * kUnit);
-#pragma unroll
-    for (uint32_t j = 0; j < kUnit; ++j) largest = max_nan(largest, fabsf(unit.at(j)));
+    most = unit.raise(most);
   }
-#pragma unroll
-  for (uint32_t d = 16; d > 0; d >>= 1) {
-    largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, d));
-  }
+  if constexpr (sizeof(T) == 2) most = max(most << 16, most & 0xffff0000u);
+  most = __reduce_max_sync(0xffffffffu, most);
   if constexpr (WARPS > 1) {
-    if ((thread & 31) == 0) partial[thread >> 5] = largest;
+    if ((thread & 31) == 0) partial[thread >> 5] = most;
     __syncthreads();
 #pragma unroll
-    for (uint32_t w = 0; w < WARPS; ++w) largest = max_nan(largest, partial[w]);
+    for (uint32_t w = 0; w < WARPS; ++w) most = max(most, partial[w]);
   }
-  const float inverse = 127.0f * (1.0f / largest);
+  // the floor 2^-100; NaN stays (its bits are above)
+  const float largest = __uint_as_float(max(most, __float_as_uint(0x1p-100f)));
+  const float inverse = __fmul_rn(127.0f, __fdiv_rn(1.0f, largest));
 #pragma unroll
   for (uint32_t i = 0; i < HELD; ++i) {
     const uint32_t u = i * kThreads + thread;

@@ -64,10 +64,46 @@ __device__ __forceinline__ float load_logit(const uint16_t* p) {
 }
 
 // top_k rounds of "largest key, lowest id" over the lane's V keys (key i belongs to
-// expert i * 32 + lane). Lane j returns the id of the j-th choice (or -1).
+// expert i * 32 + lane). Lane j returns the id of the j-th choice (or -1). Up to 8 keys are
+// sorted first (odd-even transposition, equal keys stay in the order of their ids), so that
+// a round only looks at the front one: two warp operations and one shift.
 template <typename Key, uint32_t V>
 __device__ __forceinline__ int choose(Key (&key)[V], uint32_t top_k, uint32_t lane) {
   int mine = -1;
+  if constexpr (V <= 8) {
+    uint32_t id[V];
+#pragma unroll
+    for (uint32_t i = 0; i < V; ++i) id[i] = i * 32 + lane;
+#pragma unroll
+    for (uint32_t round = 0; round < V; ++round) {
+#pragma unroll
+      for (uint32_t i = round & 1; i + 1 < V; i += 2) {
+        if (key[i + 1] > key[i]) {
+          const Key k = key[i];
+          key[i] = key[i + 1];
+          key[i + 1] = k;
+          const uint32_t e = id[i];
+          id[i] = id[i + 1];
+          id[i + 1] = e;
+        }
+      }
+    }
+    for (uint32_t j = 0; j < top_k; ++j) {
+      const Key top = warp_max(key[0]);
+      if (top == 0) break;   // nothing left that can be chosen
+      const uint32_t chosen = __reduce_min_sync(kFull, key[0] == top ? id[0] : kFull);
+      if (lane == j) mine = static_cast<int>(chosen);
+      if (id[0] == chosen) {
+#pragma unroll
+        for (uint32_t i = 0; i + 1 < V; ++i) {
+          key[i] = key[i + 1];
+          id[i] = id[i + 1];
+        }
+        key[V - 1] = 0;
+      }
+    }
+    return mine;
+  }
   for (uint32_t j = 0; j < top_k; ++j) {
     Key best = 0;
     uint32_t at = 0;
