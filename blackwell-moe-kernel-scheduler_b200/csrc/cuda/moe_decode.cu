@@ -21,6 +21,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "bmoe_b200.h"
@@ -743,76 +744,125 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
 
 // ------------------------------------------------------------------ launch --
 
-// CTAs along k: up to `most` while the grid leaves room and every CTA keeps two k-blocks.
-uint32_t split_of(uint64_t tiles, uint64_t blocks, uint32_t room, uint32_t most) {
-  uint32_t split = 1;
-  while (split < most && tiles * split * 2 <= room && split * 4 <= blocks) split *= 2;
-  return split;
-}
-
 using DecodeKernel = void (*)(const DecodeParams, uint32_t);
 
-template <DecodeKernel kernel>
-cudaError_t launch_cluster(dim3 grid, uint32_t threads, uint32_t ring_bytes, uint32_t reserved,
-                           uint32_t cluster, bool after_previous, const DecodeParams& params,
-                           cudaStream_t stream) {
-  // The opt-in shared-memory size is a per-device function attribute.
-  static bool configured[64] = {};
-  int device = 0;
-  cudaError_t rc = cudaGetDevice(&device);
-  if (rc != cudaSuccess) return rc;
-  if (device < 0 || device >= 64 || !configured[device]) {
-    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOnePerSm);
-    if (rc != cudaSuccess) return rc;
-    if (device >= 0 && device < 64) configured[device] = true;
-  }
-  const uint32_t smem = 1024 + ring_bytes + reserved;
+struct Launch {
   cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
-  config.blockDim = dim3(threads);
-  config.dynamicSmemBytes = smem;
-  config.stream = stream;
   cudaLaunchAttribute attribute[2];
-  attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = cluster;
-  attribute[0].val.clusterDim.y = 1;
-  attribute[0].val.clusterDim.z = 1;
-  attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[1].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attribute;
-  config.numAttrs = after_previous ? 2 : 1;
-  rc = cudaLaunchKernelEx(&config, kernel, params, ring_bytes);
+
+  Launch(uint32_t threads, uint32_t smem, uint32_t cluster, bool after_previous,
+         cudaStream_t stream) {
+    config.blockDim = dim3(threads);
+    config.gridDim = dim3(cluster);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim.x = cluster;
+    attribute[0].val.clusterDim.y = 1;
+    attribute[0].val.clusterDim.z = 1;
+    attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attribute;
+    config.numAttrs = after_previous ? 2 : 1;
+  }
+};
+
+// Clusters of every size that the current device runs at once (SMs of a cluster share a
+// processing cluster of the GPU): a property of the device and the kernel, asked for once, for
+// one CTA per SM. Two CTAs of half the shared memory fit where one does; the runtime's count
+// does not take that into account, so a cluster of them counts as one of half its size.
+template <DecodeKernel kernel>
+cudaError_t places_of(int device, uint32_t threads, uint32_t smem, uint32_t (&at_once)[9]) {
+  static std::atomic<uint32_t> known[64][9];   // 0: not asked yet
+  if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
+  uint32_t one[9] = {};
+  for (uint32_t size = 1; size <= 8; ++size) {
+    one[size] = known[device][size].load(std::memory_order_acquire);
+    if (one[size] != 0) continue;
+    cudaError_t rc =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOnePerSm);
+    if (rc != cudaSuccess) return rc;
+    const Launch launch(threads, kOnePerSm, size, false, nullptr);
+    int clusters = 0;
+    rc = cudaOccupancyMaxActiveClusters(&clusters, kernel, &launch.config);
+    if (rc != cudaSuccess) return rc;
+    one[size] = clusters > 0 ? static_cast<uint32_t>(clusters) : 1u;
+    known[device][size].store(one[size], std::memory_order_release);
+  }
+  at_once[1] = smem == kTwoPerSm ? 2 * one[1] : one[1];
+  for (uint32_t size = 2; size <= 8; ++size) {
+    at_once[size] = smem == kTwoPerSm ? one[(size + 1) / 2] : one[size];
+  }
+  return cudaSuccess;
+}
+
+// Cluster size (up to 8, the portable limit) that finishes first: rounds of tiles per
+// cluster times the blocks of a tile per CTA; a CTA keeps two blocks of a tile at least.
+uint32_t cluster_size(const uint32_t (&at_once)[9], uint64_t tiles, uint64_t blocks) {
+  uint32_t best = 1;
+  double least = 0.0;
+  for (uint32_t size = 1; size <= 8 && (size == 1 || 2ull * size <= blocks); ++size) {
+    const uint64_t rounds = (tiles + at_once[size] - 1) / at_once[size];
+    const double time = static_cast<double>(rounds) * static_cast<double>(blocks) / size;
+    if (size == 1 || time < 0.97 * least) {   // a larger cluster has to be worth its join
+      best = size;
+      least = time;
+    }
+  }
+  return best;
+}
+
+template <DecodeKernel kernel>
+cudaError_t run_kernel(Launch& launch, uint64_t clusters, uint32_t gridy, uint32_t ring_bytes,
+                       const DecodeParams& params) {
+  const uint32_t size = launch.attribute[0].val.clusterDim.x;
+  launch.config.gridDim = dim3(static_cast<uint32_t>(clusters * size), gridy);
+  const cudaError_t rc = cudaLaunchKernelEx(&launch.config, kernel, params, ring_bytes);
   return rc != cudaSuccess ? rc : cudaPeekAtLastError();
 }
 
 template <bool INT8, uint32_t COLS>
 cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cudaStream_t stream) {
   constexpr uint32_t kPieces = Block<INT8>::kPieces, kBlockK = Block<INT8>::kK;
+  constexpr DecodeKernel kUp = decode_up_kernel<INT8, COLS>;
+  constexpr DecodeKernel kDown = decode_down_kernel<INT8, COLS>;
   const DecodeArgs& a = up.a;
-  const uint32_t sms = device_sm_count();
   const uint32_t assignments = a.tokens * a.top_k;
   const uint32_t slots = a.by_expert != 0 ? a.experts : assignments;
-  // Two CTAs per SM: one streams while the other starts or ends.
-  const uint32_t tiles = (a.inter + 63) / 64;
-  uint32_t split = split_of(static_cast<uint64_t>(tiles) * slots,
-                            (a.hidden + kBlockK - 1) / kBlockK, 4 * sms, 8);
-  cudaError_t rc =
-      launch_cluster<decode_up_kernel<INT8, COLS>>(dim3(tiles * split, slots), kUpThreads<INT8>,
-                                                   kTwoPerSm - 1024, 0, split, false, up, stream);
+  int device = 0;
+  cudaError_t rc = cudaGetDevice(&device);
   if (rc != cudaSuccess) return rc;
-  // The sums of many tokens leave less for the ring: two CTAs per SM if three stages fit at
-  // twice the average number of an expert's tokens, else one, in clusters of 4 (of 8 with an
-  // SM each, fewer fit at once).
-  const uint32_t groups = (a.hidden + kRows - 1) / kRows;
+  uint32_t at_once[9];
+  rc = places_of<kUp>(device, kUpThreads<INT8>, kTwoPerSm, at_once);
+  if (rc != cudaSuccess) return rc;
+
+  // First kernel: a cluster per tile, two CTAs per SM (one streams while the other starts or
+  // ends), more clusters than places. Few tiles are split along k, up to 8 ways (the portable
+  // cluster size), as long as every CTA keeps two k-blocks.
+  const uint64_t tiles = (a.inter + 63) / 64;
+  const uint64_t blocks = (a.hidden + kBlockK - 1) / kBlockK;
+  uint32_t split = 1;
+  while (split < 8 && tiles * slots * split <= at_once[1] && 4 * split <= blocks) split *= 2;
+  Launch first(kUpThreads<INT8>, kTwoPerSm, split, false, stream);
+  rc = run_kernel<kUp>(first, tiles, slots, kTwoPerSm - 1024, up);
+  if (rc != cudaSuccess) return rc;
+
+  // Second kernel: a cluster per 128 channels, all at once. The sums of many tokens leave less
+  // for the ring: two CTAs per SM if three stages fit at twice the average number of an
+  // expert's tokens, else one.
   const uint32_t reserved = (a.tokens * kRows * 4 + a.experts * kListBytes + 15) / 16 * 16;
   const uint32_t twice = 2 * assignments / a.experts + kGroup;
   const uint32_t columns = (twice < a.tokens ? twice : a.tokens) / kGroup * 2 * kGroup;
-  const bool two = kTwoPerSm - 1024 >= reserved + 3 * (kABytes + kPieces * columns * 128);
-  split = split_of(groups, static_cast<uint64_t>((a.inter + kBlockK - 1) / kBlockK) * slots,
-                   two ? 2 * sms : sms, two ? 8 : 4);
-  return launch_cluster<decode_down_kernel<INT8, COLS>>(
-      dim3(groups * split), kDownThreads<INT8>, (two ? kTwoPerSm : kOnePerSm) - 1024 - reserved,
-      reserved, split, true, down, stream);
+  const bool two = kDownTmem<INT8, COLS> <= 256 &&
+                   kTwoPerSm - 1024 >= reserved + 3 * (kABytes + kPieces * columns * 128);
+  const uint32_t smem = two ? kTwoPerSm : kOnePerSm;
+  rc = places_of<kDown>(device, kDownThreads<INT8>, smem, at_once);
+  if (rc != cudaSuccess) return rc;
+  const uint64_t groups = (a.hidden + kRows - 1) / kRows;
+  const uint32_t size = cluster_size(
+      at_once, groups, static_cast<uint64_t>((a.inter + kBlockK - 1) / kBlockK) * slots);
+  Launch second(kDownThreads<INT8>, smem, size, true, stream);
+  return run_kernel<kDown>(second, groups, 1, smem - 1024 - reserved, down);
 }
 
 template <bool INT8>

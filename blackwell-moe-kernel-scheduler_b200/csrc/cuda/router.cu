@@ -4,7 +4,7 @@
 // its input (agent/search_space.yaml:10-13).
 //
 //   softmax:  key = logit                    score = exp(logit - max) / sum
-//   sigmoid:  key = sigmoid(logit) + bias    score = sigmoid(logit)
+//   sigmoid:  key = sigmoid(logit) + bias    score = sigmoid(logit)   (key = logit if no bias)
 // The k largest keys are chosen, largest first, the lower id first among equals.
 //
 // One warp per token. Keys live in registers as unsigned integers whose order is the
@@ -50,6 +50,17 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
   return (bits >> 63) != 0 ? ~bits : bits | 0x8000000000000000ull;
 }
 
+// The float of a 32-bit key.
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) != 0 ? key & 0x7fffffffu : ~key);
+}
+
+// Distance below which sums sigmoid + bias computed in 32 bits may be in another order than
+// their exact values: the sigmoid is off by at most 2^-22 (exponential one step, sum and
+// quotient half a step each), the sum by half a step of itself, both keys count: 2^-21 + 2^-23
+// for sums up to 1, doubled.
+constexpr float kCloseSums = 0x1p-20f;
+
 __device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(kFull, v); }
 
 __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
@@ -67,9 +78,20 @@ __device__ __forceinline__ float load_logit(const uint16_t* p) {
 // expert i * 32 + lane). Lane j returns the id of the j-th choice (or -1). Up to 8 keys are
 // sorted first (odd-even transposition, equal keys stay in the order of their ids), so that
 // a round only looks at the front one: two warp operations and one shift.
-template <typename Key, uint32_t V>
-__device__ __forceinline__ int choose(Key (&key)[V], uint32_t top_k, uint32_t lane) {
+// With CLOSE, *close tells whether two neighbours among the chosen, or the last one and the next
+// in line, are so close that 32-bit keys do not decide their order.
+template <bool CLOSE, typename Key, uint32_t V>
+__device__ __forceinline__ int choose(Key (&key)[V], uint32_t top_k, uint32_t lane,
+                                      bool* close) {
   int mine = -1;
+  float above = INFINITY;
+  auto check = [&](Key top) {
+    if constexpr (CLOSE) {
+      const float v = top != 0 ? key_value(top) : -INFINITY;
+      if (above - v <= kCloseSums * fmaxf(1.0f, fabsf(v))) *close = true;
+      above = v;
+    }
+  };
   if constexpr (V <= 8) {
     uint32_t id[V];
 #pragma unroll
@@ -88,9 +110,11 @@ __device__ __forceinline__ int choose(Key (&key)[V], uint32_t top_k, uint32_t la
         }
       }
     }
-    for (uint32_t j = 0; j < top_k; ++j) {
+    for (uint32_t j = 0; j < top_k + (CLOSE ? 1 : 0); ++j) {
       const Key top = warp_max(key[0]);
       if (top == 0) break;   // nothing left that can be chosen
+      check(top);
+      if (CLOSE && j == top_k) break;
       const uint32_t chosen = __reduce_min_sync(kFull, key[0] == top ? id[0] : kFull);
       if (lane == j) mine = static_cast<int>(chosen);
       if (id[0] == chosen) {
@@ -104,7 +128,7 @@ __device__ __forceinline__ int choose(Key (&key)[V], uint32_t top_k, uint32_t la
     }
     return mine;
   }
-  for (uint32_t j = 0; j < top_k; ++j) {
+  for (uint32_t j = 0; j < top_k + (CLOSE ? 1 : 0); ++j) {
     Key best = 0;
     uint32_t at = 0;
 #pragma unroll
@@ -116,6 +140,8 @@ __device__ __forceinline__ int choose(Key (&key)[V], uint32_t top_k, uint32_t la
     }
     const Key top = warp_max(best);
     if (top == 0) break;   // nothing left that can be chosen
+    check(top);
+    if (CLOSE && j == top_k) break;
     const uint32_t id = __reduce_min_sync(kFull, best == top ? at * 32 + lane : kFull);
     if (lane == j) mine = static_cast<int>(id);
 #pragma unroll
@@ -143,7 +169,24 @@ route_topk_kernel(RouteTopkArgs a, uint32_t renormalize) {
   }
 
   int id;
+  bool close = false;
   if constexpr (SIGMOID && BIAS) {
+    uint32_t key[V];
+#pragma unroll
+    for (uint32_t i = 0; i < V; ++i) {
+      const uint32_t e = i * 32 + lane;
+      const float b = e < a.experts ? a.bias[e] : 0.0f;
+      key[i] = logit[i] > -INFINITY ? order_key(1.0f / (1.0f + expf(-logit[i])) + b) : 0u;
+    }
+    id = choose<true>(key, a.top_k, lane, &close);
+  } else {
+    uint32_t key[V];
+#pragma unroll
+    for (uint32_t i = 0; i < V; ++i) key[i] = order_key(logit[i]);
+    id = choose<false>(key, a.top_k, lane, &close);
+  }
+  if (SIGMOID && BIAS && close) {
+    // (the whole warp) once in some thousand tokens: decided by the sums in 64 bits
     unsigned long long key[V];
 #pragma unroll
     for (uint32_t i = 0; i < V; ++i) {
@@ -152,12 +195,7 @@ route_topk_kernel(RouteTopkArgs a, uint32_t renormalize) {
       const double sum = 1.0 / (1.0 + exp(-static_cast<double>(logit[i]))) + b;
       key[i] = logit[i] > -INFINITY ? order_key(sum) : 0ull;
     }
-    id = choose<unsigned long long, V>(key, a.top_k, lane);
-  } else {
-    uint32_t key[V];
-#pragma unroll
-    for (uint32_t i = 0; i < V; ++i) key[i] = order_key(logit[i]);
-    id = choose<uint32_t, V>(key, a.top_k, lane);
+    id = choose<false>(key, a.top_k, lane, &close);
   }
 
   // The chosen logit, from the row again (it is in L1).
