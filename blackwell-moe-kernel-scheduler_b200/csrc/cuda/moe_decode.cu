@@ -37,6 +37,7 @@ constexpr uint32_t kMaxTokens = BMOE_MOE_DECODE_MAX_TOKENS;
 constexpr uint32_t kRows = 128;                  // weight rows of a tile
 constexpr uint32_t kABytes = kRows * 128;        // one k-block of weights: 128 bytes of a row
 constexpr uint32_t kGroup = 8;                   // tokens of one activation box
+constexpr uint32_t kMostQuads = 6;               // gathers of four tokens per piece
 constexpr uint32_t kTwoPerSm = 110u * 1024u;     // dynamic shared memory of a CTA that shares
 constexpr uint32_t kOnePerSm = 222u * 1024u;     // its SM, and of one that does not
 constexpr uint32_t kMaxStages = 12;
@@ -60,6 +61,7 @@ struct DecodeParams {
                             // w_down as {inter, hidden, experts}, box 128 B x 128
   CUtensorMap acts[kMaxTokens / kGroup];   // boxes of 8, 16, ... rows: x as {hidden, tokens},
                                            // h as {inter, rows, 2}, both halves in one box
+  CUtensorMap rows;         // x again, box of one row (gathered by four)
   DecodeArgs a;
 };
 
@@ -274,7 +276,9 @@ constexpr uint32_t kUpTmem = INT8 ? 256 : (COLS < 32 ? 32 : COLS);
 // A cluster computes 64 channels of one expert for all of its tokens: the tile's rows 0-63
 // are the channels' gate rows, 64-127 their up rows. The activations of a k-block are one box per
 // piece (every load takes the producer some 60 cycles to issue): the groups of 8 tokens from
-// the expert's first to its last.
+// the expert's first to its last. Where its tokens are few and far between that would
+// be more bytes than the weights, and an SM takes in some 30 bytes a cycle: then only the
+// tokens themselves are gathered, four per load, if that is half the rows or less.
 template <bool INT8, uint32_t COLS>
 __global__ void __launch_bounds__(kUpThreads<INT8>, 2)
 decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
@@ -358,7 +362,10 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
   const uint32_t d_tmem = tmem + (INT8 ? kTmemA : 0);
   const uint32_t token0 = list_token[0] / kGroup * kGroup;
   const uint32_t boxes = list_token[count - 1] / kGroup - token0 / kGroup + 1;
-  const uint32_t n = (boxes + 1) / 2 * 16;         // columns of the MMA: a multiple of 16
+  const uint32_t quads = (count + 3) / 4;
+  const bool gather = COLS > 16 && quads <= boxes && quads <= kMostQuads;
+  const uint32_t columns = gather ? 4 * quads : kGroup * boxes;
+  const uint32_t n = (columns + 15) / 16 * 16;     // columns of the MMA
   const Ring<INT8> ring(base, ring_bytes, n);
 
   const uint32_t rank = ptx::cluster_cta_rank(), ranks = ptx::cluster_cta_count();
@@ -368,7 +375,18 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
 
   if (warp == 0) {
     Cursor stage;
-    const uint32_t bytes = kABytes + boxes * kPieces * kGroup * 128;
+    const uint32_t bytes = kABytes + columns * kPieces * 128;
+    // token indices of the gathers, a byte each; the rows behind the last are outside x
+    uint32_t quad_tokens[kMostQuads];
+#pragma unroll
+    for (uint32_t q = 0; q < kMostQuads; ++q) {
+      quad_tokens[q] = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t t = 4 * q + i < count ? list_token[4 * q + i] : kMaxTokens;
+        quad_tokens[q] |= t << (8 * i);
+      }
+    }
     for (uint32_t b = begin; b < end; ++b) {
       if (!wait(bars.empty[stage.slot], stage.parity ^ 1u)) {
         if (lane == 0) report(a, 1);
@@ -383,8 +401,20 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
                          static_cast<int32_t>(2 * expert));
 #pragma unroll
         for (uint32_t piece = 0; piece < kPieces; ++piece) {
-          ptx::tma_load_2d(at + kABytes + piece * ring.piece_bytes, &p.acts[boxes - 1], bar,
-                           k + static_cast<int32_t>(64 * piece), static_cast<int32_t>(token0));
+          const uint32_t to = at + kABytes + piece * ring.piece_bytes;
+          const int32_t k_piece = k + static_cast<int32_t>(64 * piece);
+          if (!gather) {
+            ptx::tma_load_2d(to, &p.acts[boxes - 1], bar, k_piece, static_cast<int32_t>(token0));
+          } else if constexpr (COLS > 16) {
+#pragma unroll
+            for (uint32_t q = 0; q < kMostQuads; ++q) {
+              const uint32_t t = quad_tokens[q];
+              if (q < quads) {
+                ptx::tma_gather4(to + q * 512, &p.rows, bar, k_piece, t & 0xff, (t >> 8) & 0xff,
+                                 (t >> 16) & 0xff, t >> 24);
+              }
+            }
+          }
         }
       }
       __syncwarp();
@@ -458,7 +488,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
     const uint32_t c = i % 64, at = i / 64;
     const uint32_t channel = channel0 + c;
     if (channel >= a.inter) continue;
-    const uint32_t cell = base + ((list_token[at] - token0) * kRows + c) * 4;
+    const uint32_t cell = base + ((gather ? at : list_token[at] - token0) * kRows + c) * 4;
     float gate = sum_over_cluster(cell, ranks), up = sum_over_cluster(cell + 64 * 4, ranks);
     if constexpr (INT8) {
       gate *= channel_scale[0][c];
@@ -908,6 +938,8 @@ bool encode_maps(DecodeParams& up, DecodeParams& down, const bmoe_moe_decode_arg
   }
   const uint64_t x_dims[2] = {hidden, a.tokens}, x_strides[1] = {hidden * 2};
   const uint64_t h_dims[3] = {inter, rows, 2}, h_strides[2] = {inter * 2, rows * inter * 2};
+  const uint32_t row_box[2] = {64, 1};
+  if (!encode_box(&up.rows, a.x_dev, Elem::kBf16, 2, x_dims, x_strides, row_box)) return false;
   for (uint32_t g = 0; g * kGroup < a.tokens; ++g) {
     const uint32_t box[3] = {64, (g + 1) * kGroup, 2};
     if (!encode_box(&up.acts[g], a.x_dev, Elem::kBf16, 2, x_dims, x_strides, box) ||

@@ -206,6 +206,18 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst_smem, const void* tmap,
       : "memory");
 }
 
+// Four rows of a 2-D tensor by index (the map's box is one row high), one behind the other in
+// shared memory; rows outside the tensor are filled with zeros.
+__device__ __forceinline__ void tma_gather4(uint32_t dst_smem, const void* tmap, uint32_t bar,
+                                            int32_t c0, int32_t r0, int32_t r1, int32_t r2,
+                                            int32_t r3) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst_smem),
+      "l"(tmap), "r"(bar), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+      : "memory");
+}
+
 // 2-D tiled store shared -> global (bulk async group); rows / columns outside
 // the tensor extent are clipped by the hardware.
 __device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src_smem,
