@@ -797,6 +797,18 @@ struct Launch {
   }
 };
 
+// The opt-in shared-memory size is an attribute of a kernel on a device; set once.
+template <DecodeKernel kernel>
+cudaError_t opt_in(int device) {
+  static std::atomic<bool> done[64];
+  if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
+  if (done[device].load(std::memory_order_acquire)) return cudaSuccess;
+  const cudaError_t rc =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOnePerSm);
+  if (rc == cudaSuccess) done[device].store(true, std::memory_order_release);
+  return rc;
+}
+
 // Clusters of every size that the current device runs at once (SMs of a cluster share a
 // processing cluster of the GPU): a property of the device and the kernel, asked for once, for
 // one CTA per SM. Two CTAs of half the shared memory fit where one does; the runtime's count
@@ -809,8 +821,7 @@ cudaError_t places_of(int device, uint32_t threads, uint32_t smem, uint32_t (&at
   for (uint32_t size = 1; size <= 8; ++size) {
     one[size] = known[device][size].load(std::memory_order_acquire);
     if (one[size] != 0) continue;
-    cudaError_t rc =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOnePerSm);
+    cudaError_t rc = opt_in<kernel>(device);
     if (rc != cudaSuccess) return rc;
     const Launch launch(threads, kOnePerSm, size, false, nullptr);
     int clusters = 0;
@@ -862,17 +873,20 @@ cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cuda
   int device = 0;
   cudaError_t rc = cudaGetDevice(&device);
   if (rc != cudaSuccess) return rc;
-  uint32_t at_once[9];
-  rc = places_of<kUp>(device, kUpThreads<INT8>, kTwoPerSm, at_once);
-  if (rc != cudaSuccess) return rc;
 
   // First kernel: a cluster per tile, two CTAs per SM (one streams while the other starts or
-  // ends), more clusters than places. Few tiles are split along k, up to 8 ways (the portable
-  // cluster size), as long as every CTA keeps two k-blocks.
+  // ends). Tiles that leave SMs idle are split along k, up to 8 ways (the portable cluster
+  // size), as long as every CTA keeps two k-blocks. Splitting further, so that both places of
+  // every SM are taken, costs more in starts and joins than it spreads (96 tiles, T=1:
+  // 23.6 us in one piece, 24.1 in two, 26.1 in four).
   const uint64_t tiles = (a.inter + 63) / 64;
   const uint64_t blocks = (a.hidden + kBlockK - 1) / kBlockK;
   uint32_t split = 1;
-  while (split < 8 && tiles * slots * split <= at_once[1] && 4 * split <= blocks) split *= 2;
+  while (split < 8 && tiles * slots * split * 2 <= device_sm_count() && 4 * split <= blocks) {
+    split *= 2;
+  }
+  rc = opt_in<kUp>(device);
+  if (rc != cudaSuccess) return rc;
   Launch first(kUpThreads<INT8>, kTwoPerSm, split, false, stream);
   rc = run_kernel<kUp>(first, tiles, slots, kTwoPerSm - 1024, up);
   if (rc != cudaSuccess) return rc;
@@ -886,6 +900,7 @@ cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cuda
   const bool two = kDownTmem<INT8, COLS> <= 256 &&
                    kTwoPerSm - 1024 >= reserved + 3 * (kABytes + kPieces * columns * 128);
   const uint32_t smem = two ? kTwoPerSm : kOnePerSm;
+  uint32_t at_once[9];
   rc = places_of<kDown>(device, kDownThreads<INT8>, smem, at_once);
   if (rc != cudaSuccess) return rc;
   const uint64_t groups = (a.hidden + kRows - 1) / kRows;
