@@ -274,10 +274,11 @@ class WorklistRequest(C.Structure):
 
 class GemmArgs(C.Structure):
     _fields_ = [
-        ("a", C.POINTER(C.c_void_p)),
-        ("b", C.POINTER(C.c_void_p)),
-        ("d", C.POINTER(C.c_void_p)),
-        ("tokens_per_expert", C.POINTER(C.c_uint32)),
+        # host arrays, by address (a cast to a pointer type costs microseconds per re-plan)
+        ("a", C.c_void_p),
+        ("b", C.c_void_p),
+        ("d", C.c_void_p),
+        ("tokens_per_expert", C.c_void_p),
         ("experts", C.c_uint32),
         ("n", C.c_uint32),
         ("k", C.c_uint32),
@@ -296,8 +297,8 @@ class GemmArgs(C.Structure):
         ("results_pushed", C.c_uint32),
         ("reserved0", C.c_uint32),
         ("tokens_per_expert_dev", C.c_void_p),
-        ("row_scale", C.POINTER(C.c_void_p)),
-        ("col_scale", C.POINTER(C.c_void_p)),
+        ("row_scale", C.c_void_p),
+        ("col_scale", C.c_void_p),
         ("packed_row_scale", C.c_void_p),
     ]
 

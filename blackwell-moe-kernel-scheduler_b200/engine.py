@@ -44,15 +44,14 @@ def tiles_to_numpy(tiles, count: int) -> np.ndarray:
     return raw.copy()
 
 
-def _byte_type(a, w) -> int:
-    """Operand type of one-byte tensors: INT8 when both are ``torch.int8``, FP8 E4M3 bytes
-    (``torch.float8_e4m3fn`` or ``uint8``) when neither is; -1 for a mixture."""
+def _byte_type(a, w, scaled: bool) -> int:
+    """Operand type of one-byte tensors: with scales INT8 (both ``torch.int8``, else -1), without
+    FP8 E4M3 bytes."""
     import torch
 
-    signed = (a.dtype is torch.int8, w.dtype is torch.int8)
-    if signed == (True, True):
-        return _capi.TYPE_INT8
-    return _capi.TYPE_FP8_E4M3 if signed == (False, False) else -1
+    if not scaled:
+        return _capi.TYPE_FP8_E4M3
+    return _capi.TYPE_INT8 if a.dtype is w.dtype is torch.int8 else -1
 
 
 def _scales_fit(data_type, a, w, row_scale, col_scale) -> bool:
@@ -141,23 +140,17 @@ class GroupedGemmPlan:
                 arr = np.array([int(p or 0) for p in values], dtype=np.uint64)
             return arr if arr.size else np.zeros(1, dtype=np.uint64)
 
-        def pointer_table(values):
-            if values is None:
-                return None, None
-            arr = pointers(values)
-            return arr, arr.ctypes.data_as(C.POINTER(C.c_void_p))
-
         arr_a, arr_b, arr_d = pointers(a_ptrs), pointers(b_ptrs), pointers(d_ptrs)
-        keep_row, row_scale = pointer_table(row_scale_ptrs)
-        keep_col, col_scale = pointer_table(col_scale_ptrs)
+        arr_row = None if row_scale_ptrs is None else pointers(row_scale_ptrs)
+        arr_col = None if col_scale_ptrs is None else pointers(col_scale_ptrs)
         counts = np.ascontiguousarray(tokens_per_expert, dtype=np.uint32)
         if counts.size == 0:
             counts = np.zeros(1, dtype=np.uint32)
         args = _capi.GemmArgs(
-            a=arr_a.ctypes.data_as(C.POINTER(C.c_void_p)),
-            b=arr_b.ctypes.data_as(C.POINTER(C.c_void_p)),
-            d=arr_d.ctypes.data_as(C.POINTER(C.c_void_p)),
-            tokens_per_expert=counts.ctypes.data_as(C.POINTER(C.c_uint32)),
+            a=arr_a.ctypes.data,
+            b=arr_b.ctypes.data,
+            d=arr_d.ctypes.data,
+            tokens_per_expert=counts.ctypes.data,
             experts=experts,
             n=n,
             k=k,
@@ -176,8 +169,8 @@ class GroupedGemmPlan:
             results_pushed=1 if results_pushed else 0,
             reserved0=0,
             tokens_per_expert_dev=int(tokens_per_expert_dev) or None,
-            row_scale=row_scale,
-            col_scale=col_scale,
+            row_scale=None if arr_row is None else arr_row.ctypes.data,
+            col_scale=None if arr_col is None else arr_col.ctypes.data,
             packed_row_scale=int(packed_row_scale) or None,
         )
         return int(self._lib.bmoe_plan_initialize(self._handle, C.byref(args)))
@@ -213,7 +206,7 @@ class GroupedGemmPlan:
         if elem != int(w.element_size()) or elem not in (1, 2):
             return _capi.INVALID_ARGUMENT
         if elem == 1:
-            options["data_type"] = _byte_type(a, w)
+            options["data_type"] = _byte_type(a, w, row_scale is not None or col_scale is not None)
         if not _scales_fit(options.get("data_type"), a, w, row_scale, col_scale):
             return _capi.INVALID_ARGUMENT
         if row_scale is not None:
@@ -247,7 +240,7 @@ class GroupedGemmPlan:
         if elem != int(w.element_size()) or elem not in (1, 2):
             return _capi.INVALID_ARGUMENT
         if elem == 1:
-            options["data_type"] = _byte_type(a, w)
+            options["data_type"] = _byte_type(a, w, row_scale is not None or col_scale is not None)
         if not _scales_fit(options.get("data_type"), a, w, row_scale, col_scale):
             return _capi.INVALID_ARGUMENT
         if row_scale is not None:

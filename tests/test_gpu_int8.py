@@ -193,7 +193,8 @@ def test_int8_needs_scales_and_matching_types(engine):
     plan = engine.GroupedGemmPlan()
     bad = engine._capi.INVALID_ARGUMENT
     try:
-        assert plan.initialize_packed(a, w, d, [4]) == bad
+        assert plan.initialize_packed(a, w, d, [4], row_scale=row) == bad
+        assert plan.initialize_packed(a, w, d, [4], col_scale=col) == bad
         assert plan.initialize_packed(a, w, d, [4], row_scale=row, col_scale=col[:, :8]) == bad
         assert plan.initialize_packed(a, w, d, [4], row_scale=row[:2], col_scale=col) == bad
         assert plan.initialize_packed(a, w, d, [4], row_scale=row.double(), col_scale=col) == bad
@@ -201,6 +202,8 @@ def test_int8_needs_scales_and_matching_types(engine):
                                       col_scale=col) == bad
         assert plan.initialize_packed(a.view(torch.uint8), w.view(torch.uint8), d, [4],
                                       row_scale=row, col_scale=col) == bad
+        # bytes without scales are FP8 bit patterns, whatever the tensors' type is called
+        assert plan.initialize_packed(a, w, d, [4]) == 0
     finally:
         plan.close()
 
