@@ -953,8 +953,8 @@ bool encode_maps(DecodeParams& up, DecodeParams& down, const bmoe_moe_decode_arg
   }
   const uint64_t x_dims[2] = {hidden, a.tokens}, x_strides[1] = {hidden * 2};
   const uint64_t h_dims[3] = {inter, rows, 2}, h_strides[2] = {inter * 2, rows * inter * 2};
-  const uint32_t row_box[2] = {64, 1};
-  if (!encode_box(&up.rows, a.x_dev, Elem::kBf16, 2, x_dims, x_strides, row_box)) return false;
+  const uint32_t row_box[2] = {64, 1};   // gathered rows: more than 16 tokens only
+  if (a.tokens > 16 && !encode_box(&up.rows, a.x_dev, Elem::kBf16, 2, x_dims, x_strides, row_box)) return false;
   for (uint32_t g = 0; g * kGroup < a.tokens; ++g) {
     const uint32_t box[3] = {64, (g + 1) * kGroup, 2};
     if (!encode_box(&up.acts[g], a.x_dev, Elem::kBf16, 2, x_dims, x_strides, box) ||
@@ -964,8 +964,6 @@ bool encode_maps(DecodeParams& up, DecodeParams& down, const bmoe_moe_decode_arg
   }
   return true;
 }
-
-bool unaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
 }  // namespace
 
@@ -998,9 +996,12 @@ extern "C" int bmoe_moe_decode(const bmoe_moe_decode_args* args) {
   if (a.tokens == 0) return BMOE_OK;
   if (a.x_dev == nullptr || a.w_gate_up_dev == nullptr || a.w_down_dev == nullptr ||
       a.expert_ids_dev == nullptr || a.weights_dev == nullptr || a.out_dev == nullptr ||
-      a.workspace_dev == nullptr || bmoe::unaligned(a.x_dev) || bmoe::unaligned(a.w_gate_up_dev) ||
-      bmoe::unaligned(a.w_down_dev) || bmoe::unaligned(a.out_dev) ||
-      (reinterpret_cast<uintptr_t>(a.workspace_dev) & 255u) != 0 ||
+      a.workspace_dev == nullptr || bmoe::off_grid(a.x_dev, 16) ||
+      bmoe::off_grid(a.w_gate_up_dev, 16) || bmoe::off_grid(a.w_down_dev, 16) ||
+      bmoe::off_grid(a.out_dev, 16) || bmoe::off_grid(a.workspace_dev, 256) ||
+      bmoe::off_grid(a.expert_ids_dev, 8) || bmoe::off_grid(a.weights_dev, 4) ||
+      bmoe::off_grid(a.gate_up_scale_dev, 4) || bmoe::off_grid(a.down_scale_dev, 4) ||
+      bmoe::off_grid(a.status_dev, 4) ||
       a.workspace_bytes < bmoe_moe_decode_workspace(a.tokens, a.top_k, a.inter) ||
       (int8 && (a.gate_up_scale_dev == nullptr || a.down_scale_dev == nullptr))) {
     return BMOE_INVALID_ARGUMENT;

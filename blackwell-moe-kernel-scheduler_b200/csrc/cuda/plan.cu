@@ -247,7 +247,8 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
   if (bytes && a.k % 16 != 0) return BMOE_INVALID_ARGUMENT;
   // INT8: a scale per row and per channel, sums that cannot pass 2^31
   if (int8 && (a.k > BMOE_INT8_MAX_K || a.col_scale == nullptr ||
-               (packed ? a.packed_row_scale == nullptr : a.row_scale == nullptr))) {
+               (packed ? a.packed_row_scale == nullptr || bmoe::off_grid(a.packed_row_scale, 4)
+                       : a.row_scale == nullptr))) {
     return BMOE_INVALID_ARGUMENT;
   }
   const Elem operand = bytes ? Elem::kByte : Elem::kBf16;
@@ -287,7 +288,7 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
       return BMOE_INVALID_ARGUMENT;
     }
     if (int8 && (a.col_scale[e] == nullptr || misaligned16(a.col_scale[e]) ||
-                 (!packed && a.row_scale[e] == nullptr))) {
+                 (!packed && (a.row_scale[e] == nullptr || bmoe::off_grid(a.row_scale[e], 4))))) {
       return BMOE_INVALID_ARGUMENT;
     }
     routed_rows += host_counts[e];

@@ -29,6 +29,11 @@ inline uint32_t device_sm_count() {
   return static_cast<uint32_t>(sms);
 }
 
+// A pointer that is not on a multiple of `bytes` (a power of two); null is on every grid.
+inline bool off_grid(const void* p, uintptr_t bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0;
+}
+
 template <typename Kernel>
 cudaError_t preload_one(Kernel kernel) {
   cudaFuncAttributes attributes;

@@ -212,8 +212,8 @@ extern "C" int bmoe_quantize_rows(const bmoe_quantize_rows_args* args) {
   }
   if (a.rows == 0) return BMOE_OK;
   if (a.src_dev == nullptr || a.dst_dev == nullptr || a.scale_dev == nullptr ||
-      (reinterpret_cast<uintptr_t>(a.src_dev) & 15u) != 0 ||
-      (reinterpret_cast<uintptr_t>(a.dst_dev) & 15u) != 0 ||
+      bmoe::off_grid(a.src_dev, 16) || bmoe::off_grid(a.dst_dev, 16) ||
+      bmoe::off_grid(a.index_dev, 8) || bmoe::off_grid(a.scale_dev, 4) ||
       (a.index_dev == nullptr && a.rows > a.src_rows)) {
     return BMOE_INVALID_ARGUMENT;
   }

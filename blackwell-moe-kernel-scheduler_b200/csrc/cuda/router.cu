@@ -152,7 +152,7 @@ __device__ __forceinline__ int choose(Key (&key)[V], uint32_t top_k, uint32_t la
   return mine;
 }
 
-// V keys per lane; SIGMOID with BIAS chooses by the sum in 64 bits.
+// V keys per lane; SIGMOID with BIAS chooses by the sum, in 64 bits where 32 do not decide.
 template <typename T, uint32_t V, bool SIGMOID, bool BIAS>
 __global__ void __launch_bounds__(kRouteTopkThreads)
 route_topk_kernel(RouteTopkArgs a, uint32_t renormalize) {
@@ -308,7 +308,8 @@ extern "C" int bmoe_route_topk(const bmoe_route_topk_args* args) {
   }
   if (a.tokens == 0) return BMOE_OK;
   if (a.logits_dev == nullptr || a.expert_ids_dev == nullptr || a.weights_dev == nullptr ||
-      reinterpret_cast<uintptr_t>(a.logits_dev) % elem != 0) {
+      bmoe::off_grid(a.logits_dev, elem) || bmoe::off_grid(a.expert_ids_dev, 8) ||
+      bmoe::off_grid(a.weights_dev, 4) || bmoe::off_grid(a.bias_dev, 4)) {
     return BMOE_INVALID_ARGUMENT;
   }
   bmoe::RouteTopkArgs k;

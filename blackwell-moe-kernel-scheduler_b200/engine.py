@@ -44,6 +44,10 @@ def tiles_to_numpy(tiles, count: int) -> np.ndarray:
     return raw.copy()
 
 
+def _address(arr: np.ndarray) -> int:
+    return arr.__array_interface__["data"][0]
+
+
 def _byte_type(a, w, scaled: bool) -> int:
     """Operand type of one-byte tensors: with scales INT8 (both ``torch.int8``, else -1), without
     FP8 E4M3 bytes."""
@@ -72,8 +76,7 @@ def _scales_fit(data_type, a, w, row_scale, col_scale) -> bool:
 def _expert_pointers(per_expert) -> np.ndarray:
     """Address of every expert's slice of a contiguous FP32 tensor [experts, n]."""
     experts, n = int(per_expert.shape[0]), int(per_expert.shape[1])
-    return (np.uint64(per_expert.data_ptr()) +
-            np.arange(experts, dtype=np.uint64) * np.uint64(n * 4))
+    return per_expert.data_ptr() + np.arange(experts, dtype=np.uint64) * (n * 4)
 
 
 class GroupedGemmPlan:
@@ -134,11 +137,11 @@ class GroupedGemmPlan:
         experts = len(tokens_per_expert)
 
         def pointers(values):
-            if isinstance(values, np.ndarray):
-                arr = np.ascontiguousarray(values, dtype=np.uint64)
-            else:
-                arr = np.array([int(p or 0) for p in values], dtype=np.uint64)
-            return arr if arr.size else np.zeros(1, dtype=np.uint64)
+            if not isinstance(values, np.ndarray):
+                values = np.array([int(p or 0) for p in values], dtype=np.uint64)
+            elif values.dtype != np.uint64 or not values.flags.c_contiguous:
+                values = np.ascontiguousarray(values, dtype=np.uint64)
+            return values if values.size else np.zeros(1, dtype=np.uint64)
 
         arr_a, arr_b, arr_d = pointers(a_ptrs), pointers(b_ptrs), pointers(d_ptrs)
         arr_row = None if row_scale_ptrs is None else pointers(row_scale_ptrs)
@@ -147,32 +150,13 @@ class GroupedGemmPlan:
         if counts.size == 0:
             counts = np.zeros(1, dtype=np.uint32)
         args = _capi.GemmArgs(
-            a=arr_a.ctypes.data,
-            b=arr_b.ctypes.data,
-            d=arr_d.ctypes.data,
-            tokens_per_expert=counts.ctypes.data,
-            experts=experts,
-            n=n,
-            k=k,
-            data_type=data_type,
-            scheduler=_scheduler_id(scheduler),
-            claim_size=claim_size,
-            hybrid_tail_tiles=hybrid_tail_tiles,
-            cta_count=min(int(cta_count), 0xFFFFFFFF),
-            tile_n=tile_n,
-            cta_group=cta_group,
-            raster_along_m=raster_along_m,
-            output_f32=1 if output_f32 else 0,
-            stream=_stream_ptr(stream),
-            packed_a=int(packed_a) or None,
-            packed_rows=int(packed_rows),
-            results_pushed=1 if results_pushed else 0,
-            reserved0=0,
-            tokens_per_expert_dev=int(tokens_per_expert_dev) or None,
-            row_scale=None if arr_row is None else arr_row.ctypes.data,
-            col_scale=None if arr_col is None else arr_col.ctypes.data,
-            packed_row_scale=int(packed_row_scale) or None,
-        )
+            _address(arr_a), _address(arr_b), _address(arr_d), _address(counts),
+            experts, n, k, data_type, _scheduler_id(scheduler), claim_size, hybrid_tail_tiles,
+            min(int(cta_count), 0xFFFFFFFF), tile_n, cta_group, raster_along_m,
+            1 if output_f32 else 0, _stream_ptr(stream), int(packed_a) or None, int(packed_rows),
+            1 if results_pushed else 0, 0, int(tokens_per_expert_dev) or None,
+            None if arr_row is None else _address(arr_row),
+            None if arr_col is None else _address(arr_col), int(packed_row_scale) or None)
         return int(self._lib.bmoe_plan_initialize(self._handle, C.byref(args)))
 
     def initialize_packed(self, a, w, d, tokens_per_expert: Sequence[int], *,
@@ -201,7 +185,7 @@ class GroupedGemmPlan:
         total = int(counts.sum())
         if int(a.shape[0]) < total or int(d.shape[0]) < total:
             return _capi.INVALID_ARGUMENT
-        first_row = (np.cumsum(counts) - counts).astype(np.uint64)
+        first_row = (counts.cumsum() - counts).view(np.uint64)
         elem = int(a.element_size())
         if elem != int(w.element_size()) or elem not in (1, 2):
             return _capi.INVALID_ARGUMENT
@@ -210,14 +194,13 @@ class GroupedGemmPlan:
         if not _scales_fit(options.get("data_type"), a, w, row_scale, col_scale):
             return _capi.INVALID_ARGUMENT
         if row_scale is not None:
-            options["row_scale_ptrs"] = np.uint64(row_scale.data_ptr()) + first_row * np.uint64(4)
+            options["row_scale_ptrs"] = row_scale.data_ptr() + first_row * 4
             options["col_scale_ptrs"] = _expert_pointers(col_scale)
             if single_a_map:
                 options["packed_row_scale"] = row_scale.data_ptr()
-        a_ptrs = np.uint64(a.data_ptr()) + first_row * np.uint64(k * elem)
-        b_ptrs = (np.uint64(w.data_ptr()) +
-                  np.arange(experts, dtype=np.uint64) * np.uint64(n * k * elem))
-        d_ptrs = np.uint64(d.data_ptr()) + first_row * np.uint64(n * d_elem)
+        a_ptrs = a.data_ptr() + first_row * (k * elem)
+        b_ptrs = w.data_ptr() + np.arange(experts, dtype=np.uint64) * (n * k * elem)
+        d_ptrs = d.data_ptr() + first_row * (n * d_elem)
         self._keep = (a, w, d, row_scale, col_scale)
         if single_a_map:
             options.update(packed_a=a.data_ptr(), packed_rows=int(a.shape[0]))

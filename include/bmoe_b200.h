@@ -942,7 +942,8 @@ uint64_t bmoe_moe_decode_workspace(uint32_t tokens, uint32_t top_k, uint32_t int
  * as the integers they are and scaled per output channel in FP32. An expert that a token
  * names twice counts with the sum of both weights. Dropped assignments contribute nothing;
  * a token with nothing else gets a row of zeros. Results do not depend on the run: no
- * atomics. All pointers 16-byte aligned. For more tokens there is the grouped GEMM plan. */
+ * atomics. x, the weights and out are 16-byte aligned, the rest as their types. out may be x.
+ * For more tokens there is the grouped GEMM plan. */
 int bmoe_moe_decode(const bmoe_moe_decode_args* args);
 
 /* Library build information ("sm_100a", CUDA runtime version, ...). */

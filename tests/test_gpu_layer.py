@@ -427,6 +427,81 @@ def test_moe_decode_workspace_streams_and_graphs(engine):
         assert torch.equal(captured, step())
 
 
+def test_moe_decode_may_write_its_input_and_leaves_the_status_word_alone(engine):
+    import ctypes as C
+
+    for int8 in (False, True):
+        layer = make_layer(40, 12, 3, 384, 320, int8, seed=8)
+        want = run_layer(engine, layer)
+        to = {k: (v.cuda() if v is not None else None) for k, v in layer.items()}
+        got = engine.moe_decode(to["x"], to["w1"], to["w2"], to["ids"], to["coef"],
+                                gate_up_scale=to["s1"], down_scale=to["s2"], out=to["x"])
+        assert got is to["x"] and torch.equal(got, want)
+    cap = engine._capi
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(want)
+    workspace = torch.empty(engine.moe_decode_workspace(40, 3, 320), dtype=torch.uint8,
+                            device="cuda")
+    to["x"].copy_(layer["x"])
+    args = cap.MoeDecodeArgs(
+        to["x"].data_ptr(), to["w1"].data_ptr(), to["w2"].data_ptr(), to["s1"].data_ptr(),
+        to["s2"].data_ptr(), to["ids"].data_ptr(), to["coef"].data_ptr(), out.data_ptr(),
+        workspace.data_ptr(), workspace.numel(), 40, 3, 12, 384, 320, cap.TYPE_INT8, None,
+        status.data_ptr())
+    assert cap.load().bmoe_moe_decode(C.byref(args)) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and status.item() == 0
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("tokens", [17, 33, 64])
+def test_moe_decode_sparse_and_spread_tokens(engine, tokens, int8):
+    """Experts whose few tokens lie far apart, close together, and at both ends."""
+    layer = make_layer(tokens, 9, 2, 192, 128, int8, seed=tokens)
+    ids = torch.full((tokens, 2), -1, dtype=torch.int64)
+    ids[0, 0] = ids[tokens - 1, 0] = 0                 # first and last
+    ids[tokens // 2, 1] = 1                            # one in the middle
+    ids[::5, 1] = 2
+    ids[1:5, 0] = 3
+    ids[tokens - 3:, 1] = 4
+    ids[::2, 0] = torch.where(ids[::2, 0] < 0, 5, ids[::2, 0])
+    ids[3::8, 1] = 6                                   # one of every group of 8
+    layer["ids"] = ids
+    check_layer(engine, layer)
+
+
+def test_operators_at_once_from_two_host_threads(engine):
+    import threading
+
+    layers = [make_layer(9 + i, 7, 2, 256, 192, bool(i), seed=50 + i) for i in range(2)]
+    wants = [run_layer(engine, layer) for layer in layers]
+    logits = torch.randn(300, 64, generator=gen(1)).cuda()
+    want_ids = engine.route_topk(logits, 4)[0]
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(i):
+        try:
+            to = {k: (v.cuda() if v is not None else None) for k, v in layers[i].items()}
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(30):
+                    got = engine.moe_decode(to["x"], to["w1"], to["w2"], to["ids"], to["coef"],
+                                            gate_up_scale=to["s1"], down_scale=to["s2"])
+                    ids = engine.route_topk(logits, 4)[0]
+                    stream.synchronize()
+                    assert torch.equal(got, wants[i]) and torch.equal(ids, want_ids)
+        except Exception as error:   # noqa: BLE001 - reported by the main thread
+            failures.append(error)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
+
+
 def test_moe_decode_weights_past_32_bit_offsets(engine):
     """The last expert's weights start beyond 2^32 bytes (and 2^31 elements)."""
     experts, hidden, inter = 70, 4096, 8192

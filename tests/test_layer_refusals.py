@@ -33,6 +33,9 @@ def route_args(cap, **change):
     (dict(logits_dev=P + 2), "INVALID_ARGUMENT"),
     (dict(expert_ids_dev=None), "INVALID_ARGUMENT"),
     (dict(weights_dev=None), "INVALID_ARGUMENT"),
+    (dict(expert_ids_dev=P + 4), "INVALID_ARGUMENT"),
+    (dict(weights_dev=P + 2), "INVALID_ARGUMENT"),
+    (dict(scoring=1, bias_dev=P + 2), "INVALID_ARGUMENT"),
     (dict(tokens=0, logits_dev=None), "OK"),
 ])
 def test_route_topk_checks(engine, change, want):
@@ -59,6 +62,8 @@ def quantize_args(cap, **change):
     (dict(src_dev=None), "INVALID_ARGUMENT"),
     (dict(dst_dev=None), "INVALID_ARGUMENT"),
     (dict(scale_dev=None), "INVALID_ARGUMENT"),
+    (dict(scale_dev=P + 2), "INVALID_ARGUMENT"),
+    (dict(index_dev=P + 4), "INVALID_ARGUMENT"),
     (dict(rows=1 << 31, src_rows=1 << 31), "INVALID_ARGUMENT"),
     (dict(rows=5), "INVALID_ARGUMENT"),                # no index: row i is source row i
     (dict(rows=0, src_dev=None), "OK"),
@@ -102,6 +107,10 @@ def decode_args(cap, **change):
     (dict(workspace_dev=None), "INVALID_ARGUMENT"),
     (dict(workspace_dev=P + 16), "INVALID_ARGUMENT"),
     (dict(workspace_bytes=0), "INVALID_ARGUMENT"),
+    (dict(expert_ids_dev=P + 4), "INVALID_ARGUMENT"),
+    (dict(weights_dev=P + 1), "INVALID_ARGUMENT"),
+    (dict(status_dev=P + 2), "INVALID_ARGUMENT"),
+    (dict(data_type=3, gate_up_scale_dev=P + 2, down_scale_dev=P), "INVALID_ARGUMENT"),
     (dict(data_type=3), "INVALID_ARGUMENT"),                       # INT8 without scales
     (dict(data_type=3, gate_up_scale_dev=P), "INVALID_ARGUMENT"),
     (dict(data_type=3, gate_up_scale_dev=P, down_scale_dev=P, hidden=72), "INVALID_ARGUMENT"),
@@ -143,6 +152,8 @@ def test_int8_plan_checks(engine):
         assert status(k=24, **scales) == cap.INVALID_ARGUMENT                # k % 16
         assert status(k=131072, **scales) == cap.INVALID_ARGUMENT            # sums pass 2^31
         assert status(packed_a=4096, packed_rows=12, **scales) == cap.INVALID_ARGUMENT
+        assert status(packed_a=4096, packed_rows=12, packed_row_scale=4098,
+                      col_scale_ptrs=scales["col_scale_ptrs"]) == cap.INVALID_ARGUMENT
         assert plan.run() == cap.INVALID_ARGUMENT
     finally:
         plan.close()
