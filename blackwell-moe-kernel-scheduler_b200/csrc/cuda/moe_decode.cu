@@ -115,16 +115,20 @@ __device__ __forceinline__ void report(const DecodeArgs& a, uint32_t site) {
   if (a.status != nullptr) atomicCAS(a.status, 0u, 0x50000000u | site);
 }
 
-// Two signed bytes of `word` (selector 0x4140: bytes 0, 1; 0x4342: bytes 2, 3) -> BF16 pair,
-// exact. With v = 128 + (b & 127) as the bits 0x4300 | (b & 0x7f), and 128 or 256 as the bits
-// 0x4300 | (b & 0x80), the signed value is their difference. (One permutation and three FMAs
-// do it without the masks: f = bits 0x43 u of u = b + 128, q = f / 2 - 128, value
-// q - max(0, -q); measured 11 % more cycles per block.)
-__device__ __forceinline__ uint32_t int8_pair(uint32_t word, uint32_t selector) {
-  const uint32_t both = __byte_perm(word, 0x43434343u, selector);
-  uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(both & 0xff7fff7fu), "r"(both & 0xff80ff80u));
-  return r;
+// The signed bytes of `word` as BF16 pairs (bytes 0 and 1, 2 and 3), exact. With 128 + (b & 127)
+// as the bits 0x4300 | (b & 0x7f), and 128 or 256 as the bits 0x4300 | (b & 0x80), the signed value
+// is their difference: two masks, four byte permutations, two subtractions. (Masking the
+// permuted pairs is as many instructions and 1.5 % slower over a layer; arithmetic without
+// masks - f = bits 0x43 u of u = b + 128, q = f / 2 - 128, value q - max(0, -q) or
+// min(q, f - 256) - is no faster.)
+__device__ __forceinline__ void int8_pairs(uint32_t word, uint32_t& low, uint32_t& high) {
+  const uint32_t bits = word & 0x7f7f7f7fu, signs = word & 0x80808080u;
+  asm("sub.rn.bf16x2 %0, %1, %2;"
+      : "=r"(low)
+      : "r"(__byte_perm(bits, 0x43434343u, 0x4140)), "r"(__byte_perm(signs, 0x43434343u, 0x4140)));
+  asm("sub.rn.bf16x2 %0, %1, %2;"
+      : "=r"(high)
+      : "r"(__byte_perm(bits, 0x43434343u, 0x4342)), "r"(__byte_perm(signs, 0x43434343u, 0x4342)));
 }
 
 __device__ __forceinline__ uint16_t to_bf16(float v) {
@@ -202,14 +206,10 @@ __device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars,
       for (uint32_t c = 0; c < 4; ++c) {
         // 16-byte pieces of a 128-byte row are swizzled by the row's place in its group of 8
         const uint4 w = ptx::ld_shared_v4(row + (((half * 4 + c) ^ (lane & 7)) << 4));
-        v[8 * c + 0] = int8_pair(w.x, 0x4140);
-        v[8 * c + 1] = int8_pair(w.x, 0x4342);
-        v[8 * c + 2] = int8_pair(w.y, 0x4140);
-        v[8 * c + 3] = int8_pair(w.y, 0x4342);
-        v[8 * c + 4] = int8_pair(w.z, 0x4140);
-        v[8 * c + 5] = int8_pair(w.z, 0x4342);
-        v[8 * c + 6] = int8_pair(w.w, 0x4140);
-        v[8 * c + 7] = int8_pair(w.w, 0x4342);
+        int8_pairs(w.x, v[8 * c + 0], v[8 * c + 1]);
+        int8_pairs(w.y, v[8 * c + 2], v[8 * c + 3]);
+        int8_pairs(w.z, v[8 * c + 4], v[8 * c + 5]);
+        int8_pairs(w.w, v[8 * c + 6], v[8 * c + 7]);
       }
       ptx::tmem_store_32x32(to + half * 32, v);
     }
