@@ -501,7 +501,8 @@ grouped_gemm_kernel(const __grid_constant__ GemmParams p) {
     uint64_t t_info = 0, t_stage = 0;
     // bytes that land per stage: the A box (possibly fewer than 128 rows) and the B box
     const uint32_t tx_bytes = (p.a_box_bytes + Cfg::kBBytes) * Cfg::kGroup;
-    const uint32_t k_block_elems = p.byte_operands != 0 ? 2 * kBlockK : kBlockK;   // 128 bytes of a row
+    // 128 bytes of a row
+    const uint32_t k_block_elems = p.byte_operands != 0 ? 2 * kBlockK : kBlockK;
     while (true) {
       const uint32_t slot = reads % kSchedSlots;
       const uint32_t round = (reads / kSchedSlots) & 1u;
@@ -827,9 +828,13 @@ grouped_gemm_kernel(const __grid_constant__ GemmParams p) {
       if constexpr (INT8) {
         if (row_in_tile + lane < valid_m) {
           const uint32_t row = row0 + row_in_tile + lane;
-          row_scale = p.a_row_offsets != nullptr
-                          ? p.packed_row_scale[p.a_row_offsets[expert] + row]
-                          : p.row_scale[expert][row];
+          if (p.a_row_offsets == nullptr) {
+            row_scale = p.row_scale[expert][row];
+          } else {
+            // counts that only the device knows may claim rows that the buffer does not have
+            const uint64_t packed_row = static_cast<uint64_t>(p.a_row_offsets[expert]) + row;
+            if (packed_row < p.check_a_rows) row_scale = p.packed_row_scale[packed_row];
+          }
         }
         col_scale = p.col_scale[expert] + col0;
       }

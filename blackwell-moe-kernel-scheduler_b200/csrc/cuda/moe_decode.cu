@@ -18,6 +18,16 @@
 // the lower halves of the tokens are separate columns of the same MMA.
 // Few tiles are split along k over the CTAs of a cluster, joined in a fixed order through
 // distributed shared memory: no atomics, the same bits on every run.
+//
+// Measured on B200 (us of device time in a CUDA graph, inputs past L2; share of the 6.55 TB/s a
+// copy reaches): hidden 4096, inter 14336, two of 8 experts, T=1: 112 BF16 (96 %), 74 INT8 (73 %);
+// all 8, T=16: 368 BF16 (1.02), T=64: 449 BF16 (96 %), 285 INT8 (76 %). 128 experts of 2048 x
+// 768, top-8: T=1 22.3 BF16 (52 %), T=32 142 (90 %). hidden 512, inter 1024, T=1: 9.7 (latency
+// of two dependent launches). Fragments loaded straight into registers for mma.sync, the
+// version before, took 178 / 848 / 2170 / 1227 us for the first, third, fourth and fifth.
+// One grid that fills the GPU once with an equal share of blocks per CTA was tried for the
+// first kernel and is 0-25 % slower: SMs do not get equal shares of HBM, and a grid of more
+// CTAs than places evens that out.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -185,11 +195,15 @@ __device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars,
 }
 
 // INT8: one warp's 32 rows of every second of `blocks` k-blocks (`turn` 0 or 1, and that buffer)
-// from shared memory to Tensor Memory as BF16. A block takes a warp some 800 cycles, most of
-// them latency, so two groups of four warps take turns.
+// from shared memory to Tensor Memory as BF16. A block takes a warp some 900 cycles, half of
+// them on the integer pipe, so two groups of four warps take turns. This is what keeps INT8
+// layers at 70-75 % of the copy bandwidth (the same kernels without the conversion stream at
+// 85 %): at HBM's rate the integer pipe is busy two thirds of the time. Converting earlier,
+// before the buffer is free, and four groups instead of two measured no better.
 __device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars,
-                                               const Ring<true>& ring, uint32_t tmem, uint32_t quad, uint32_t turn,
-                                               uint32_t lane, uint32_t blocks) {
+                                               const Ring<true>& ring, uint32_t tmem,
+                                               uint32_t quad, uint32_t turn, uint32_t lane,
+                                               uint32_t blocks) {
   Cursor stage;
   uint32_t a_parity = 0;
   if (turn != 0) stage.next(ring.stages);
@@ -452,8 +466,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
       if (!ok && lane == 0) report(a, 3);
     }
     // Accumulator -> shared memory [column][row], over the ring: all of its bytes are used.
-    if (warp >= 8) {
-    } else if (ok && wait(bars.d_full[0], 0)) {
+    if (warp < 8 && ok && wait(bars.d_full[0], 0)) {
       ptx::tc_fence_after_sync();
       const uint32_t to = base + (quad * 32 + lane) * 4;
 #pragma unroll
@@ -470,7 +483,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
         }
       }
       ptx::tc_fence_before_sync();
-    } else if (lane == 0) {
+    } else if (warp < 8 && lane == 0) {
       report(a, 4);
     }
   }
@@ -954,7 +967,10 @@ bool encode_maps(DecodeParams& up, DecodeParams& down, const bmoe_moe_decode_arg
   const uint64_t x_dims[2] = {hidden, a.tokens}, x_strides[1] = {hidden * 2};
   const uint64_t h_dims[3] = {inter, rows, 2}, h_strides[2] = {inter * 2, rows * inter * 2};
   const uint32_t row_box[2] = {64, 1};   // gathered rows: more than 16 tokens only
-  if (a.tokens > 16 && !encode_box(&up.rows, a.x_dev, Elem::kBf16, 2, x_dims, x_strides, row_box)) return false;
+  if (a.tokens > 16 &&
+      !encode_box(&up.rows, a.x_dev, Elem::kBf16, 2, x_dims, x_strides, row_box)) {
+    return false;
+  }
   for (uint32_t g = 0; g * kGroup < a.tokens; ++g) {
     const uint32_t box[3] = {64, (g + 1) * kGroup, 2};
     if (!encode_box(&up.acts[g], a.x_dev, Elem::kBf16, 2, x_dims, x_strides, box) ||

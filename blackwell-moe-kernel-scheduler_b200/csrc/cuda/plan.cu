@@ -15,6 +15,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <cstring>
+#include <exception>
 #include <new>
 #include <vector>
 
@@ -212,8 +213,7 @@ void bmoe_plan_destroy(bmoe_plan* plan) {
   delete plan;
 }
 
-int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
-  if (plan == nullptr || args == nullptr) return BMOE_INVALID_ARGUMENT;
+static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
   plan->ready = false;
   plan->stats = bmoe_plan_stats{};
   const bmoe_gemm_args& a = *args;
@@ -378,10 +378,16 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
   bmoe_plan::Setup& before = plan->setup[plan->turn];
   plan->turn ^= 1u;
   bmoe_plan::Setup& setup = plan->setup[plan->turn];
-  // on another stream than the last set-up, this one follows it
-  if (before.done != nullptr && previous_stream != plan->setup_stream &&
-      cudaStreamWaitEvent(plan->setup_stream, before.done, 0) != cudaSuccess) {
-    return BMOE_CUDA_ERROR;
+  // On another stream than the last set-up, this one follows it. A stream that is being
+  // captured cannot wait for work outside of its graph; there the host waits.
+  if (before.done != nullptr && previous_stream != plan->setup_stream) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(plan->setup_stream, &capture) != cudaSuccess ||
+        (capture == cudaStreamCaptureStatusNone
+             ? cudaStreamWaitEvent(plan->setup_stream, before.done, 0)
+             : cudaEventSynchronize(before.done)) != cudaSuccess) {
+      return BMOE_CUDA_ERROR;
+    }
   }
   if (setup.done == nullptr) {
     if (cudaEventCreateWithFlags(&setup.done, cudaEventDisableTiming) != cudaSuccess) {
@@ -559,6 +565,15 @@ int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
   plan->stats.sm_count = static_cast<uint32_t>(sm_count);
   plan->ready = true;
   return BMOE_OK;
+}
+
+int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args) {
+  if (plan == nullptr || args == nullptr) return BMOE_INVALID_ARGUMENT;
+  try {
+    return initialize_plan(plan, args);
+  } catch (const std::exception&) {   // host memory for the per-expert arrays
+    return BMOE_CUDA_ERROR;
+  }
 }
 
 int bmoe_preload_kernels(void) {

@@ -3,6 +3,13 @@
 // bytes written. Per row, FP32, one rounding per operation:
 //   largest = max(max |x|, 2^-100), scale = largest / 127, q = rint(x * (127 * (1 / largest)))
 // The floor keeps 1 / largest finite and makes a row of zeros quantise to zeros.
+//
+// Bound: HBM, 3 bytes per BF16 value, and close behind it the ALU (two integer operations a
+// pair for the maximum, a shift or mask, a product, a sum and three quarters of a permutation
+// per value). Measured on B200: 16384 rows of 2048 in 17 us (5.9 TB/s, 0.90 of a copy), 8192
+// rows of 4096 gathered from 4096 in 15.9 us (10.3 for the bytes alone, the second reads
+// come from L2), 512 rows of 7168 in 3.4 us. Two passes over the row, one value a thread, took
+// 36.9 us for the gathered case; clamping before the conversion and FP32 maxima 18.2.
 #include <cuda_runtime.h>
 
 #include <cstdint>

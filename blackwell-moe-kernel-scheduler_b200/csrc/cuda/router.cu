@@ -10,6 +10,12 @@
 // One warp per token. Keys live in registers as unsigned integers whose order is the
 // order of the floats; a choice is one warp maximum over the keys and one warp minimum
 // over the ids that hold it.
+//
+// Bound: latency (loads, top_k dependent rounds) for few tokens, instruction issue for many (77 %
+// of the slots; the bytes alone would take 0.9 us). Measured on B200: 16384 x 128 BF16, top-8,
+// softmax 9.0 us; 4 x 256 FP32, top-8, sigmoid with bias 4.9 us. Scanning all keys of a lane in
+// every round instead of sorting them once took 11.0 us; one packed 32-bit key and id for
+// BF16, which saves the second warp operation, measured no faster (9.0).
 #include <cuda_runtime.h>
 
 #include <cstdint>

@@ -65,7 +65,8 @@ def _scales_fit(data_type, a, w, row_scale, col_scale) -> bool:
 
     if data_type != _capi.TYPE_INT8:
         return data_type != -1 and row_scale is None and col_scale is None
-    return (row_scale is not None and col_scale is not None
+    return (a.dtype is w.dtype is torch.int8
+            and row_scale is not None and col_scale is not None
             and row_scale.dtype is torch.float32 and col_scale.dtype is torch.float32
             and row_scale.device == a.device and col_scale.device == a.device
             and row_scale.is_contiguous() and col_scale.is_contiguous()

@@ -3,9 +3,10 @@
 
 Thin wrappers of the C entry points (``include/bmoe_b200.h``, section 6). Each allocates the
 outputs it is not given, launches on ``stream`` (default: the current stream of the tensors'
-device) and does not synchronise. Wrong shapes, types or devices raise ``ValueError``, a
-status of the engine raises ``EngineError``. The reference has no counterpart: routed
-token counts are its input (agent/search_space.yaml:10-13).
+device) and does not synchronise; what it allocates belongs to that stream. Wrong shapes,
+types or devices raise ``ValueError``, a status of the engine raises ``EngineError``. The
+reference has no counterpart: routed token counts are its input
+(agent/search_space.yaml:10-13).
 """
 
 from __future__ import annotations
@@ -24,15 +25,19 @@ _NO_GUARD = contextlib.nullcontext()
 _current_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _on(index: int):
-    """Context in which device ``index`` is the current one."""
-    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
-
-
-def _raw_stream(stream, index: int) -> int | None:
+def _on(index: int, stream):
+    """Context in which device ``index`` and ``stream`` are the current ones: what is allocated
+    in it belongs to the stream that the launch goes to, so the allocator neither hands out
+    memory that older work of another stream still reads nor takes it back too early."""
     if stream is None:
-        return _current_raw_stream(index) or None
-    return int(getattr(stream, "cuda_stream", stream)) or None
+        return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
+    if not isinstance(stream, torch.cuda.Stream):
+        raw = int(getattr(stream, "cuda_stream", stream))
+        stream = (torch.cuda.ExternalStream(raw, device=index) if raw
+                  else torch.cuda.default_stream(index))
+    if stream.device_index != index:
+        raise ValueError(f"stream: one of cuda:{index} needed, got {stream.device}")
+    return torch.cuda.stream(stream)
 
 
 def _is(x, dtype, shape, index: int) -> bool:
@@ -76,7 +81,7 @@ def route_topk(logits, top_k: int, *, scoring: str = "softmax", renormalize: boo
         raise ValueError(f"unknown scoring: {scoring}")
     if bias is not None:
         _need(bias, "bias", torch.float32, (experts,), index)
-    with _on(index):
+    with _on(index, stream):
         if expert_ids is None:
             expert_ids = torch.empty(tokens, top_k, dtype=torch.int64, device=logits.device)
         else:
@@ -88,7 +93,7 @@ def route_topk(logits, top_k: int, *, scoring: str = "softmax", renormalize: boo
         args = _capi.RouteTopkArgs(
             logits.data_ptr(), None if bias is None else bias.data_ptr(), expert_ids.data_ptr(),
             weights.data_ptr(), tokens, row_stride, experts, top_k, _ROW_TYPES[logits.dtype],
-            _capi.SCORINGS[scoring], int(renormalize), scale, _raw_stream(stream, index))
+            _capi.SCORINGS[scoring], int(renormalize), scale, _current_raw_stream(index) or None)
         _capi.check(_capi.load().bmoe_route_topk(C.byref(args)), "bmoe_route_topk")
     return expert_ids, weights
 
@@ -104,7 +109,7 @@ def quantize_rows(x, index=None, *, out=None, scale=None, stream=None):
     if index is not None:
         rows = index.numel()
         _need(index, "index", torch.int64, (rows,), device)
-    with _on(device):
+    with _on(device, stream):
         if out is None:
             out = torch.empty(rows, cols, dtype=torch.int8, device=x.device)
         else:
@@ -116,7 +121,7 @@ def quantize_rows(x, index=None, *, out=None, scale=None, stream=None):
         args = _capi.QuantizeRowsArgs(
             x.data_ptr(), None if index is None else index.data_ptr(), out.data_ptr(),
             scale.data_ptr(), rows, src_rows, row_stride, cols, _ROW_TYPES[x.dtype],
-            _raw_stream(stream, device))
+            _current_raw_stream(device) or None)
         _capi.check(_capi.load().bmoe_quantize_rows(C.byref(args)), "bmoe_quantize_rows")
     return out, scale
 
@@ -163,7 +168,7 @@ def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
         _need(gate_up_scale, "gate_up_scale", torch.float32, (experts, 2 * inter), index)
         _need(down_scale, "down_scale", torch.float32, (experts, hidden), index)
     lib = _capi.load()
-    with _on(index):
+    with _on(index, stream):
         if out is None:
             out = torch.empty_like(x)
         else:
@@ -178,6 +183,6 @@ def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
             gate_up_scale.data_ptr() if int8 else None, down_scale.data_ptr() if int8 else None,
             expert_ids.data_ptr(), weights.data_ptr(), out.data_ptr(), workspace.data_ptr(),
             workspace.numel(), tokens, top_k, experts, hidden, inter, _WEIGHT_TYPES[kind],
-            _raw_stream(stream, index))
+            _current_raw_stream(index) or None)
         _capi.check(lib.bmoe_moe_decode(C.byref(args)), "bmoe_moe_decode")
     return out

@@ -277,3 +277,49 @@ def test_quantised_layer_as_it_is_used(engine):
     want = want.sum(1)
     assert torch.all((combined.double() - want).abs() <= want.abs() * half16
                      + size * top_k * 2.0 ** -23)
+
+
+def test_int8_type_needs_one_byte_operands(engine):
+    a = torch.zeros(16, 32, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(1, 8, 32, dtype=torch.bfloat16, device="cuda")
+    d = torch.zeros(16, 8, dtype=torch.bfloat16, device="cuda")
+    scales = dict(row_scale=torch.ones(16, device="cuda"), col_scale=torch.ones(1, 8, device="cuda"))
+    plan = engine.GroupedGemmPlan()
+    try:
+        assert plan.initialize_packed(a, w, d, [16], data_type=3, **scales) == \
+            engine._capi.INVALID_ARGUMENT
+    finally:
+        plan.close()
+
+
+def test_plan_recaptured_on_another_stream(engine):
+    """A plan that was set up eagerly on one stream is set up again while another stream is
+    captured (relaxed mode): the graph holds set-up and launch and replays on new inputs."""
+    counts, n, k = [37, 0, 1, 200], 384, 192
+    a, w, row, col = make_int8(counts, n, k)
+    dev = [t.cuda() for t in (a, w, row, col)]
+    d = torch.zeros(sum(counts), n, dtype=torch.bfloat16, device="cuda")
+    plan, side = engine.GroupedGemmPlan(), torch.cuda.Stream()
+    try:
+        for _ in range(2):
+            assert plan.initialize_packed(dev[0], dev[1], d, counts, row_scale=dev[2],
+                                          col_scale=dev[3], stream=None) == 0
+            assert plan.run() == 0
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side, capture_error_mode="relaxed"):
+            assert plan.initialize_packed(dev[0], dev[1], d, counts, row_scale=dev[2],
+                                          col_scale=dev[3], stream=side) == 0
+            assert plan.run(side) == 0
+        for seed in (5, 6):
+            a = make_int8(counts, n, k, seed=seed)[0]
+            dev[0].copy_(a)
+            d.fill_(float("nan"))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            check(d.cpu(), exact(a, w, row, col, counts), 2.0 ** -8 + 4 * 2.0 ** -24)
+        del graph
+    finally:
+        torch.cuda.synchronize()
+        plan.close()

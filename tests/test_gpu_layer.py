@@ -523,3 +523,36 @@ def test_moe_decode_weights_past_32_bit_offsets(engine):
     want, bound = layer_oracle(small)
     assert torch.all((out[:1].double().cpu() - want).abs() <= bound)
     assert torch.all(out[1] == 0)
+
+
+def test_allocations_belong_to_the_stream_of_the_launch(engine, monkeypatch):
+    """Memory that a call allocates for a launch on another stream must not be handed out on
+    the current stream while the launch has not run yet."""
+    layer = make_layer(5, 6, 2, 256, 128, False, seed=3)
+    dev = {k: (v.cuda() if v is not None else None) for k, v in layer.items()}
+    seen = []
+    make = engine._capi.MoeDecodeArgs
+    monkeypatch.setattr(engine._capi, "MoeDecodeArgs",
+                        lambda *a: (lambda args: seen.append(args.workspace_dev) or args)(make(*a)))
+    side = torch.cuda.Stream()
+    need = engine.moe_decode_workspace(5, 2, 128)
+    logits, rows = torch.randn(5, 6, device="cuda"), torch.randn(5, 256, device="cuda")
+    want = check_layer(engine, layer)
+    torch.cuda.synchronize()
+    for stream in (side, side.cuda_stream):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        got = engine.moe_decode(dev["x"], dev["w1"], dev["w2"], dev["ids"], dev["coef"],
+                                stream=stream)
+        ids, coef = engine.route_topk(logits, 2, stream=stream)
+        q, scale = engine.quantize_rows(rows, stream=stream)
+        taken = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes()
+                 for t in (ids, coef, q, scale)}
+        taken[seen[-1]] = need
+        del ids, coef, q, scale
+        fresh = [torch.full((size,), 0xFF, dtype=torch.uint8, device="cuda")
+                 for size in taken.values()]
+        assert not {t.data_ptr() for t in fresh} & set(taken)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    assert torch.cuda.current_stream() != side
