@@ -195,11 +195,12 @@ __device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars,
 }
 
 // INT8: one warp's 32 rows of every second of `blocks` k-blocks (`turn` 0 or 1, and that buffer)
-// from shared memory to Tensor Memory as BF16. A block takes a warp some 900 cycles, half of
-// them on the integer pipe, so two groups of four warps take turns. This is what keeps INT8
-// layers at 70-75 % of the copy bandwidth (the same kernels without the conversion stream at
-// 85 %): at HBM's rate the integer pipe is busy two thirds of the time. Converting earlier,
-// before the buffer is free, and four groups instead of two measured no better.
+// from shared memory to Tensor Memory as BF16. Two groups of four warps take turns, since most
+// of a block's time in a warp is latency. The conversion is what keeps INT8 layers at 72-76 %
+// of the copy bandwidth: without it (wrong results, streaming only) the same kernels reach
+// 85-87 %. With it the integer pipe is busy 56 % of the time at 4.5 TB/s and the issue slots
+// 49 % (one token); fewer integer operations (see int8_pairs), four groups instead of two and
+// converting ahead of the free buffer all measured within 1 %.
 __device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars,
                                                const Ring<true>& ring, uint32_t tmem,
                                                uint32_t quad, uint32_t turn, uint32_t lane,
