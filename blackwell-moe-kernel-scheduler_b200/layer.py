@@ -133,7 +133,7 @@ def moe_decode_workspace(tokens: int, top_k: int, inter: int) -> int:
 
 def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
                down_scale=None, out=None, workspace=None, stream=None):
-    """A whole expert layer for up to 64 tokens, in two launches.
+    """A whole expert layer for up to 64 tokens.
 
     ``x`` BF16 [tokens, hidden]; ``w_gate_up`` [experts, 2 * inter, hidden] (gate rows, then
     up rows) and ``w_down`` [experts, hidden, inter], both BF16, or both INT8 with the

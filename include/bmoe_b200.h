@@ -933,16 +933,18 @@ typedef struct bmoe_moe_decode_args {
  * captured graphs replayed at once) need a workspace each. */
 uint64_t bmoe_moe_decode_workspace(uint32_t tokens, uint32_t top_k, uint32_t inter);
 
-/* A whole expert layer for a few tokens (a decode step), in two launches:
+/* A whole expert layer for a few tokens (a decode step), in two launches or four:
  *   h[t, j] = silu(x[t] Wgate_e^T) * (x[t] Wup_e^T),  e = expert_ids[t, j]
  *   out[t]  = bf16( sum_j weights[t, j] * (h[t, j] Wdown_e^T) )
  * with silu(v) = v / (1 + exp(-v)). Every weight of an expert that some token chose is
  * read once, the others not at all. Products of BF16 operands are summed in FP32, h keeps
  * 16 significant bits or more, one BF16 rounding at the end; INT8 weights are multiplied
- * as the integers they are and scaled per output channel in FP32. An expert that a token
+ * as the integers they are and scaled per output channel in FP32. Where INT8 weights outweigh
+ * two more launches, the rows of x and h become fixed-point numbers whose last place is 2^-22 of
+ * the row's largest magnitude or less, and their sums with the weights are exact; a row of x
+ * or h with a NaN or an infinity then makes its token's output NaN. An expert that a token
  * names twice counts with the sum of both weights. Dropped assignments contribute nothing;
- * a token with nothing else gets a row of zeros. Results do not depend on the run: no
- * atomics. x, the weights and out are 16-byte aligned, the rest as their types. out may be x.
+ * a token with nothing else gets a row of zeros. Results do not depend on the run. x, the weights and out are 16-byte aligned, the rest as their types. out may be x.
  * For more tokens there is the grouped GEMM plan. */
 int bmoe_moe_decode(const bmoe_moe_decode_args* args);
 

@@ -556,3 +556,108 @@ def test_allocations_belong_to_the_stream_of_the_launch(engine, monkeypatch):
         torch.cuda.synchronize()
         assert torch.equal(got, want)
     assert torch.cuda.current_stream() != side
+
+
+# INT8 layers with 36 MB of chosen weights or more and at most 24 tokens an expert: activations
+# as fixed-point digits (the rule in moe_decode.cu).
+DIGIT_LAYERS = [
+    # tokens, experts, top_k, hidden, inter
+    (1, 1, 1, 3504, 3504), (1, 2, 2, 2064, 3008), (2, 8, 8, 1040, 1456), (5, 3, 2, 2064, 2000),
+    (16, 8, 4, 1040, 1456), (17, 8, 4, 1040, 1456), (33, 8, 4, 1040, 1456), (64, 8, 3, 1040, 1456),
+    (9, 40, 5, 4000, 80), (24, 1024, 32, 112, 144), (64, 1024, 16, 128, 96), (3, 8, 3, 288, 14336),
+]
+
+
+def digit_bound(layer, bound):
+    """The operator's bound plus what the digits lose: an x is off by 2^-22 of its row's largest
+    at most, and so is an h (times its weight); the sums of digits are exact."""
+    x, extra = layer["x"].double(), torch.zeros_like(bound)
+    most = 2.0 ** -22 * x.abs().amax(1)
+    for t in range(x.shape[0]):
+        for j, e in enumerate(layer["ids"][t].tolist()):
+            if not 0 <= e < layer["w1"].shape[0]:
+                continue
+            inter = layer["w2"].shape[2]
+            w1 = layer["w1"][e].double() * layer["s1"][e].double()[:, None]
+            w2 = (layer["w2"][e].double() * layer["s2"][e].double()[:, None]).abs()
+            both, both_err = w1 @ x[t], w1.abs().sum(1) * most[t]
+            gate, up = both[:inter], both[inter:]
+            silu = gate / (1 + torch.exp(-gate))
+            h_err = (1.1 * both_err[:inter] * (up.abs() + both_err[inter:])
+                     + silu.abs() * both_err[inter:])
+            h_err = h_err + ((silu * up).abs() + h_err).max() * 2.0 ** -22
+            extra[t] += layer["coef"][t, j].double().abs() * (w2 @ h_err)
+    return bound + extra
+
+
+@pytest.mark.parametrize("sizes", DIGIT_LAYERS)
+def test_moe_decode_digits(engine, sizes):
+    layer = make_layer(*sizes, True, seed=sum(sizes), drop=0.1 if sizes[0] > 2 else 0.0)
+    check_layer(engine, layer)
+
+
+def test_moe_decode_digits_of_rows_with_a_wide_range(engine):
+    """One large value in a row, values far below it, a row of zeros, one of subnormals, one
+    of the largest numbers; rows that hold a NaN or an infinity stay alone with it."""
+    layer = make_layer(8, 8, 8, 1040, 1456, True, seed=77)
+    x, g = layer["x"], gen(78)
+    x[0, 17] = 4096.0
+    x[1] = x[1] * (2.0 ** torch.randint(-40, 1, (1040,), generator=g)).to(torch.bfloat16)
+    x[2] = 0.0
+    x[3] = x[3].sign() * 2.0 ** -130
+    x[4] = x[4] * 2.0 ** 20
+    layer["coef"][5] = 2.0 ** -60
+    clean = run_layer(engine, layer)
+    want, bound = layer_oracle(layer)
+    bound = digit_bound(layer, bound)
+    assert torch.all((clean.double().cpu() - want).abs() <= bound)
+    assert torch.all(clean[2:4] == 0)
+    bad = dict(layer, x=x.clone())
+    bad["x"][6, 3], bad["x"][7, 1039] = math.nan, math.inf
+    got = run_layer(engine, bad)
+    assert torch.equal(got[:6], clean[:6])
+    assert not torch.isfinite(got[6:]).any()
+
+
+def test_moe_decode_digits_that_do_not_fit_beside_h(engine):
+    """hidden > top_k * inter: the weights are converted instead."""
+    check_layer(engine, make_layer(20, 64, 1, 4000, 160, True, seed=8))
+
+
+def test_moe_decode_digits_dropped_repeated_streams_and_graphs(engine):
+    layer = make_layer(16, 8, 4, 1040, 1456, True, seed=12)
+    layer["ids"][3] = 5                                 # four times the same expert
+    layer["ids"][4, 2:] = torch.tensor([-1, 90])
+    layer["ids"][5] = -1
+    need = engine.moe_decode_workspace(16, 4, 1456)
+    dirty = torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda")
+    want = check_layer(engine, layer, workspace=dirty)
+    assert torch.all(want[5] == 0)
+    dev = {k: v.cuda() for k, v in layer.items()}
+
+    def call(x=dev["x"], ids=dev["ids"], **options):
+        return engine.moe_decode(x, dev["w1"], dev["w2"], ids, dev["coef"],
+                                 gate_up_scale=dev["s1"], down_scale=dev["s2"], **options)
+
+    assert torch.all(call(ids=torch.full_like(dev["ids"], -1)) == 0)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    results = [call(stream=s) for _ in range(10) for s in streams]
+    torch.cuda.synchronize()
+    assert all(torch.equal(r, want) for r in results)
+    x = dev["x"].clone()
+    call(x=x, out=x)                                    # in place
+    assert torch.equal(x, want)
+    x.copy_(dev["x"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(x=x)
+    for seed in (1, 2):
+        x.copy_(torch.randn(16, 1040, generator=gen(seed)).to(torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call(x=x))
+    x.copy_(dev["x"])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
