@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -511,6 +512,30 @@ def load() -> C.CDLL:
         fn.argtypes = argtypes
     _lib = lib
     return lib
+
+
+_PACK_CODES = {C.c_void_p: "Q", C.c_uint64: "Q", C.c_uint32: "I", C.c_float: "f"}
+
+
+def entry(name: str, layout):
+    """The C function ``name`` of one argument struct, as a call with the struct's fields in
+    order (0 for a null pointer). Packing bytes costs a third of building the ctypes structure
+    ``layout`` (0.4 instead of 1.2 us a call), which counts beside a kernel of a few."""
+    packer = struct.Struct("@" + "".join(_PACK_CODES[kind] for _, kind in layout._fields_))
+    assert packer.size == C.sizeof(layout)
+    function = None
+
+    def call(*fields) -> int:
+        nonlocal function
+        if function is None:
+            function = load()[name]      # an own function object, beside the declared one
+            function.restype, function.argtypes = C.c_int, [C.c_char_p]
+        try:
+            return function(packer.pack(*fields))
+        except struct.error as wrong:
+            raise ValueError(f"{name}: {wrong}") from None
+
+    return call
 
 
 def status_string(status: int) -> str:

@@ -12,7 +12,6 @@ reference has no counterpart: routed token counts are its input
 from __future__ import annotations
 
 import contextlib
-import ctypes as C
 
 import torch
 
@@ -23,6 +22,9 @@ _WEIGHT_TYPES = {torch.bfloat16: _capi.TYPE_BF16, torch.int8: _capi.TYPE_INT8}
 _NO_GUARD = contextlib.nullcontext()
 # the raw handle of a device's current stream, without building a Stream object
 _current_raw_stream = torch._C._cuda_getCurrentRawStream
+_route_topk = _capi.entry("bmoe_route_topk", _capi.RouteTopkArgs)
+_quantize_rows = _capi.entry("bmoe_quantize_rows", _capi.QuantizeRowsArgs)
+_moe_decode = _capi.entry("bmoe_moe_decode", _capi.MoeDecodeArgs)
 
 
 def _on(index: int, stream):
@@ -42,7 +44,7 @@ def _on(index: int, stream):
 
 def _is(x, dtype, shape, index: int) -> bool:
     """``x`` is a contiguous tensor of that type and shape on CUDA device ``index``."""
-    return (x.dtype is dtype and x.shape == shape and x.is_cuda and x.get_device() == index
+    return (x.dtype is dtype and x.shape == shape and x.get_device() == index
             and x.is_contiguous())
 
 
@@ -90,11 +92,11 @@ def route_topk(logits, top_k: int, *, scoring: str = "softmax", renormalize: boo
             weights = torch.empty(tokens, top_k, dtype=torch.float32, device=logits.device)
         else:
             _need(weights, "weights", torch.float32, (tokens, top_k), index)
-        args = _capi.RouteTopkArgs(
-            logits.data_ptr(), None if bias is None else bias.data_ptr(), expert_ids.data_ptr(),
+        status = _route_topk(
+            logits.data_ptr(), 0 if bias is None else bias.data_ptr(), expert_ids.data_ptr(),
             weights.data_ptr(), tokens, row_stride, experts, top_k, _ROW_TYPES[logits.dtype],
-            _capi.SCORINGS[scoring], int(renormalize), scale, _current_raw_stream(index) or None)
-        _capi.check(_capi.load().bmoe_route_topk(C.byref(args)), "bmoe_route_topk")
+            _capi.SCORINGS[scoring], 1 if renormalize else 0, scale, _current_raw_stream(index))
+        _capi.check(status, "bmoe_route_topk")
     return expert_ids, weights
 
 
@@ -118,11 +120,11 @@ def quantize_rows(x, index=None, *, out=None, scale=None, stream=None):
             scale = torch.empty(rows, dtype=torch.float32, device=x.device)
         else:
             _need(scale, "scale", torch.float32, (rows,), device)
-        args = _capi.QuantizeRowsArgs(
-            x.data_ptr(), None if index is None else index.data_ptr(), out.data_ptr(),
+        status = _quantize_rows(
+            x.data_ptr(), 0 if index is None else index.data_ptr(), out.data_ptr(),
             scale.data_ptr(), rows, src_rows, row_stride, cols, _ROW_TYPES[x.dtype],
-            _current_raw_stream(device) or None)
-        _capi.check(_capi.load().bmoe_quantize_rows(C.byref(args)), "bmoe_quantize_rows")
+            _current_raw_stream(device))
+        _capi.check(status, "bmoe_quantize_rows")
     return out, scale
 
 
@@ -178,11 +180,11 @@ def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
                                     dtype=torch.uint8, device=x.device)
         else:
             _need(workspace, "workspace", torch.uint8, (workspace.numel(),), index)
-        args = _capi.MoeDecodeArgs(
+        status = _moe_decode(
             x.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(),
-            gate_up_scale.data_ptr() if int8 else None, down_scale.data_ptr() if int8 else None,
+            gate_up_scale.data_ptr() if int8 else 0, down_scale.data_ptr() if int8 else 0,
             expert_ids.data_ptr(), weights.data_ptr(), out.data_ptr(), workspace.data_ptr(),
             workspace.numel(), tokens, top_k, experts, hidden, inter, _WEIGHT_TYPES[kind],
-            _current_raw_stream(index) or None)
-        _capi.check(lib.bmoe_moe_decode(C.byref(args)), "bmoe_moe_decode")
+            _current_raw_stream(index), 0)
+        _capi.check(status, "bmoe_moe_decode")
     return out

@@ -531,9 +531,9 @@ def test_allocations_belong_to_the_stream_of_the_launch(engine, monkeypatch):
     layer = make_layer(5, 6, 2, 256, 128, False, seed=3)
     dev = {k: (v.cuda() if v is not None else None) for k, v in layer.items()}
     seen = []
-    make = engine._capi.MoeDecodeArgs
-    monkeypatch.setattr(engine._capi, "MoeDecodeArgs",
-                        lambda *a: (lambda args: seen.append(args.workspace_dev) or args)(make(*a)))
+    run = engine.layer._moe_decode
+    place = [name for name, _ in engine._capi.MoeDecodeArgs._fields_].index("workspace_dev")
+    monkeypatch.setattr(engine.layer, "_moe_decode", lambda *a: seen.append(a[place]) or run(*a))
     side = torch.cuda.Stream()
     need = engine.moe_decode_workspace(5, 2, 128)
     logits, rows = torch.randn(5, 6, device="cuda"), torch.randn(5, 256, device="cuda")

@@ -168,3 +168,24 @@ def test_python_wrappers_refuse_cpu_tensors(engine):
         engine.quantize_rows(torch.zeros(2, 16))
     with pytest.raises(ValueError):
         engine.moe_decode(torch.zeros(2, 16), None, None, None, None)
+
+
+def test_packed_calls_reach_the_same_checks(engine):
+    """The wrappers pass a struct's bytes: the layout is that of the ctypes structure."""
+    cap = engine._capi
+    for name, layout, args in (("bmoe_route_topk", cap.RouteTopkArgs, route_args(cap)),
+                               ("bmoe_quantize_rows", cap.QuantizeRowsArgs, quantize_args(cap)),
+                               ("bmoe_moe_decode", cap.MoeDecodeArgs, decode_args(cap))):
+        call = cap.entry(name, layout)
+        fields = [getattr(args, field) or 0 for field, _ in layout._fields_]
+        names = [field for field, _ in layout._fields_]
+        tokens = names.index("tokens" if "tokens" in names else "rows")
+        assert call(*(0 if i == tokens else v for i, v in enumerate(fields))) == cap.OK
+        last = names.index({"bmoe_route_topk": "top_k", "bmoe_quantize_rows": "cols",
+                            "bmoe_moe_decode": "inter"}[name])
+        assert call(*(7777777 if i == last else v for i, v in enumerate(fields))) == \
+            cap.INVALID_ARGUMENT
+        with pytest.raises(ValueError):
+            call(*(-1 if i == last else v for i, v in enumerate(fields)))
+        with pytest.raises(ValueError):
+            call(*fields[:-1])
