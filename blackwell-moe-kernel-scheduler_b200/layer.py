@@ -12,6 +12,7 @@ reference has no counterpart: routed token counts are its input
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
 
@@ -20,7 +21,8 @@ from . import _capi
 _ROW_TYPES = {torch.bfloat16: _capi.TYPE_BF16, torch.float32: _capi.TYPE_FP32}
 _WEIGHT_TYPES = {torch.bfloat16: _capi.TYPE_BF16, torch.int8: _capi.TYPE_INT8}
 _NO_GUARD = contextlib.nullcontext()
-# the raw handle of a device's current stream, without building a Stream object
+# the current device, and the raw handle of its current stream without a Stream object
+_current_device = torch._C._cuda_getDevice
 _current_raw_stream = torch._C._cuda_getCurrentRawStream
 _route_topk = _capi.entry("bmoe_route_topk", _capi.RouteTopkArgs)
 _quantize_rows = _capi.entry("bmoe_quantize_rows", _capi.QuantizeRowsArgs)
@@ -32,7 +34,7 @@ def _on(index: int, stream):
     in it belongs to the stream that the launch goes to, so the allocator neither hands out
     memory that older work of another stream still reads nor takes it back too early."""
     if stream is None:
-        return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
+        return _NO_GUARD if index == _current_device() else torch.cuda.device(index)
     if not isinstance(stream, torch.cuda.Stream):
         raw = int(getattr(stream, "cuda_stream", stream))
         stream = (torch.cuda.ExternalStream(raw, device=index) if raw
@@ -128,6 +130,7 @@ def quantize_rows(x, index=None, *, out=None, scale=None, stream=None):
     return out, scale
 
 
+@functools.lru_cache(maxsize=256)
 def moe_decode_workspace(tokens: int, top_k: int, inter: int) -> int:
     """Bytes of workspace ``moe_decode`` needs for these sizes."""
     return int(_capi.load().bmoe_moe_decode_workspace(tokens, top_k, inter))
@@ -169,14 +172,13 @@ def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
     if int8:
         _need(gate_up_scale, "gate_up_scale", torch.float32, (experts, 2 * inter), index)
         _need(down_scale, "down_scale", torch.float32, (experts, hidden), index)
-    lib = _capi.load()
     with _on(index, stream):
         if out is None:
             out = torch.empty_like(x)
         else:
             _need(out, "out", torch.bfloat16, (tokens, hidden), index)
         if workspace is None:
-            workspace = torch.empty(lib.bmoe_moe_decode_workspace(tokens, top_k, inter),
+            workspace = torch.empty(moe_decode_workspace(tokens, top_k, inter),
                                     dtype=torch.uint8, device=x.device)
         else:
             _need(workspace, "workspace", torch.uint8, (workspace.numel(),), index)
