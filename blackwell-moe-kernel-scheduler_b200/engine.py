@@ -74,6 +74,12 @@ def _scales_fit(data_type, a, w, row_scale, col_scale) -> bool:
             and tuple(col_scale.shape) == tuple(w.shape[:2]))
 
 
+def _table(index: np.ndarray, columns) -> np.ndarray:
+    """One line ``base + index * size`` per (base, size); addresses are whole uint64 values."""
+    spec = np.array(columns, dtype=np.uint64)
+    return spec[:, :1] + spec[:, 1:] * index
+
+
 def _expert_pointers(per_expert) -> np.ndarray:
     """Address of every expert's slice of a contiguous FP32 tensor [experts, n]."""
     experts, n = int(per_expert.shape[0]), int(per_expert.shape[1])
@@ -135,8 +141,6 @@ class GroupedGemmPlan:
         is then ignored). ``results_pushed``: no D descriptors, results leave through
         ``set_push``. ``row_scale_ptrs`` / ``col_scale_ptrs`` / ``packed_row_scale``: scales
         of INT8 operands (``data_type`` 3)."""
-        experts = len(tokens_per_expert)
-
         def pointers(values):
             if not isinstance(values, np.ndarray):
                 values = np.array([int(p or 0) for p in values], dtype=np.uint64)
@@ -144,20 +148,32 @@ class GroupedGemmPlan:
                 values = np.ascontiguousarray(values, dtype=np.uint64)
             return values if values.size else np.zeros(1, dtype=np.uint64)
 
-        arr_a, arr_b, arr_d = pointers(a_ptrs), pointers(b_ptrs), pointers(d_ptrs)
-        arr_row = None if row_scale_ptrs is None else pointers(row_scale_ptrs)
-        arr_col = None if col_scale_ptrs is None else pointers(col_scale_ptrs)
+        arrays = [None if ptrs is None else pointers(ptrs)
+                  for ptrs in (a_ptrs, b_ptrs, d_ptrs, row_scale_ptrs, col_scale_ptrs)]
+        return self._initialize(
+            *(None if arr is None else _address(arr) for arr in arrays), tokens_per_expert, n, k,
+            scheduler=scheduler, data_type=data_type, stream=stream, claim_size=claim_size,
+            hybrid_tail_tiles=hybrid_tail_tiles, cta_count=cta_count, tile_n=tile_n,
+            cta_group=cta_group, raster_along_m=raster_along_m, output_f32=output_f32,
+            packed_a=packed_a, packed_rows=packed_rows, results_pushed=results_pushed,
+            tokens_per_expert_dev=tokens_per_expert_dev, packed_row_scale=packed_row_scale)
+
+    def _initialize(self, a, b, d, row_scale, col_scale, tokens_per_expert, n, k, *,
+                    scheduler="expert_order", data_type=0, stream=None, claim_size=0,
+                    hybrid_tail_tiles=0, cta_count=0, tile_n=0, cta_group=0, raster_along_m=-1,
+                    output_f32=False, packed_a=0, packed_rows=0, results_pushed=False,
+                    tokens_per_expert_dev=0, packed_row_scale=0) -> int:
+        """``initialize`` with the addresses of the pointer arrays, which outlive the call."""
         counts = np.ascontiguousarray(tokens_per_expert, dtype=np.uint32)
-        if counts.size == 0:
+        experts = counts.size
+        if experts == 0:
             counts = np.zeros(1, dtype=np.uint32)
         args = _capi.GemmArgs(
-            _address(arr_a), _address(arr_b), _address(arr_d), _address(counts),
-            experts, n, k, data_type, _scheduler_id(scheduler), claim_size, hybrid_tail_tiles,
-            min(int(cta_count), 0xFFFFFFFF), tile_n, cta_group, raster_along_m,
+            a, b, d, _address(counts), experts, n, k, data_type, _scheduler_id(scheduler),
+            claim_size, hybrid_tail_tiles, min(int(cta_count), 0xFFFFFFFF), tile_n, cta_group, raster_along_m,
             1 if output_f32 else 0, _stream_ptr(stream), int(packed_a) or None, int(packed_rows),
             1 if results_pushed else 0, 0, int(tokens_per_expert_dev) or None,
-            None if arr_row is None else _address(arr_row),
-            None if arr_col is None else _address(arr_col), int(packed_row_scale) or None)
+            row_scale, col_scale, int(packed_row_scale) or None)
         return int(self._lib.bmoe_plan_initialize(self._handle, C.byref(args)))
 
     def initialize_packed(self, a, w, d, tokens_per_expert: Sequence[int], *,
@@ -173,39 +189,42 @@ class GroupedGemmPlan:
         ``a`` instead of one per expert (cheaper to re-plan; tiles at an expert's ragged
         edge then also load the next expert's rows, which costs bandwidth when experts
         have few rows and changes no result)."""
-        experts = len(tokens_per_expert)
-        n, k = int(w.shape[1]), int(w.shape[2])
+        experts, n, k = w.shape
         d_elem = 4 if options.get("output_f32") else 2
         if d.element_size() != d_elem:
             return _capi.INVALID_ARGUMENT
-        if int(w.shape[0]) != experts or int(a.shape[1]) != k or int(d.shape[1]) != n:
+        if experts != len(tokens_per_expert) or a.shape[1] != k or d.shape[1] != n:
             return _capi.INVALID_ARGUMENT
         if not (a.is_contiguous() and w.is_contiguous() and d.is_contiguous()):
             return _capi.INVALID_ARGUMENT
         counts = np.asarray(tokens_per_expert, dtype=np.int64)
-        total = int(counts.sum())
-        if int(a.shape[0]) < total or int(d.shape[0]) < total:
+        ends = counts.cumsum()
+        total = int(ends[-1]) if experts else 0
+        if a.shape[0] < total or d.shape[0] < total:
             return _capi.INVALID_ARGUMENT
-        first_row = (counts.cumsum() - counts).view(np.uint64)
-        elem = int(a.element_size())
-        if elem != int(w.element_size()) or elem not in (1, 2):
+        elem = a.element_size()
+        if elem != w.element_size() or elem not in (1, 2):
             return _capi.INVALID_ARGUMENT
         if elem == 1:
             options["data_type"] = _byte_type(a, w, row_scale is not None or col_scale is not None)
         if not _scales_fit(options.get("data_type"), a, w, row_scale, col_scale):
             return _capi.INVALID_ARGUMENT
-        if row_scale is not None:
-            options["row_scale_ptrs"] = row_scale.data_ptr() + first_row * 4
-            options["col_scale_ptrs"] = _expert_pointers(col_scale)
-            if single_a_map:
-                options["packed_row_scale"] = row_scale.data_ptr()
-        a_ptrs = a.data_ptr() + first_row * (k * elem)
-        b_ptrs = w.data_ptr() + np.arange(experts, dtype=np.uint64) * (n * k * elem)
-        d_ptrs = d.data_ptr() + first_row * (n * d_elem)
-        self._keep = (a, w, d, row_scale, col_scale)
+        scaled = row_scale is not None
+        # every expert's address: base + first row * bytes of a row, or + id * bytes of a slice
+        rows = _table((ends - counts).view(np.uint64), (
+            (a.data_ptr(), k * elem), (d.data_ptr(), n * d_elem),
+            (row_scale.data_ptr() if scaled else 0, 4)))
+        slices = _table(np.arange(experts, dtype=np.uint64), (
+            (w.data_ptr(), n * k * elem), (col_scale.data_ptr() if scaled else 0, 4 * n)))
+        by_row, by_slice, line = _address(rows), _address(slices), 8 * experts
         if single_a_map:
-            options.update(packed_a=a.data_ptr(), packed_rows=int(a.shape[0]))
-        return self.initialize(a_ptrs, b_ptrs, d_ptrs, counts, n, k, **options)
+            options.update(packed_a=a.data_ptr(), packed_rows=a.shape[0])
+            if scaled:
+                options["packed_row_scale"] = row_scale.data_ptr()
+        self._keep = (a, w, d, row_scale, col_scale)
+        return self._initialize(
+            by_row, by_slice, by_row + line, by_row + 2 * line if scaled else None,
+            by_slice + line if scaled else None, counts, n, k, **options)
 
     def initialize_packed_device_counts(self, a, w, counts_dev_ptr: int, *, row_scale=None,
                                         col_scale=None, **options) -> int:
