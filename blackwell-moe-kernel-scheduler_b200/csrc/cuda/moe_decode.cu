@@ -223,6 +223,13 @@ __device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars,
 // 85-87 %. With it the integer pipe is busy 56 % of the time at 4.5 TB/s and the issue slots
 // 49 % (one token); fewer integer operations (see int8_pairs), four groups instead of two and
 // converting ahead of the free buffer all measured within 1 %.
+//
+// The buffer is waited for before the stage. With an odd number of stages the two groups use a
+// slot in turn, so a group has not seen the slot's use before its own, and a wait by parity
+// takes that use, if its load is still under way, for the one it waits for: the block of one
+// ring earlier would be converted. Buffer b % 2 is free when the MMAs of block b - 2 are
+// through, so block b - 2 and all before it have landed, and with two stages or more the
+// slot's use before is one of them.
 __device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars,
                                                const Ring<Kind::kConvert>& ring, uint32_t tmem,
                                                uint32_t quad, uint32_t turn, uint32_t lane,
@@ -232,8 +239,8 @@ __device__ __forceinline__ bool convert_blocks(const Wait& wait, Barriers& bars,
   if (turn != 0) stage.next(ring.stages);
   const uint32_t to = tmem + turn * (kTmemA / 2) + ((quad * 32) << 16);
   for (uint32_t b = turn; b < blocks; b += 2) {
-    if (!wait(bars.full[stage.slot], stage.parity)) return false;
     if (!wait(bars.a_empty[turn], a_parity ^ 1u)) return false;
+    if (!wait(bars.full[stage.slot], stage.parity)) return false;
     ptx::tc_fence_after_sync();
     const uint32_t row = ring.at(stage.slot) + (quad * 32 + lane) * 128;
 #pragma unroll
@@ -1137,6 +1144,14 @@ cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cuda
   constexpr uint32_t kPieces = Block<KIND>::kPieces, kBlockK = Block<KIND>::kK;
   constexpr DecodeKernel kUp = decode_up_kernel<KIND, COLS>;
   constexpr DecodeKernel kDown = decode_down_kernel<KIND, COLS>;
+  // convert_blocks needs two stages: at the most columns an MMA can have, with the sums of
+  // COLS tokens and the lists of all experts taken from the second kernel's ring
+  constexpr uint32_t kLeast = kABytes + 2 * COLS * 128, kLeastDown = kABytes + 4 * COLS * 128;
+  constexpr uint32_t kSmem = kDownTmem<KIND, COLS> <= 256 ? kTwoPerSm : kOnePerSm;
+  static_assert(KIND != Kind::kConvert ||
+                (kTwoPerSm - 1024 >= 2 * kLeast &&
+                 kSmem - 1024 >= COLS * kRows * 4 + BMOE_MOE_DECODE_MAX_EXPERTS * kListBytes +
+                                     2 * kLeastDown));
   const DecodeArgs& a = up.a;
   const uint32_t assignments = a.tokens * a.top_k;
   const uint32_t slots = a.by_expert != 0 ? a.experts : assignments;

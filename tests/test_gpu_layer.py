@@ -335,6 +335,77 @@ def test_moe_decode(engine, sizes, int8):
     assert torch.equal(first.view(torch.int16), again.view(torch.int16))
 
 
+def big_layer(tokens, experts, top_k, hidden, inter, int8, seed):
+    """A layer made on the GPU, for weights that do not fit its L2."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def weights(rows, cols):
+        w = torch.randn(experts, rows, cols, generator=g, device="cuda") * cols ** -0.5
+        if not int8:
+            return w.to(torch.bfloat16), None
+        scale = w.abs().amax(2) / 127
+        return torch.round(w / scale[..., None]).to(torch.int8), scale
+
+    (w1, s1), (w2, s2) = weights(2 * inter, hidden), weights(hidden, inter)
+    x = torch.randn(tokens, hidden, generator=g, device="cuda").to(torch.bfloat16)
+    ids = torch.rand(tokens, experts, generator=g, device="cuda").argsort(1)[:, :top_k]
+    coef = torch.rand(tokens, top_k, generator=g, device="cuda") + 0.05
+    return {"x": x, "w1": w1, "w2": w2, "s1": s1, "s2": s2, "ids": ids.contiguous(), "coef": coef}
+
+
+def big_layer_oracle(layer):
+    """``layer_oracle`` with its bound, an expert at a time on the GPU (a token names an expert
+    once)."""
+    x, ids = layer["x"].double(), layer["ids"]
+    (tokens, hidden), (experts, _, inter) = x.shape, layer["w2"].shape
+    out = torch.zeros(tokens, hidden, dtype=torch.float64, device="cuda")
+    err, step = torch.zeros_like(out), 2 * HALF32
+    for e in range(experts):
+        token, place = torch.nonzero(ids == e, as_tuple=True)
+        if token.numel() == 0:
+            continue
+        w1, w2 = layer["w1"][e].double(), layer["w2"][e].double()
+        if layer["s1"] is not None:
+            w1 = w1 * layer["s1"][e].double()[:, None]
+            w2 = w2 * layer["s2"][e].double()[:, None]
+        both, size = x[token] @ w1.t(), x[token].abs() @ w1.abs().t()
+        both_err = size * (hidden / 16 + 16) * step * 2
+        gate, up = both.chunk(2, 1)
+        gate_err, up_err = both_err.chunk(2, 1)
+        silu = gate / (1 + torch.exp(-gate))
+        h = silu * up
+        h_err = (1.1 * gate_err * (up.abs() + up_err) + silu.abs() * up_err
+                 + h.abs() * (2.0 ** -16 + 8 * HALF32))
+        c = layer["coef"][token, place].double()[:, None]
+        out.index_add_(0, token, c * (h @ w2.t()))
+        err.index_add_(0, token, c * ((h_err + h.abs() * (inter / 16 + 24) * step * 2)
+                                      @ w2.abs().t()))
+    return out, err + out.abs() * HALF16 + 2.0 ** -133
+
+
+# INT8 weights that are converted (small layers, crowded experts) with rings of three stages, of
+# the first or the second kernel or both, and eight k-blocks or more a CTA: the converting warps
+# take turns at a slot.
+@pytest.mark.parametrize("sizes", [(64, 4, 2, 4096, 4096), (32, 8, 2, 1024, 1024),
+                                   (64, 1, 1, 4096, 2048), (48, 2, 1, 2064, 1040),
+                                   (28, 6, 3, 1024, 1008), (40, 3, 2, 4096, 1456)])
+def test_moe_decode_converted_weights_with_three_stages(engine, sizes):
+    layer = big_layer(*sizes, True, seed=sum(sizes))
+    want, bound = big_layer_oracle(layer)
+    cold = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+
+    def call():
+        cold.zero_()                                   # weights come from HBM, not from L2
+        return engine.moe_decode(layer["x"], layer["w1"], layer["w2"], layer["ids"],
+                                 layer["coef"], gate_up_scale=layer["s1"],
+                                 down_scale=layer["s2"])
+
+    first = call()
+    off = (first.double() - want).abs()
+    assert torch.all(off <= bound), (off / bound).max()
+    assert all(torch.equal(call(), first) for _ in range(20))
+
+
 @pytest.mark.parametrize("hidden,inter", [(8, 8), (24, 40), (72, 8), (1000, 56), (264, 1032)])
 def test_moe_decode_odd_multiples_of_eight(engine, hidden, inter):
     for tokens in (1, 6, 20):
