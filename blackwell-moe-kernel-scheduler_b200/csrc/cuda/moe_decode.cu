@@ -1144,14 +1144,16 @@ cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cuda
   constexpr uint32_t kPieces = Block<KIND>::kPieces, kBlockK = Block<KIND>::kK;
   constexpr DecodeKernel kUp = decode_up_kernel<KIND, COLS>;
   constexpr DecodeKernel kDown = decode_down_kernel<KIND, COLS>;
-  // convert_blocks needs two stages: at the most columns an MMA can have, with the sums of
-  // COLS tokens and the lists of all experts taken from the second kernel's ring
-  constexpr uint32_t kLeast = kABytes + 2 * COLS * 128, kLeastDown = kABytes + 4 * COLS * 128;
-  constexpr uint32_t kSmem = kDownTmem<KIND, COLS> <= 256 ? kTwoPerSm : kOnePerSm;
-  static_assert(KIND != Kind::kConvert ||
-                (kTwoPerSm - 1024 >= 2 * kLeast &&
-                 kSmem - 1024 >= COLS * kRows * 4 + BMOE_MOE_DECODE_MAX_EXPERTS * kListBytes +
-                                     2 * kLeastDown));
+  // Rings of two stages at least, whatever the experts' columns: loads overlap MMAs, and
+  // convert_blocks counts on it. The second kernel's ring shares its place with the sums of the
+  // tokens and the lists of the experts.
+  constexpr auto stage_most = [](uint32_t columns) {
+    return kABytes + kPieces * ((columns + 15) / 16 * 16) * 128;
+  };
+  constexpr uint32_t kUpPlanes = DIGITS ? kDigits : 1, kDownPlanes = DIGITS ? kDigits : 2;
+  static_assert(kTwoPerSm - 1024 >= 2 * stage_most(COLS * kUpPlanes));
+  static_assert(kOnePerSm - 1024 >= COLS * kRows * 4 + BMOE_MOE_DECODE_MAX_EXPERTS * kListBytes +
+                                        2 * stage_most(COLS * kDownPlanes));
   const DecodeArgs& a = up.a;
   const uint32_t assignments = a.tokens * a.top_k;
   const uint32_t slots = a.by_expert != 0 ? a.experts : assignments;
@@ -1186,13 +1188,15 @@ cudaError_t launch_decode(const DecodeParams& up, const DecodeParams& down, cuda
 
   // Second kernel: a cluster per 128 channels, all at once. The sums of many tokens leave less
   // for the ring: two CTAs per SM if three stages fit at twice the average number of an
-  // expert's tokens, else one.
+  // expert's tokens and two if one expert has them all, else one.
   const uint32_t reserved = (a.tokens * kRows * 4 + a.experts * kListBytes + 15) / 16 * 16;
   const uint32_t twice = 2 * assignments / a.experts + kGroup;
   const uint32_t columns =
       (twice < a.tokens ? twice : a.tokens) / kGroup * (DIGITS ? 4 : 2) * kGroup;
+  const uint32_t crowd = (a.tokens + kGroup - 1) / kGroup * kGroup;
   const bool two = kDownTmem<KIND, COLS> <= 256 &&
-                   kTwoPerSm - 1024 >= reserved + 3 * (kABytes + kPieces * columns * 128);
+                   kTwoPerSm - 1024 >= reserved + 3 * (kABytes + kPieces * columns * 128) &&
+                   kTwoPerSm - 1024 >= reserved + 2 * stage_most(crowd * kDownPlanes);
   const uint32_t smem = two ? kTwoPerSm : kOnePerSm;
   uint32_t at_once[9];
   rc = places_of<kDown>(device, kDownThreads<KIND>, smem, at_once);

@@ -406,6 +406,21 @@ def test_moe_decode_converted_weights_with_three_stages(engine, sizes):
     assert all(torch.equal(call(), first) for _ in range(20))
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("tokens", [16, 32, 57, 64])
+def test_moe_decode_one_of_many_experts_has_every_token(engine, tokens, int8):
+    """The lists of about a thousand experts and the columns of all tokens leave the least
+    room for stages; the average number of an expert's tokens says nothing of it."""
+    layer = big_layer(tokens, 1000, 2, 128, 1040, int8, seed=tokens)
+    layer["ids"][:, 0], layer["ids"][:, 1] = 777, -1
+    layer["ids"][::16, 1] = 3
+    want, bound = big_layer_oracle(layer)
+    got = engine.moe_decode(layer["x"], layer["w1"], layer["w2"], layer["ids"], layer["coef"],
+                            gate_up_scale=layer["s1"], down_scale=layer["s2"])
+    off = (got.double() - want).abs()
+    assert torch.all(off <= bound), (off / bound).max()
+
+
 @pytest.mark.parametrize("hidden,inter", [(8, 8), (24, 40), (72, 8), (1000, 56), (264, 1032)])
 def test_moe_decode_odd_multiples_of_eight(engine, hidden, inter):
     for tokens in (1, 6, 20):
