@@ -143,6 +143,14 @@ __device__ __forceinline__ void report(const DecodeArgs& a, uint32_t site) {
   if (a.status != nullptr) atomicCAS(a.status, 0u, 0x50000000u | site);
 }
 
+// A wait of this call, or of one before it that shares the status word, ran out: the result
+// is NaN rather than plausible. An epilogue whose own waits succeeded has all of its sums, so it
+// is the one that knows.
+__device__ __forceinline__ bool failed_before(const DecodeArgs& a) {
+  return a.status != nullptr && *a.status != 0;
+}
+__device__ __forceinline__ float not_a_number() { return __uint_as_float(0x7fc00000u); }
+
 // The signed bytes of `word` as BF16 pairs (bytes 0 and 1, 2 and 3), exact. With 128 + (b & 127)
 // as the bits 0x4300 | (b & 0x7f), and 128 or 256 as the bits 0x4300 | (b & 0x80), the signed value
 // is their difference: two masks, four byte permutations, two subtractions. (Masking the
@@ -537,6 +545,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
   const uint32_t columns = plane * kPlanes;
   const uint32_t n = (columns + 15) / 16 * 16;     // columns of the MMA
   const Ring<KIND> ring(base, ring_bytes, n);
+  bool spoiled = false;                    // epilogue: the sums of this thread's row
 
   const uint32_t rank = ptx::cluster_cta_rank(), ranks = ptx::cluster_cta_count();
   const uint32_t channel0 = blockIdx.x / ranks * 64;
@@ -651,6 +660,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
       if (!ok && lane == 0) report(a, 3);
     }
     // Accumulator -> shared memory [column][row], over the ring: all of its bytes are used.
+    spoiled = warp < 8 && failed_before(a);
     if (warp < 8 && ok && wait(bars.d_full[0], 0)) {
       ptx::tc_fence_after_sync();
       const uint32_t to = base + (quad * 32 + lane) * 4;
@@ -679,13 +689,22 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
         }
       }
       ptx::tc_fence_before_sync();
-    } else if (warp < 8 && lane == 0) {
-      report(a, 4);
+    } else if (warp < 8) {
+      spoiled = true;
+      if (lane == 0) report(a, 4);
     }
   }
   __syncwarp();
   if constexpr (DIGITS) ptx::wait_for_previous_grid();   // x_most; and see above
   settle(&abort_slot);
+  if (spoiled) {
+    // NaN in h, and from there in every output channel of the expert's tokens
+    for (uint32_t c = 0; c < plane; ++c) {
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + (c * kRows + (warp & 3) * 32 + lane) * 4),
+                   "f"(not_a_number())
+                   : "memory");
+    }
+  }
   if (ranks > 1) {
     ptx::cluster_sync();
   } else {
@@ -932,6 +951,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
     const uint32_t quad = warp & 3;
     const uint32_t row = quad * 32 + lane;
     float* const mine = sums + row;
+    bool spoiled = failed_before(a);
     Cursor d_buf;
     if constexpr (DIGITS) ptx::wait_for_previous_grid();   // h_most
     for (uint32_t at = begin; at < end;) {
@@ -947,6 +967,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
       }
       if (!wait(bars.d_full[d_buf.slot], d_buf.parity)) {
         if (lane == 0) report(a, 9);
+        spoiled = true;
         break;
       }
       ptx::tc_fence_after_sync();
@@ -982,6 +1003,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
       d_buf.next(2);
       at += run;
     }
+    for (uint32_t t = 0; spoiled && t < a.tokens; ++t) mine[t * kRows] = not_a_number();
   }
   __syncwarp();
   // No thread goes on before the first kernel has ended: out may be x, and this grid must

@@ -137,7 +137,7 @@ def moe_decode_workspace(tokens: int, top_k: int, inter: int) -> int:
 
 
 def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
-               down_scale=None, out=None, workspace=None, stream=None):
+               down_scale=None, out=None, workspace=None, status=None, stream=None):
     """A whole expert layer for up to 64 tokens.
 
     ``x`` BF16 [tokens, hidden]; ``w_gate_up`` [experts, 2 * inter, hidden] (gate rows, then
@@ -148,7 +148,11 @@ def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
     ``out[t] = sum_j weights[t, j] * (silu(x Wgate^T) * (x Wup^T)) Wdown^T``.
 
     ``workspace``: contiguous uint8 tensor of ``moe_decode_workspace`` bytes, for callers that
-    keep one; calls that may overlap need one each."""
+    keep one; calls that may overlap need one each.
+
+    ``status``: int32 tensor [1] that starts at zero and may serve many calls. Every wait inside
+    the kernels is bounded (one second); one that runs out leaves a non-zero word there, and NaN
+    in what could not be computed. A call that finds the word set makes all of ``out`` NaN."""
     if not x.is_cuda:
         raise ValueError("x: the engine has no CPU path, a CUDA tensor is needed")
     if x.dim() != 2 or w_gate_up.dim() != 3 or expert_ids.dim() != 2:
@@ -182,11 +186,13 @@ def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
                                     dtype=torch.uint8, device=x.device)
         else:
             _need(workspace, "workspace", torch.uint8, (workspace.numel(),), index)
-        status = _moe_decode(
+        if status is not None:
+            _need(status, "status", torch.int32, (1,), index)
+        result = _moe_decode(
             x.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(),
             gate_up_scale.data_ptr() if int8 else 0, down_scale.data_ptr() if int8 else 0,
             expert_ids.data_ptr(), weights.data_ptr(), out.data_ptr(), workspace.data_ptr(),
             workspace.numel(), tokens, top_k, experts, hidden, inter, _WEIGHT_TYPES[kind],
-            _current_raw_stream(index), 0)
-        _capi.check(status, "bmoe_moe_decode")
+            _current_raw_stream(index), 0 if status is None else status.data_ptr())
+        _capi.check(result, "bmoe_moe_decode")
     return out

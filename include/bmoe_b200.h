@@ -924,9 +924,11 @@ typedef struct bmoe_moe_decode_args {
   uint32_t inter;                 /* multiple of 8 (BF16 weights) or 16 (INT8) */
   uint32_t data_type;             /* of the weights: BMOE_TYPE_BF16 or BMOE_TYPE_INT8 */
   void* stream;
-  uint32_t* status_dev;           /* optional: 0x50000000 | site if a bounded wait inside a
-                                     launch ran out (out is then invalid); zeroed by the
-                                     caller */
+  uint32_t* status_dev;           /* optional, zeroed by the caller: 0x50000000 | site if a
+                                     bounded wait inside a launch ran out. What such a call
+                                     could not compute is NaN in out, with or without this
+                                     word. A call that finds the word set (layers that share
+                                     one) leaves it and makes all of out NaN */
 } bmoe_moe_decode_args;
 
 /* Workspace of a bmoe_moe_decode call in bytes. Calls that may overlap (two streams, two

@@ -539,6 +539,26 @@ def test_moe_decode_may_write_its_input_and_leaves_the_status_word_alone(engine)
     assert torch.equal(out, want) and status.item() == 0
 
 
+@pytest.mark.parametrize("sizes,int8", [
+    ((1, 8, 2, 512, 1024), False), ((9, 6, 2, 528, 96), True), ((40, 12, 3, 384, 320), False),
+    ((64, 3, 2, 160, 272), True), ((16, 8, 4, 1040, 1456), True)])
+def test_moe_decode_after_a_wait_that_ran_out(engine, sizes, int8):
+    """The status word reaches the caller, and a call that finds it set gives NaN everywhere: the
+    way a wait of its own that ran out would, without one."""
+    layer = make_layer(*sizes, int8, seed=sum(sizes))
+    want = run_layer(engine, layer)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert torch.equal(run_layer(engine, layer, status=status), want) and status.item() == 0
+    status.fill_(0x50000004)
+    got = run_layer(engine, layer, status=status)
+    assert torch.isnan(got).all() and status.item() == 0x50000004
+    status.zero_()
+    assert torch.equal(run_layer(engine, layer, status=status), want) and status.item() == 0
+    for bad in (status.float(), torch.zeros(2, dtype=torch.int32, device="cuda"), status.cpu()):
+        with pytest.raises(ValueError):
+            run_layer(engine, layer, status=bad)
+
+
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("tokens", [17, 33, 64])
 def test_moe_decode_sparse_and_spread_tokens(engine, tokens, int8):
