@@ -14,19 +14,27 @@ from __future__ import annotations
 import contextlib
 import functools
 
-import torch
-
 from . import _capi
 
-_ROW_TYPES = {torch.bfloat16: _capi.TYPE_BF16, torch.float32: _capi.TYPE_FP32}
-_WEIGHT_TYPES = {torch.bfloat16: _capi.TYPE_BF16, torch.int8: _capi.TYPE_INT8}
+# PyTorch and what is looked up in it, at the first call: the rest of the package works without
+torch = None
 _NO_GUARD = contextlib.nullcontext()
-# the current device, and the raw handle of its current stream without a Stream object
-_current_device = torch._C._cuda_getDevice
-_current_raw_stream = torch._C._cuda_getCurrentRawStream
 _route_topk = _capi.entry("bmoe_route_topk", _capi.RouteTopkArgs)
 _quantize_rows = _capi.entry("bmoe_quantize_rows", _capi.QuantizeRowsArgs)
 _moe_decode = _capi.entry("bmoe_moe_decode", _capi.MoeDecodeArgs)
+
+
+def _bind_torch() -> None:
+    global torch, _ROW_TYPES, _WEIGHT_TYPES, _current_device, _current_raw_stream
+    import torch as module
+
+    _ROW_TYPES = {module.bfloat16: _capi.TYPE_BF16, module.float32: _capi.TYPE_FP32}
+    _WEIGHT_TYPES = {module.bfloat16: _capi.TYPE_BF16, module.int8: _capi.TYPE_INT8}
+    # the current device, and the raw handle of its current stream without a Stream object (a
+    # build of PyTorch without CUDA has neither, nor tensors that get that far)
+    _current_device = getattr(module._C, "_cuda_getDevice", None)
+    _current_raw_stream = getattr(module._C, "_cuda_getCurrentRawStream", None)
+    torch = module
 
 
 def _on(index: int, stream):
@@ -80,6 +88,8 @@ def route_topk(logits, top_k: int, *, scoring: str = "softmax", renormalize: boo
     lower id. ``scoring`` "softmax" or "sigmoid"; ``bias`` [experts] float32 is added to a
     sigmoid score for the choice only; ``renormalize`` divides by the sum over the chosen.
     Experts at -inf or NaN are never chosen; a token left with fewer gets id -1, weight 0."""
+    if torch is None:
+        _bind_torch()
     tokens, experts, row_stride, index = _rows(logits, "logits")
     if scoring not in _capi.SCORINGS:
         raise ValueError(f"unknown scoring: {scoring}")
@@ -108,6 +118,8 @@ def quantize_rows(x, index=None, *, out=None, scale=None, stream=None):
     Returns ``(q int8, scale float32)`` with ``x[i] ~ q[i] * scale[i]``: the A operand and
     ``row_scale`` of an INT8 product. With ``index`` (int64) output row i is row
     ``index[i]``; an index outside ``x`` leaves its output row untouched."""
+    if torch is None:
+        _bind_torch()
     src_rows, cols, row_stride, device = _rows(x, "x")
     rows = src_rows
     if index is not None:
@@ -153,6 +165,8 @@ def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
     ``status``: int32 tensor [1] that starts at zero and may serve many calls. Every wait inside
     the kernels is bounded (one second); one that runs out leaves a non-zero word there, and NaN
     in what could not be computed. A call that finds the word set makes all of ``out`` NaN."""
+    if torch is None:
+        _bind_torch()
     if not x.is_cuda:
         raise ValueError("x: the engine has no CPU path, a CUDA tensor is needed")
     if x.dim() != 2 or w_gate_up.dim() != 3 or expert_ids.dim() != 2:

@@ -189,3 +189,47 @@ def test_packed_calls_reach_the_same_checks(engine):
             call(*(-1 if i == last else v for i, v in enumerate(fields)))
         with pytest.raises(ValueError):
             call(*fields[:-1])
+
+
+def run_alone(code):
+    """``code`` in an interpreter of its own, from the repository's root."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
+                          cwd=Path(__file__).resolve().parent.parent, timeout=300)
+    assert done.returncode == 0, done.stderr
+
+
+def test_the_package_imports_without_torch():
+    """Planner, C binding and CSV helpers never need it; the layer operators at their first call."""
+    run_alone("""
+import sys
+sys.modules["torch"] = None                      # import torch raises ModuleNotFoundError
+import bmoe_b200
+assert bmoe_b200.moe_decode_workspace(4, 2, 32) > 0
+assert bmoe_b200.host_tiles([5, 0, 9], 256, 128, 256)[1] == 2
+try:
+    bmoe_b200.route_topk(None, 2)
+except ModuleNotFoundError:
+    pass
+else:
+    raise AssertionError("no error")
+""")
+
+
+def test_the_package_imports_beside_a_torch_without_cuda():
+    run_alone("""
+import torch
+for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+import bmoe_b200
+try:
+    bmoe_b200.route_topk(torch.zeros(2, 8), 2)
+except ValueError:
+    pass
+else:
+    raise AssertionError("no error")
+""")
