@@ -3,10 +3,10 @@
 
 Thin wrappers of the C entry points (``include/bmoe_b200.h``, section 6). Each allocates the
 outputs it is not given, launches on ``stream`` (default: the current stream of the tensors'
-device) and does not synchronise; what it allocates belongs to that stream. Wrong shapes,
-types or devices raise ``ValueError``, a status of the engine raises ``EngineError``. The
-reference has no counterpart: routed token counts are its input
-(agent/search_space.yaml:10-13).
+device) and does not synchronise; what it allocates belongs to that stream. There is no backward
+pass: with gradients enabled, inputs that require one are refused. Wrong shapes, types or
+devices raise ``ValueError``, a status of the engine raises ``EngineError``. The reference has
+no counterpart: routed token counts are its input (agent/search_space.yaml:10-13).
 """
 
 from __future__ import annotations
@@ -52,6 +52,15 @@ def _on(index: int, stream):
     return torch.cuda.stream(stream)
 
 
+def _forward_only(*tensors) -> None:
+    """The operators have no backward pass: a result that should carry a gradient is refused."""
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                raise ValueError("no backward pass: detach what requires a gradient, or call "
+                                 "under torch.no_grad()")
+
+
 def _is(x, dtype, shape, index: int) -> bool:
     """``x`` is a contiguous tensor of that type and shape on CUDA device ``index``."""
     return (x.dtype is dtype and x.shape == shape and x.get_device() == index
@@ -90,6 +99,7 @@ def route_topk(logits, top_k: int, *, scoring: str = "softmax", renormalize: boo
     Experts at -inf or NaN are never chosen; a token left with fewer gets id -1, weight 0."""
     if torch is None:
         _bind_torch()
+    _forward_only(logits, bias)
     tokens, experts, row_stride, index = _rows(logits, "logits")
     if scoring not in _capi.SCORINGS:
         raise ValueError(f"unknown scoring: {scoring}")
@@ -120,6 +130,7 @@ def quantize_rows(x, index=None, *, out=None, scale=None, stream=None):
     ``index[i]``; an index outside ``x`` leaves its output row untouched."""
     if torch is None:
         _bind_torch()
+    _forward_only(x)
     src_rows, cols, row_stride, device = _rows(x, "x")
     rows = src_rows
     if index is not None:
@@ -167,6 +178,7 @@ def moe_decode(x, w_gate_up, w_down, expert_ids, weights, *, gate_up_scale=None,
     in what could not be computed. A call that finds the word set makes all of ``out`` NaN."""
     if torch is None:
         _bind_torch()
+    _forward_only(x, w_gate_up, w_down, weights, gate_up_scale, down_scale)
     if not x.is_cuda:
         raise ValueError("x: the engine has no CPU path, a CUDA tensor is needed")
     if x.dim() != 2 or w_gate_up.dim() != 3 or expert_ids.dim() != 2:

@@ -191,6 +191,31 @@ def test_packed_calls_reach_the_same_checks(engine):
             call(*fields[:-1])
 
 
+def test_inputs_that_require_a_gradient_are_refused(engine):
+    """There is no backward pass, so a result cut off from the graph would be a silent zero."""
+    import torch
+
+    def leaf(*shape):
+        return torch.zeros(*shape, requires_grad=True)
+
+    x, w1, w2 = torch.zeros(2, 16), torch.zeros(4, 32, 16), torch.zeros(4, 16, 16)
+    ids, coef = torch.zeros(2, 2, dtype=torch.int64), torch.zeros(2, 2)
+    calls = (lambda: engine.route_topk(leaf(2, 8), 2),
+             lambda: engine.route_topk(torch.zeros(2, 8), 2, scoring="sigmoid", bias=leaf(8)),
+             lambda: engine.quantize_rows(leaf(2, 16)),
+             lambda: engine.moe_decode(leaf(2, 16), w1, w2, ids, coef),
+             lambda: engine.moe_decode(x, leaf(4, 32, 16), w2, ids, coef),
+             lambda: engine.moe_decode(x, w1, leaf(4, 16, 16), ids, coef),
+             lambda: engine.moe_decode(x, w1, w2, ids, leaf(2, 2)),
+             lambda: engine.moe_decode(x, w1, w2, ids, coef, gate_up_scale=leaf(4, 32)),
+             lambda: engine.moe_decode(x, w1, w2, ids, coef, down_scale=leaf(4, 16)))
+    for call in calls:
+        with pytest.raises(ValueError, match="backward"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="no CPU path"):
+            call()
+
+
 def run_alone(code):
     """``code`` in an interpreter of its own, from the repository's root."""
     import subprocess
