@@ -4,9 +4,9 @@
 // checks, policy resolution, host encoding of one TMA descriptor triple per
 // active expert, ONE asynchronous copy (from pinned staging memory) of counts,
 // descriptors, queue and status words, and the on-device worklist build. It
-// enqueues on the plan's stream and does not wait for the device; a plan must
-// not be re-initialised while launches of it are still in flight on ANOTHER
-// stream. run() is a single kernel launch. Behavioural contract
+// enqueues on the plan's stream and does not wait for the device. run() is a single
+// kernel launch. Set-ups and launches of one plan share its device storage, so they run in
+// the order of the calls, also where these name different streams. Behavioural contract
 // (status codes, null / zero handling, stream override) follows
 // baselines/cutlass/cutlass_baseline.cu:195-377 of the reference.
 #include <cuda.h>
@@ -96,6 +96,12 @@ struct bmoe_plan {
     cudaEvent_t done = nullptr;
   } setup[2];
   uint32_t turn = 0;   // the area of the current plan
+
+  // The last set-up or launch that was enqueued. One on another stream waits for it: a
+  // set-up overwrites what launches read, and launches share the queue words. Streams are
+  // told apart by their ids: a handle may come back after its stream was destroyed.
+  cudaEvent_t used = nullptr;
+  unsigned long long used_on = 0;
   DeviceBlock worklist;   // bmoe_tile [capacity]
   DeviceBlock workspace;  // worklist builder arrays
 
@@ -121,6 +127,8 @@ struct bmoe_plan {
       if (s.done != nullptr) cudaEventDestroy(s.done);
       s.done = nullptr;
     }
+    if (used != nullptr) cudaEventDestroy(used);
+    used = nullptr;
     b_encoded_for.clear();
     worklist.release();
     workspace.release();
@@ -202,6 +210,37 @@ Resolved resolve_policy(const bmoe_gemm_args& a, uint32_t tile_m, uint32_t tile_
 }
 
 }  // namespace
+
+// Before and after work of the plan is enqueued on `stream`. A stream that is being captured
+// cannot wait for work outside of its graph; there the host waits. (Asking such a stream for its
+// id ends the capture.)
+static bool capturing(cudaStream_t stream, bool* yes) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) return false;
+  *yes = capture != cudaStreamCaptureStatusNone;
+  return true;
+}
+
+static bool follow(bmoe_plan* plan, cudaStream_t stream) {
+  bool captured = false;
+  if (!capturing(stream, &captured)) return false;
+  if (plan->used == nullptr &&
+      cudaEventCreateWithFlags(&plan->used, cudaEventDisableTiming) != cudaSuccess) {
+    return false;
+  }
+  if (captured) return cudaEventSynchronize(plan->used) == cudaSuccess;
+  unsigned long long id = 0;
+  if (cudaStreamGetId(stream, &id) != cudaSuccess) return false;
+  return plan->used_on == id || cudaStreamWaitEvent(stream, plan->used, 0) == cudaSuccess;
+}
+
+static bool leave(bmoe_plan* plan, cudaStream_t stream) {
+  bool captured = false;
+  if (!capturing(stream, &captured)) return false;
+  if (captured) return true;
+  return cudaStreamGetId(stream, &plan->used_on) == cudaSuccess &&
+         cudaEventRecord(plan->used, stream) == cudaSuccess;
+}
 
 extern "C" {
 
@@ -296,10 +335,7 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
   }
   if (packed && !dev_counts && routed_rows > a.packed_rows) return BMOE_INVALID_ARGUMENT;
   plan->stats.active_experts = active;
-  const cudaStream_t previous_stream = plan->setup_stream;
   plan->default_stream = static_cast<cudaStream_t>(a.stream);
-  plan->setup_stream = plan->default_stream;
-  plan->last_stream = plan->default_stream;
   if (active == 0) {
     // A routing result without active experts is valid and launches nothing.
     plan->ready = true;
@@ -375,20 +411,10 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
   const size_t off_scales = off_maps + map_bytes;
   const size_t meta_bytes =
       off_scales + (int8 ? 2 * sizeof(float*) * static_cast<size_t>(a.experts) : 0);
-  bmoe_plan::Setup& before = plan->setup[plan->turn];
+  const cudaStream_t stream = plan->default_stream;
+  if (!follow(plan, stream)) return BMOE_CUDA_ERROR;
   plan->turn ^= 1u;
   bmoe_plan::Setup& setup = plan->setup[plan->turn];
-  // On another stream than the last set-up, this one follows it. A stream that is being
-  // captured cannot wait for work outside of its graph; there the host waits.
-  if (before.done != nullptr && previous_stream != plan->setup_stream) {
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(plan->setup_stream, &capture) != cudaSuccess ||
-        (capture == cudaStreamCaptureStatusNone
-             ? cudaStreamWaitEvent(plan->setup_stream, before.done, 0)
-             : cudaEventSynchronize(before.done)) != cudaSuccess) {
-      return BMOE_CUDA_ERROR;
-    }
-  }
   if (setup.done == nullptr) {
     if (cudaEventCreateWithFlags(&setup.done, cudaEventDisableTiming) != cudaSuccess) {
       return BMOE_CUDA_ERROR;
@@ -402,7 +428,6 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
       !plan->workspace.reserve(layout.bytes)) {
     return BMOE_CUDA_ERROR;
   }
-  const cudaStream_t stream = plan->setup_stream;
   uint8_t* const stage = static_cast<uint8_t*>(setup.staging.ptr);
   uint8_t* const meta = static_cast<uint8_t*>(plan->meta.ptr);
 
@@ -490,13 +515,15 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
   request.tile_n = tile_n;
   request.order = policy.order;
   request.raster = raster;
-  int rc = bmoe_worklist_build(dev_counts ? a.tokens_per_expert_dev
-                                          : reinterpret_cast<const uint32_t*>(meta + off_counts),
-                               &request,
-                               static_cast<bmoe_tile*>(plan->worklist.ptr), tiles,
-                               plan->workspace.ptr, stream);
+  const int rc = bmoe_worklist_build(
+      dev_counts ? a.tokens_per_expert_dev : reinterpret_cast<const uint32_t*>(meta + off_counts),
+      &request, static_cast<bmoe_tile*>(plan->worklist.ptr), tiles, plan->workspace.ptr, stream);
+  plan->setup_stream = stream;
+  plan->last_stream = stream;
+  if (cudaEventRecord(setup.done, stream) != cudaSuccess || !leave(plan, stream)) {
+    return BMOE_CUDA_ERROR;
+  }
   if (rc != BMOE_OK) return rc;
-  if (cudaEventRecord(setup.done, stream) != cudaSuccess) return BMOE_CUDA_ERROR;
 
   // ---- launch parameters ----
   const CUtensorMap* const dev_maps = reinterpret_cast<const CUtensorMap*>(meta + off_maps);
@@ -674,15 +701,12 @@ int bmoe_plan_run(bmoe_plan* plan, void* stream) {
   if (plan->needs_push && plan->params.push_origin == nullptr) return BMOE_INVALID_ARGUMENT;
   cudaStream_t s = stream == nullptr ? plan->default_stream
                                      : static_cast<cudaStream_t>(stream);
-  if (s != plan->setup_stream &&
-      cudaStreamWaitEvent(s, plan->setup[plan->turn].done, 0) != cudaSuccess) {
-    return BMOE_CUDA_ERROR;
-  }
+  if (!follow(plan, s)) return BMOE_CUDA_ERROR;
   const cudaError_t err =
       bmoe::launch_grouped_gemm(plan->params, plan->tile_n, plan->cta_group, plan->out_f32,
                                 plan->int8, plan->units, s);
   plan->last_stream = s;
-  if (err != cudaSuccess) return BMOE_CUDA_ERROR;
+  if (err != cudaSuccess || !leave(plan, s)) return BMOE_CUDA_ERROR;
   plan->stats.launches += 1;
   return BMOE_OK;
 }

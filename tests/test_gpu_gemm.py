@@ -272,6 +272,78 @@ def test_plan_is_reusable_and_reinitialisable(engine, oracle):
         plan.close()
 
 
+def test_plan_keeps_the_order_of_its_calls_across_streams(engine, oracle):
+    """One plan, two streams, work of the first still pending: set-ups and launches share the
+    plan's device storage and must not overtake each other."""
+    import torch
+
+    problems = []
+    for counts, n, k, seed in (([37, 0, 1, 200], 384, 192, 1), ([90, 5, 260, 31], 256, 320, 2)):
+        a, w = make_inputs(counts, n, k, seed)
+        problems.append((a, w, counts, a.cuda(), w.cuda(),
+                         torch.empty(sum(counts), n, dtype=torch.bfloat16, device="cuda")))
+    first, second = problems
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    plan = engine.GroupedGemmPlan()
+
+    def fresh():
+        torch.cuda.synchronize()
+        for problem in problems:
+            problem[5].fill_(float("nan"))
+        torch.cuda.synchronize()
+
+    def busy(stream):
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(40_000_000)
+
+    def set_up(problem, stream, counts=None, **options):
+        return plan.initialize_packed(problem[3], problem[4], problem[5],
+                                      problem[2] if counts is None else counts, stream=stream,
+                                      **options)
+
+    def check(problem):
+        check_against_oracle(oracle, problem[0], problem[1], problem[2], bits_of(problem[5]))
+
+    try:
+        for scheduler in ("expert_order", "dynamic_queue"):
+            fresh()                                    # set-up behind a pending launch
+            busy(one)
+            assert set_up(first, one, scheduler=scheduler) == 0 and plan.run(one) == 0
+            assert set_up(second, two, scheduler=scheduler) == 0 and plan.run(two) == 0
+            torch.cuda.synchronize()
+            check(first), check(second)
+            assert plan.poll()[0] == 0
+
+            fresh()                                    # the same with the launch elsewhere
+            assert set_up(first, one, scheduler=scheduler) == 0
+            busy(two)
+            assert plan.run(two) == 0
+            assert set_up(second, one, scheduler=scheduler) == 0 and plan.run(one) == 0
+            torch.cuda.synchronize()
+            check(first), check(second)
+
+            fresh()                                    # a pending set-up, two that enqueue nothing
+            busy(one)
+            assert set_up(first, one, scheduler=scheduler) == 0
+            assert set_up(second, two, counts=[0, 0, 0, 0]) == 0 and plan.run(two) == 0
+            assert set_up(second, two, tile_n=32) == engine._capi.INVALID_ARGUMENT
+            assert set_up(second, two, scheduler=scheduler) == 0 and plan.run(two) == 0
+            assert plan.poll()[0] == 0
+            check(second)
+            assert torch.isnan(first[5]).all()
+
+            fresh()                                    # launches of one set-up on both
+            assert set_up(second, one, scheduler=scheduler) == 0
+            busy(one)
+            assert all(plan.run(stream) == 0 for stream in (one, two, None, two, one))
+            torch.cuda.synchronize()
+            check(second)
+            assert plan.poll()[0] == 0
+    finally:
+        torch.cuda.synchronize()
+        plan.close()
+
+
 def test_benchmark_shape_properties(engine, oracle, golden):
     """Full-size Mixtral-shaped case: policies bit-identical, sampled rows within
     tolerance of the oracle, every tile run exactly once."""
