@@ -6,7 +6,8 @@
 // descriptors, queue and status words, and the on-device worklist build. It
 // enqueues on the plan's stream and does not wait for the device. run() is a single
 // kernel launch. Set-ups and launches of one plan share its device storage, so they run in
-// the order of the calls, also where these name different streams. Behavioural contract
+// the order of the calls, also where these name different streams. Both can be captured:
+// storage that a graph reads is the graph's from then on. Behavioural contract
 // (status codes, null / zero handling, stream override) follows
 // baselines/cutlass/cutlass_baseline.cu:195-377 of the reference.
 #include <cuda.h>
@@ -16,7 +17,9 @@
 #include <cstdint>
 #include <cstring>
 #include <exception>
+#include <memory>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "blackwell_moe/dispatch.hpp"
@@ -76,14 +79,45 @@ bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u)
 
 }  // namespace
 
-struct bmoe_plan {
-  bool ready = false;
-  bmoe_plan_stats stats{};
-  cudaStream_t default_stream = nullptr;
-  cudaStream_t setup_stream = nullptr;
-  cudaStream_t last_stream = nullptr;
-  int device = -1;
+namespace {
 
+// Where a call enqueues its work: a stream, or one of the streams of a capture. Streams are
+// told apart by their ids (a handle may come back after its stream was destroyed), those of one
+// capture by their handles (asking one for its id ends the capture).
+struct Site {
+  unsigned long long capture = 0;   // 0: none
+  unsigned long long stream = 0;
+  bool find(cudaStream_t s) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(s, &status, &id) != cudaSuccess) return false;
+    if (status == cudaStreamCaptureStatusNone) return cudaStreamGetId(s, &stream) == cudaSuccess;
+    capture = id + 1;
+    stream = reinterpret_cast<uintptr_t>(s);
+    return status == cudaStreamCaptureStatusActive;
+  }
+};
+
+// Allocations, and waits for work outside of the graph, beside a stream of this thread that is
+// being captured: they are not meant to become part of it.
+class BesideCapture {
+ public:
+  explicit BesideCapture(bool captured) : captured_(captured) {
+    if (captured_) cudaThreadExchangeStreamCaptureMode(&mode_);
+  }
+  ~BesideCapture() {
+    if (captured_) cudaThreadExchangeStreamCaptureMode(&mode_);
+  }
+  BesideCapture(const BesideCapture&) = delete;
+  BesideCapture& operator=(const BesideCapture&) = delete;
+
+ private:
+  bool captured_;
+  cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+};
+
+// What a set-up fills and the launches behind it read.
+struct Storage {
   // One metadata block, filled by a single copy from pinned staging memory:
   //   [0, 256) queue words   [256, 512) DeviceStatus
   //   [512, ...) counts uint32 [experts]   then CUtensorMap [3][experts] (128-aligned)
@@ -95,15 +129,83 @@ struct bmoe_plan {
     PinnedBlock staging;
     cudaEvent_t done = nullptr;
   } setup[2];
-  uint32_t turn = 0;   // the area of the current plan
-
-  // The last set-up or launch that was enqueued. One on another stream waits for it: a
-  // set-up overwrites what launches read, and launches share the queue words. Streams are
-  // told apart by their ids: a handle may come back after its stream was destroyed.
-  cudaEvent_t used = nullptr;
-  unsigned long long used_on = 0;
+  uint32_t turn = 0;      // the area of the current set-up
   DeviceBlock worklist;   // bmoe_tile [capacity]
   DeviceBlock workspace;  // worklist builder arrays
+
+  bool of_graph = false;  // a captured set-up or launch refers to it
+
+  // The last set-up or launch that was enqueued (its event, and where). One elsewhere waits
+  // for it: a set-up overwrites what launches read, and launches share the queue words.
+  cudaEvent_t launched[2] = {nullptr, nullptr};   // outside of captures / inside
+  cudaEvent_t used = nullptr;
+  Site used_at;
+
+  Storage() = default;
+  Storage(const Storage&) = delete;
+  Storage& operator=(const Storage&) = delete;
+  ~Storage() {
+    meta.release();
+    worklist.release();
+    workspace.release();
+    for (Setup& s : setup) {
+      s.staging.release();
+      if (s.done != nullptr) cudaEventDestroy(s.done);
+    }
+    for (cudaEvent_t event : launched) {
+      if (event != nullptr) cudaEventDestroy(event);
+    }
+  }
+
+  // Before work is enqueued on `stream`. A capture cannot wait for work outside of it, so the
+  // host does; work of another graph runs when that is replayed, which the caller orders.
+  bool follow(cudaStream_t stream, const Site& at) const {
+    if (used == nullptr) return true;
+    if (used_at.capture == at.capture) {
+      return used_at.stream == at.stream || cudaStreamWaitEvent(stream, used, 0) == cudaSuccess;
+    }
+    if (used_at.capture != 0) return true;
+    const BesideCapture guard(true);
+    return cudaEventSynchronize(used) == cudaSuccess;
+  }
+  // After it.
+  bool leave(cudaStream_t stream, const Site& at, cudaEvent_t& event) {
+    if (event == nullptr &&
+        cudaEventCreateWithFlags(&event, cudaEventDisableTiming) != cudaSuccess) {
+      return false;
+    }
+    used = event;
+    used_at = at;
+    return cudaEventRecord(event, stream) == cudaSuccess;
+  }
+};
+
+}  // namespace
+
+struct bmoe_plan {
+  bool ready = false;
+  bmoe_plan_stats stats{};
+  cudaStream_t default_stream = nullptr;
+  cudaStream_t setup_stream = nullptr;
+  cudaStream_t last_stream = nullptr;
+  int device = -1;
+
+  std::unique_ptr<Storage> storage;   // of the current set-up
+  std::unique_ptr<Storage> spare;     // of those outside of captures, while a graph's is current
+  std::vector<std::unique_ptr<Storage>> of_graphs;   // earlier ones that graphs refer to
+
+  // Storage for a set-up: a graph's is left to the graph, a captured set-up gets one of its own.
+  Storage* next_storage(bool captured) {
+    if (storage != nullptr && storage->of_graph) {
+      of_graphs.push_back(std::move(storage));
+    } else if (storage != nullptr && captured) {
+      spare = std::move(storage);
+    }
+    if (storage == nullptr && !captured) storage = std::move(spare);
+    if (storage == nullptr) storage.reset(new Storage);
+    storage->of_graph = captured;
+    return storage.get();
+  }
 
   // B descriptors and what they were encoded for (reused while the expert's weight pointer,
   // the shape and the box do not change).
@@ -120,19 +222,14 @@ struct bmoe_plan {
   bool out_f32 = false;
   bool int8 = false;
 
-  void release_all() {
-    meta.release();
-    for (Setup& s : setup) {
-      s.staging.release();
-      if (s.done != nullptr) cudaEventDestroy(s.done);
-      s.done = nullptr;
-    }
-    if (used != nullptr) cudaEventDestroy(used);
-    used = nullptr;
+  // Storage and descriptors belong to a device; what graphs refer to stays.
+  void change_device(int to) {
+    if (storage != nullptr && storage->of_graph) of_graphs.push_back(std::move(storage));
+    storage.reset();
+    spare.reset();
     b_encoded_for.clear();
-    worklist.release();
-    workspace.release();
     ready = false;
+    device = to;
   }
 };
 
@@ -211,35 +308,23 @@ Resolved resolve_policy(const bmoe_gemm_args& a, uint32_t tile_m, uint32_t tile_
 
 }  // namespace
 
-// Before and after work of the plan is enqueued on `stream`. A stream that is being captured
-// cannot wait for work outside of its graph; there the host waits. (Asking such a stream for its
-// id ends the capture.)
-static bool capturing(cudaStream_t stream, bool* yes) {
-  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) return false;
-  *yes = capture != cudaStreamCaptureStatusNone;
-  return true;
-}
-
-static bool follow(bmoe_plan* plan, cudaStream_t stream) {
-  bool captured = false;
-  if (!capturing(stream, &captured)) return false;
-  if (plan->used == nullptr &&
-      cudaEventCreateWithFlags(&plan->used, cudaEventDisableTiming) != cudaSuccess) {
-    return false;
+// The set-up of a captured plan, once outside of the graph: a plan is ready for a launch or a
+// poll from the start, not from the first replay on. With counts that only the device knows
+// (counts_dev null) there are no tiles until then.
+static bool set_up_now(const Storage& st, size_t meta_bytes, const uint32_t* counts_dev,
+                       const bmoe_worklist_request& request, uint32_t tiles) {
+  cudaStream_t stream = nullptr;
+  if (cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking) != cudaSuccess) return false;
+  bool ok = cudaMemcpyAsync(st.meta.ptr, st.setup[st.turn].staging.ptr, meta_bytes,
+                            cudaMemcpyHostToDevice, stream) == cudaSuccess;
+  if (counts_dev != nullptr) {
+    ok = ok && bmoe_worklist_build(counts_dev, &request, static_cast<bmoe_tile*>(st.worklist.ptr),
+                                   tiles, st.workspace.ptr, stream) == BMOE_OK;
+  } else {
+    ok = ok && cudaMemsetAsync(st.workspace.ptr, 0, st.workspace.bytes, stream) == cudaSuccess;
   }
-  if (captured) return cudaEventSynchronize(plan->used) == cudaSuccess;
-  unsigned long long id = 0;
-  if (cudaStreamGetId(stream, &id) != cudaSuccess) return false;
-  return plan->used_on == id || cudaStreamWaitEvent(stream, plan->used, 0) == cudaSuccess;
-}
-
-static bool leave(bmoe_plan* plan, cudaStream_t stream) {
-  bool captured = false;
-  if (!capturing(stream, &captured)) return false;
-  if (captured) return true;
-  return cudaStreamGetId(stream, &plan->used_on) == cudaSuccess &&
-         cudaEventRecord(plan->used, stream) == cudaSuccess;
+  ok = cudaStreamSynchronize(stream) == cudaSuccess && ok;
+  return cudaStreamDestroy(stream) == cudaSuccess && ok;
 }
 
 extern "C" {
@@ -248,7 +333,6 @@ bmoe_plan* bmoe_plan_create(void) { return new (std::nothrow) bmoe_plan; }
 
 void bmoe_plan_destroy(bmoe_plan* plan) {
   if (plan == nullptr) return;
-  plan->release_all();
   delete plan;
 }
 
@@ -309,10 +393,7 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
   }
   // The kernels are built for sm_100a only (tcgen05, TMEM).
   if (major != 10 || minor != 0) return BMOE_UNSUPPORTED_DEVICE;
-  if (plan->device != device) {
-    plan->release_all();
-    plan->device = device;
-  }
+  if (plan->device != device) plan->change_device(device);
 
   uint32_t active = 0;
   uint64_t routed_rows = 0;
@@ -412,9 +493,14 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
   const size_t meta_bytes =
       off_scales + (int8 ? 2 * sizeof(float*) * static_cast<size_t>(a.experts) : 0);
   const cudaStream_t stream = plan->default_stream;
-  if (!follow(plan, stream)) return BMOE_CUDA_ERROR;
-  plan->turn ^= 1u;
-  bmoe_plan::Setup& setup = plan->setup[plan->turn];
+  Site at;
+  if (!at.find(stream)) return BMOE_CUDA_ERROR;
+  const bool captured = at.capture != 0;
+  const BesideCapture guard(captured);
+  Storage* const storage = plan->next_storage(captured);
+  if (!storage->follow(stream, at)) return BMOE_CUDA_ERROR;
+  storage->turn ^= 1u;
+  Storage::Setup& setup = storage->setup[storage->turn];
   if (setup.done == nullptr) {
     if (cudaEventCreateWithFlags(&setup.done, cudaEventDisableTiming) != cudaSuccess) {
       return BMOE_CUDA_ERROR;
@@ -423,13 +509,13 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
     // the copy of the set-up before the last one still reads this staging area
     return BMOE_CUDA_ERROR;
   }
-  if (!plan->meta.reserve(meta_bytes) || !setup.staging.reserve(meta_bytes) ||
-      !plan->worklist.reserve(sizeof(bmoe_tile) * static_cast<size_t>(tiles)) ||
-      !plan->workspace.reserve(layout.bytes)) {
+  if (!storage->meta.reserve(meta_bytes) || !setup.staging.reserve(meta_bytes) ||
+      !storage->worklist.reserve(sizeof(bmoe_tile) * static_cast<size_t>(tiles)) ||
+      !storage->workspace.reserve(layout.bytes)) {
     return BMOE_CUDA_ERROR;
   }
   uint8_t* const stage = static_cast<uint8_t*>(setup.staging.ptr);
-  uint8_t* const meta = static_cast<uint8_t*>(plan->meta.ptr);
+  uint8_t* const meta = static_cast<uint8_t*>(storage->meta.ptr);
 
   // ---- queue and status words, counts, one TMA descriptor triple per active expert ----
   const uint32_t tail = policy.tail_tiles < tiles ? policy.tail_tiles : tiles;
@@ -515,15 +601,18 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
   request.tile_n = tile_n;
   request.order = policy.order;
   request.raster = raster;
-  const int rc = bmoe_worklist_build(
-      dev_counts ? a.tokens_per_expert_dev : reinterpret_cast<const uint32_t*>(meta + off_counts),
-      &request, static_cast<bmoe_tile*>(plan->worklist.ptr), tiles, plan->workspace.ptr, stream);
+  const uint32_t* const host_counts_dev = reinterpret_cast<const uint32_t*>(meta + off_counts);
+  const int rc = bmoe_worklist_build(dev_counts ? a.tokens_per_expert_dev : host_counts_dev,
+                                     &request, static_cast<bmoe_tile*>(storage->worklist.ptr),
+                                     tiles, storage->workspace.ptr, stream);
   plan->setup_stream = stream;
   plan->last_stream = stream;
-  if (cudaEventRecord(setup.done, stream) != cudaSuccess || !leave(plan, stream)) {
+  if (!storage->leave(stream, at, setup.done)) return BMOE_CUDA_ERROR;
+  if (rc != BMOE_OK) return rc;
+  if (captured &&
+      !set_up_now(*storage, meta_bytes, dev_counts ? nullptr : host_counts_dev, request, tiles)) {
     return BMOE_CUDA_ERROR;
   }
-  if (rc != BMOE_OK) return rc;
 
   // ---- launch parameters ----
   const CUtensorMap* const dev_maps = reinterpret_cast<const CUtensorMap*>(meta + off_maps);
@@ -532,7 +621,7 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
   p.tmap_a = dev_maps;
   p.tmap_b = dev_maps + a.experts;
   p.tmap_d = dev_maps + 2 * static_cast<size_t>(a.experts);
-  p.tiles = static_cast<const bmoe_tile*>(plan->worklist.ptr);
+  p.tiles = static_cast<const bmoe_tile*>(storage->worklist.ptr);
   p.tile_count = tiles;
   p.k_blocks = bytes ? (a.k + 127) / 128 : (a.k + 63) / 64;   // 128 bytes of a row each
   p.byte_operands = bytes ? 1u : 0u;
@@ -559,12 +648,12 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
   if (packed) {
     // first row of every expert in the packed buffer, as the worklist builder left it
     p.a_row_offsets = reinterpret_cast<const unsigned long long*>(
-        static_cast<const uint8_t*>(plan->workspace.ptr) + layout.off_row_offsets);
+        static_cast<const uint8_t*>(storage->workspace.ptr) + layout.off_row_offsets);
   }
   plan->needs_push = pushed;
   if (dev_counts) {
     p.tile_count_dev = reinterpret_cast<const uint32_t*>(
-        static_cast<const uint8_t*>(plan->workspace.ptr) + layout.off_totals +
+        static_cast<const uint8_t*>(storage->workspace.ptr) + layout.off_totals +
         offsetof(bmoe_worklist_totals, total_tiles));
   }
 
@@ -578,7 +667,7 @@ static int initialize_plan(bmoe_plan* plan, const bmoe_gemm_args* args) {
 
   plan->stats.threadblock_count = plan->units * cta_group;
   plan->stats.workspace_bytes =
-      plan->meta.bytes + plan->worklist.bytes + plan->workspace.bytes;
+      storage->meta.bytes + storage->worklist.bytes + storage->workspace.bytes;
   plan->stats.total_tiles = tiles;
   plan->stats.tile_m = tile_m;
   plan->stats.tile_n = tile_n;
@@ -701,12 +790,18 @@ int bmoe_plan_run(bmoe_plan* plan, void* stream) {
   if (plan->needs_push && plan->params.push_origin == nullptr) return BMOE_INVALID_ARGUMENT;
   cudaStream_t s = stream == nullptr ? plan->default_stream
                                      : static_cast<cudaStream_t>(stream);
-  if (!follow(plan, s)) return BMOE_CUDA_ERROR;
+  Storage& storage = *plan->storage;
+  Site at;
+  if (!at.find(s) || !storage.follow(s, at)) return BMOE_CUDA_ERROR;
+  const bool captured = at.capture != 0;
+  storage.of_graph = storage.of_graph || captured;
   const cudaError_t err =
       bmoe::launch_grouped_gemm(plan->params, plan->tile_n, plan->cta_group, plan->out_f32,
                                 plan->int8, plan->units, s);
   plan->last_stream = s;
-  if (err != cudaSuccess || !leave(plan, s)) return BMOE_CUDA_ERROR;
+  if (err != cudaSuccess || !storage.leave(s, at, storage.launched[captured ? 1 : 0])) {
+    return BMOE_CUDA_ERROR;
+  }
   plan->stats.launches += 1;
   return BMOE_OK;
 }
@@ -741,7 +836,7 @@ int bmoe_plan_poll(bmoe_plan* plan, bmoe_device_report* report) {
   uint32_t control_init[128];
   std::memset(control_init, 0, sizeof(control_init));
   control_init[1] = plan->params.main_end;
-  cudaMemcpy(plan->meta.ptr, control_init, sizeof(control_init), cudaMemcpyHostToDevice);
+  cudaMemcpy(plan->storage->meta.ptr, control_init, sizeof(control_init), cudaMemcpyHostToDevice);
   return BMOE_DEVICE_TIMEOUT;
 }
 
@@ -754,7 +849,7 @@ int bmoe_plan_read_worklist(bmoe_plan* plan, bmoe_tile* tiles_host, uint32_t cap
   if (n_copy == 0) return BMOE_OK;
   if (tiles_host == nullptr) return BMOE_INVALID_ARGUMENT;
   if (cudaStreamSynchronize(plan->setup_stream) != cudaSuccess) return BMOE_CUDA_ERROR;
-  return cudaMemcpy(tiles_host, plan->worklist.ptr, sizeof(bmoe_tile) * n_copy,
+  return cudaMemcpy(tiles_host, plan->storage->worklist.ptr, sizeof(bmoe_tile) * n_copy,
                     cudaMemcpyDeviceToHost) == cudaSuccess
              ? BMOE_OK
              : BMOE_CUDA_ERROR;

@@ -87,7 +87,12 @@ def _expert_pointers(per_expert) -> np.ndarray:
 
 
 class GroupedGemmPlan:
-    """Reusable launch plan for ``D_e = A_e @ B_e^T`` over routed experts."""
+    """Reusable launch plan for ``D_e = A_e @ B_e^T`` over routed experts.
+
+    Set-ups and launches take effect in the order of the calls, on any streams, and can be
+    captured into CUDA graphs; a graph keeps what it refers to, until the plan is closed, and
+    the plan can be set up again meanwhile. The tensors of a captured set-up are the caller's
+    to keep."""
 
     def __init__(self) -> None:
         self._lib = _capi.load()

@@ -423,6 +423,13 @@ typedef struct bmoe_plan bmoe_plan;
 bmoe_plan* bmoe_plan_create(void);
 void bmoe_plan_destroy(bmoe_plan* plan);
 int bmoe_plan_initialize(bmoe_plan* plan, const bmoe_gemm_args* args);
+/* Set-ups and launches of a plan take effect in the order of the calls, also on different
+ * streams (a launch waits for the one before it then). Both can be captured into a CUDA graph,
+ * set-up and launch together or the launch alone. The storage that a graph refers to is the
+ * graph's: later set-ups take other storage, and the graph replays what was captured (the same
+ * pointers; the same counts, or those in tokens_per_expert_dev at the replay) until the plan is
+ * destroyed, which also is when that storage is freed. Replays against each other and against
+ * launches of the set-up they contain are ordered by the caller. */
 int bmoe_plan_run(bmoe_plan* plan, void* stream);
 int bmoe_plan_stats_get(const bmoe_plan* plan, bmoe_plan_stats* out);
 

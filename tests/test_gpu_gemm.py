@@ -344,6 +344,182 @@ def test_plan_keeps_the_order_of_its_calls_across_streams(engine, oracle):
         plan.close()
 
 
+def graph_problem(counts, n, k, seed):
+    import torch
+
+    a, w = make_inputs(counts, n, k, seed)
+    return {"a": a, "w": w, "counts": counts, "a_dev": a.cuda(), "w_dev": w.cuda(),
+            "d": torch.full((sum(counts), n), float("nan"), dtype=torch.bfloat16, device="cuda")}
+
+
+def test_captured_plans_survive_later_set_ups(engine, oracle):
+    """Set-up and launch in a graph, set-ups outside of it, a second graph, replays in any order;
+    a plan that was never set up before, in the default capture mode."""
+    import torch
+
+    first = graph_problem([37, 0, 1, 200], 384, 192, 1)
+    second = graph_problem([90, 5, 260, 31, 0, 777], 256, 320, 2)
+    third = graph_problem([3, 300], 512, 128, 3)
+    warm = engine.GroupedGemmPlan()                    # kernels are loaded outside of captures
+    side = torch.cuda.Stream()
+    plan = engine.GroupedGemmPlan()
+
+    def set_up(problem, stream=None, on=plan):
+        assert on.initialize_packed(problem["a_dev"], problem["w_dev"], problem["d"],
+                                    problem["counts"], stream=stream,
+                                    scheduler="dynamic_queue") == 0
+
+    def capture(problem):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            set_up(problem, side)
+            assert plan.run(side) == 0
+        return graph
+
+    def check(problem):
+        torch.cuda.synchronize()
+        check_against_oracle(oracle, problem["a"], problem["w"], problem["counts"],
+                             bits_of(problem["d"]))
+        problem["d"].fill_(float("nan"))
+        torch.cuda.synchronize()
+
+    def new_input(problem, seed):
+        problem["a"] = make_inputs(problem["counts"], problem["w"].shape[1],
+                                   problem["w"].shape[2], seed)[0]
+        problem["a_dev"].copy_(problem["a"])
+        torch.cuda.synchronize()
+
+    try:
+        set_up(third, on=warm)
+        assert warm.run() == 0
+        check(third)
+        graph = capture(first)
+        assert torch.isnan(first["d"]).all()           # nothing has run yet
+        assert plan.poll()[0] == 0 and len(plan.worklist()) == plan.stats().total_tiles
+        assert plan.run() == 0                         # the captured set-up, before any replay
+        check(first)
+        for seed in (11, 12, 13):
+            new_input(first, seed)
+            graph.replay()
+            check(first)
+            set_up(second)
+            assert plan.run() == 0
+            check(second)
+            set_up(third)
+            assert plan.run() == 0 and plan.poll()[0] == 0
+            check(third)
+        other = capture(second)
+        for seed in (21, 22):
+            new_input(second, seed)
+            other.replay()
+            check(second)
+            new_input(first, seed)
+            graph.replay()
+            check(first)
+            assert plan.run() == 0                     # the set-up of the second graph
+            check(second)
+            assert plan.poll()[0] == 0
+        set_up(third)
+        assert plan.run() == 0
+        check(third)
+        other.replay()
+        graph.replay()
+        check(first), check(second)
+        del graph, other
+    finally:
+        torch.cuda.synchronize()
+        plan.close()
+        warm.close()
+
+
+def test_captured_launch_of_a_set_up_outside_of_the_graph(engine, oracle):
+    """The graph holds run() alone; the plan is set up for other counts afterwards."""
+    import torch
+
+    first = graph_problem([37, 0, 1, 200], 384, 192, 1)
+    second = graph_problem([90, 5, 260, 31, 0, 777], 256, 320, 2)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    plan = engine.GroupedGemmPlan()
+    try:
+        for problem in (second, first):
+            assert plan.initialize_packed(problem["a_dev"], problem["w_dev"], problem["d"],
+                                          problem["counts"], stream=other) == 0
+            assert plan.run(other) == 0
+        graph, fork = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            assert plan.run(side) == 0
+        with torch.cuda.graph(fork, stream=side):      # launches on two streams of a capture
+            assert plan.run(side) == 0
+            other.wait_stream(side)
+            assert plan.run(other) == 0 and plan.run(side) == 0
+            side.wait_stream(other)
+        for replay in (graph.replay, fork.replay, graph.replay):
+            assert plan.initialize_packed(second["a_dev"], second["w_dev"], second["d"],
+                                          second["counts"], stream=other) == 0
+            assert plan.run(other) == 0
+            torch.cuda.synchronize()
+            for problem in (first, second):
+                check_against_oracle(oracle, problem["a"], problem["w"], problem["counts"],
+                                     bits_of(problem["d"]))
+                problem["d"].fill_(float("nan"))
+            torch.cuda.synchronize()
+            replay()
+        torch.cuda.synchronize()
+        check_against_oracle(oracle, first["a"], first["w"], first["counts"], bits_of(first["d"]))
+        assert torch.isnan(second["d"]).all() and plan.poll()[0] == 0
+        del graph, fork
+    finally:
+        torch.cuda.synchronize()
+        plan.close()
+
+
+def test_captured_plan_whose_counts_are_on_the_device(engine, oracle):
+    """A graph's set-up reads the counts of each replay; before the first there are no tiles."""
+    import torch
+
+    n, k, cap = 264, 128, 300
+    w = make_inputs([1] * 4, n, k, 5)[1]
+    a_dev = torch.zeros(cap, k, dtype=torch.bfloat16, device="cuda")
+    counts_dev = torch.zeros(4, dtype=torch.int32, device="cuda")
+    first_dev = torch.zeros(4, dtype=torch.int32, device="cuda")
+    order = torch.arange(cap, device="cuda")
+    out = torch.full((cap, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    bases = torch.tensor([out.data_ptr()], dtype=torch.int64, device="cuda")
+    w_dev, plan, side = w.cuda(), engine.GroupedGemmPlan(), torch.cuda.Stream()
+
+    def step(stream=None):
+        assert plan.initialize_packed_device_counts(a_dev, w_dev, counts_dev.data_ptr(),
+                                                    stream=stream) == 0
+        assert plan.set_push(order.data_ptr(), first_dev.data_ptr(), bases.data_ptr(), 1, cap) == 0
+        assert plan.run(stream) == 0
+
+    try:
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step(side)
+        assert plan.run() == 0 and plan.poll()[0] == 0
+        assert torch.isnan(out).all()
+        for counts in ([33, 0, 190, 7], [0, 0, 0, 0], [1, 250, 3, 4]):
+            a = make_inputs(counts, n, k, 6 + counts[0])[0]
+            a_dev[:sum(counts)].copy_(a)
+            counts_dev.copy_(torch.tensor(counts))
+            first_dev.copy_(torch.tensor(counts).cumsum(0) - torch.tensor(counts))
+            for again in (graph.replay, plan.run):     # and a launch of what the replay set up
+                out.fill_(float("nan"))
+                torch.cuda.synchronize()
+                again()
+                torch.cuda.synchronize()
+                if sum(counts):
+                    check_against_oracle(oracle, a, w, counts, bits_of(out[:sum(counts)]))
+                assert torch.isnan(out[sum(counts):]).all()
+        del graph
+    finally:
+        torch.cuda.synchronize()
+        plan.close()
+
+
 def test_benchmark_shape_properties(engine, oracle, golden):
     """Full-size Mixtral-shaped case: policies bit-identical, sampled rows within
     tolerance of the oracle, every tile run exactly once."""
