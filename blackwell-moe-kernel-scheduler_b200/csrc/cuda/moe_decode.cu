@@ -461,7 +461,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
   constexpr uint32_t kPlanes = DIGITS ? kDigits : 1;   // columns per token
   extern __shared__ uint8_t smem_raw[];
   __shared__ Barriers bars;
-  __shared__ uint32_t tmem_slot, abort_slot;
+  __shared__ uint32_t tmem_slot, abort_slot, spoiled_slot;
   __shared__ uint32_t list_mask[2], list_base, list_expert;   // tokens of the expert
   __shared__ float list_coef[kMaxTokens], channel_scale[2][64];
   __shared__ uint8_t list_token[kMaxTokens];
@@ -515,6 +515,7 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
   } else if (warp == 1) {
     if (lane == 0) {
       abort_slot = 0;
+      spoiled_slot = failed_before(a) ? 1u : 0u;
       init_barriers(bars);
     }
     __syncwarp();
@@ -545,7 +546,6 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
   const uint32_t columns = plane * kPlanes;
   const uint32_t n = (columns + 15) / 16 * 16;     // columns of the MMA
   const Ring<KIND> ring(base, ring_bytes, n);
-  bool spoiled = false;                    // epilogue: the sums of this thread's row
 
   const uint32_t rank = ptx::cluster_cta_rank(), ranks = ptx::cluster_cta_count();
   const uint32_t channel0 = blockIdx.x / ranks * 64;
@@ -660,7 +660,6 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
       if (!ok && lane == 0) report(a, 3);
     }
     // Accumulator -> shared memory [column][row], over the ring: all of its bytes are used.
-    spoiled = warp < 8 && failed_before(a);
     if (warp < 8 && ok && wait(bars.d_full[0], 0)) {
       ptx::tc_fence_after_sync();
       const uint32_t to = base + (quad * 32 + lane) * 4;
@@ -689,15 +688,15 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
         }
       }
       ptx::tc_fence_before_sync();
-    } else if (warp < 8) {
-      spoiled = true;
-      if (lane == 0) report(a, 4);
+    } else if (warp < 8 && lane == 0) {
+      spoiled_slot = 1;
+      report(a, 4);
     }
   }
   __syncwarp();
   if constexpr (DIGITS) ptx::wait_for_previous_grid();   // x_most; and see above
   settle(&abort_slot);
-  if (spoiled) {
+  if (warp >= 4 && warp < 8 && spoiled_slot != 0) {
     // NaN in h, and from there in every output channel of the expert's tokens
     for (uint32_t c = 0; c < plane; ++c) {
       asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + (c * kRows + (warp & 3) * 32 + lane) * 4),
@@ -776,7 +775,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
   constexpr uint32_t kColumns = DIGITS ? 4 * COLS : 2 * COLS;   // of an accumulator
   extern __shared__ uint8_t smem_raw[];
   __shared__ Barriers bars;
-  __shared__ uint32_t tmem_slot, abort_slot, active_count;
+  __shared__ uint32_t tmem_slot, abort_slot, spoiled_slot, active_count;
   const DecodeArgs& a = p.a;
   const uint32_t raw = ptx::smem_addr(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -795,6 +794,7 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
   if (warp == 1) {
     if (lane == 0) {
       abort_slot = 0;
+      spoiled_slot = failed_before(a) ? 1u : 0u;
       init_barriers(bars);
     }
     __syncwarp();
@@ -951,7 +951,6 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
     const uint32_t quad = warp & 3;
     const uint32_t row = quad * 32 + lane;
     float* const mine = sums + row;
-    bool spoiled = failed_before(a);
     Cursor d_buf;
     if constexpr (DIGITS) ptx::wait_for_previous_grid();   // h_most
     for (uint32_t at = begin; at < end;) {
@@ -966,8 +965,10 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
         }
       }
       if (!wait(bars.d_full[d_buf.slot], d_buf.parity)) {
-        if (lane == 0) report(a, 9);
-        spoiled = true;
+        if (lane == 0) {
+          spoiled_slot = 1;
+          report(a, 9);
+        }
         break;
       }
       ptx::tc_fence_after_sync();
@@ -1003,7 +1004,10 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
       d_buf.next(2);
       at += run;
     }
-    for (uint32_t t = 0; spoiled && t < a.tokens; ++t) mine[t * kRows] = not_a_number();
+    __syncwarp();
+    if (spoiled_slot != 0) {
+      for (uint32_t t = 0; t < a.tokens; ++t) mine[t * kRows] = not_a_number();
+    }
   }
   __syncwarp();
   // No thread goes on before the first kernel has ended: out may be x, and this grid must
