@@ -12,7 +12,11 @@
 //   warp 1     MMA issuer (one elected lane), Tensor Memory
 //   warps 4-7  epilogue
 // BF16 weights: h keeps 16 significant bits as two BF16 numbers whose products are added: the
-// upper and the lower halves of the tokens are separate columns of the same MMA.
+// upper and the lower halves of the tokens are separate columns of the same MMA. What that leaves
+// out (2.5e-6 of the result in norm) is about what the MMA's own FP32 sums do (2.1e-6 over 2048
+// products, 4.4e-6 over 4096, 1.6e-5 over 14336 in one accumulator; a BF16 result's half
+// step is 3.9e-3): a third BF16 number would cost half as many activation bytes again for less
+// than that.
 // INT8 weights are multiplied in one of two ways (use_digits has the rule and what it measured):
 //   as they are, against activations written as fixed-point numbers of three signed bytes. The
 //   digits of a token are three columns of the same MMA, its sums are exact 32-bit integers.
@@ -27,8 +31,10 @@
 //
 // Measured on B200 (us of device time in a CUDA graph, inputs past L2; share of the 6.55 TB/s a
 // copy reaches): hidden 4096, inter 14336, two of 8 experts, T=1: 112 BF16 (96 %), 65 INT8 (83 %);
-// all 8, T=16: 370 BF16 (1.02), T=64: 449 BF16 (96 %), 256 INT8 (84 %). 128 experts of 2048 x
-// 768, top-8: T=1 22.3 BF16 (52 %), T=32 142 (90 %). hidden 512, inter 1024, T=1: 9.7 (latency
+// all 8 hit, T=16: 444-456 BF16 (94-97 %), 226 INT8 (95 %), T=64: 448 BF16 (96 %), 254 INT8 (85 %).
+// 128 experts of 2048 x 768, top-8: T=1 22.6 BF16 (51 %), T=32 143 (90 %). INT8 that is converted,
+// 64 tokens on one expert of (4096, 14336): 65 (41 %), on each of two: 111 (48 %). (Of one GPU;
+// others of the same kind, and long runs at the 1000 W limit, take up to 8 % longer.) hidden 512, inter 1024, T=1: 9.7 (latency
 // of two dependent launches). Fragments loaded straight into registers for mma.sync, the first
 // version, took 178 us for T=1, 848 for T=32 and 1227 for T=64 in INT8.
 // One grid that fills the GPU once with an equal share of blocks per CTA was tried for the
@@ -226,11 +232,11 @@ __device__ __forceinline__ bool issue_blocks(const Wait& wait, Barriers& bars,
 
 // INT8: one warp's 32 rows of every second of `blocks` k-blocks (`turn` 0 or 1, and that buffer)
 // from shared memory to Tensor Memory as BF16. Two groups of four warps take turns, since most
-// of a block's time in a warp is latency. The conversion is what keeps INT8 layers at 72-76 %
-// of the copy bandwidth: without it (wrong results, streaming only) the same kernels reach
-// 85-87 %. With it the integer pipe is busy 56 % of the time at 4.5 TB/s and the issue slots
-// 49 % (one token); fewer integer operations (see int8_pairs), four groups instead of two and
-// converting ahead of the free buffer all measured within 1 %.
+// of a block's time in a warp is latency. The conversion costs a large layer of few tokens 72-76
+// instead of 85-87 % of the copy bandwidth (hence the digits, which leave it the small layers and
+// the crowded experts): the integer pipe is busy 56 % of the time at 4.5 TB/s and the issue
+// slots 49 % (one token). Fewer integer operations (see int8_pairs), four groups instead of two
+// and converting ahead of the free buffer all measured within 1 %.
 //
 // The buffer is waited for before the stage. With an odd number of stages the two groups use a
 // slot in turn, so a group has not seen the slot's use before its own, and a wait by parity
@@ -369,7 +375,7 @@ __device__ __forceinline__ void load16(const float* from, float (&v)[16]) {
 // smaller ones are off by half a unit at most, 2^-22 of the largest. Three digits because two
 // (2^-14) would be coarser than BF16 itself and four cost the MMA, the ring and the SM's intake
 // a third more. A row with a NaN or an infinity has the unit NaN; e >= -100 keeps the factor
-// 1 / unit finite, and a row of zeros zero.
+// 1 / unit finite, and a row of zeros zero (rows whose largest is below 2^-100 have the unit 2^-121).
 __device__ __forceinline__ uint32_t digit_exponent(uint32_t most) {   // e + 127
   return min(max(most >> 23, 27u), 254u);
 }

@@ -950,7 +950,7 @@ uint64_t bmoe_moe_decode_workspace(uint32_t tokens, uint32_t top_k, uint32_t int
  * 16 significant bits or more, one BF16 rounding at the end; INT8 weights are multiplied
  * as the integers they are and scaled per output channel in FP32. Where INT8 weights outweigh
  * two more launches, the rows of x and h become fixed-point numbers whose last place is 2^-22 of
- * the row's largest magnitude or less, and their sums with the weights are exact; a row of x
+ * the row's largest magnitude or less (2^-121 at least), and their sums with the weights are exact; a row of x
  * or h with a NaN or an infinity then makes its token's output NaN. An expert that a token
  * names twice counts with the sum of both weights. Dropped assignments contribute nothing;
  * a token with nothing else gets a row of zeros. Results do not depend on the run. x, the weights and out are 16-byte aligned, the rest as their types. out may be x.
