@@ -77,10 +77,6 @@ struct PinnedBlock {
 
 bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
-}  // namespace
-
-namespace {
-
 // Where a call enqueues its work: a stream, or one of the streams of a capture. Streams are
 // told apart by their ids (a handle may come back after its stream was destroyed), those of one
 // capture by their handles (asking one for its id ends the capture).

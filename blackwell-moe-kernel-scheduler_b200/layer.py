@@ -3,8 +3,9 @@
 
 Thin wrappers of the C entry points (``include/bmoe_b200.h``, section 6). Each allocates the
 outputs it is not given, launches on ``stream`` (default: the current stream of the tensors'
-device) and does not synchronise; what it allocates belongs to that stream. There is no backward
-pass: with gradients enabled, inputs that require one are refused. Wrong shapes, types or
+device) and does not synchronise; what it allocates belongs to that stream. Inputs, and outputs
+that are given, stay the caller's, who keeps them until the launch has run where they belong to
+another stream. There is no backward pass: with gradients enabled, inputs that require one are refused. Wrong shapes, types or
 devices raise ``ValueError``, a status of the engine raises ``EngineError``. The reference has
 no counterpart: routed token counts are its input (agent/search_space.yaml:10-13).
 """
