@@ -304,7 +304,8 @@ __device__ __forceinline__ void settle(volatile uint32_t* abort_word) {
 }
 
 // The word at the same shared-memory address of every CTA of the cluster, summed in the order
-// of their ranks; all loads are in flight together.
+// of their ranks; all loads are in flight together. The sum has to be used before the cluster's
+// last barrier: a load that nobody waits for could still be under way when its CTA is gone.
 __device__ __forceinline__ float sum_over_cluster(uint32_t address, uint32_t ranks) {
   float part[8];
   if (ranks == 1) {
@@ -725,7 +726,11 @@ decode_up_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) {
     const bool inside = channel < a.inter;
     if (!DIGITS && !inside) continue;
     const uint32_t cell = base + ((gather ? at : list_token[at] - token0) * kRows + c) * 4;
-    float gate = sum_over_cluster(cell, ranks), up = sum_over_cluster(cell + 64 * 4, ranks);
+    float gate = 0.0f, up = 0.0f;
+    if (inside) {
+      gate = sum_over_cluster(cell, ranks);
+      up = sum_over_cluster(cell + 64 * 4, ranks);
+    }
     if constexpr (INT8) {
       const float unit = DIGITS ? digit_unit(a.x_most[list_token[at]]) : 1.0f;
       gate *= channel_scale[0][c] * unit;
@@ -1030,8 +1035,8 @@ decode_down_kernel(const __grid_constant__ DecodeParams p, uint32_t ring_bytes) 
   const uint32_t sums_smem = ptx::smem_addr(sums);
   for (uint32_t i = rank * kThreads + threadIdx.x; i < a.tokens * kRows; i += ranks * kThreads) {
     const uint32_t channel = channel0 + i % kRows;
-    const float sum = sum_over_cluster(sums_smem + i * 4, ranks);
     if (channel < a.hidden) {
+      const float sum = sum_over_cluster(sums_smem + i * 4, ranks);
       a.out[static_cast<size_t>(i / kRows) * a.hidden + channel] = to_bf16(sum);
     }
   }

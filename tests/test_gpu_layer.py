@@ -725,6 +725,21 @@ def test_moe_decode_digits_of_rows_with_a_wide_range(engine):
     assert not torch.isfinite(got[6:]).any()
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("tokens", [1, 4, 18])
+def test_moe_decode_last_tiles_of_few_channels(engine, tokens, int8):
+    """Tiles split over a cluster whose last 16 channels leave whole warps without any."""
+    layer = big_layer(tokens, 2, 2, 2064, 3088, int8, seed=tokens)
+    want, bound = big_layer_oracle(layer)
+    if int8:
+        cpu = {name: t.cpu() for name, t in layer.items()}
+        bound = digit_bound(cpu, bound.cpu()).cuda()
+    got = engine.moe_decode(layer["x"], layer["w1"], layer["w2"], layer["ids"], layer["coef"],
+                            gate_up_scale=layer["s1"], down_scale=layer["s2"])
+    off = (got.double() - want).abs()
+    assert torch.all(off <= bound), (off / bound).max()
+
+
 def test_moe_decode_digits_that_do_not_fit_beside_h(engine):
     """hidden > top_k * inter: the weights are converted instead."""
     check_layer(engine, make_layer(20, 64, 1, 4000, 160, True, seed=8))
